@@ -409,6 +409,44 @@ int amdseg_heads_bwd_rows(const float* gout, const float* x, int M, int H, float
  * would cost all fp32 digits of (mask - lse) in rows whose visible keys are all masked).  exp() of a masked score is an exact 0 next to
  * any real score either way, which is what the reference's finfo.min mask yields. */
 
+/* ---- attention under a learned relative position bias (csrc/relpos_fwd.hip, relpos_bwd.hip, relpos_bias.hip) ----------------------------------
+ *   s_ij = scale q_i . k_j + table[map[clamp(rel, -span, span) + span], head],   rel = j - (i + off),   off = 0 or (align_end) keys - queries of the sequence
+ *   p_ij = softmax over the visible keys;  out_i = sum_j p_ij v_j;  lse_i = log sum_j exp(s_ij)
+ * Key j is visible from query i iff j < keys of the sequence, key_mask (optional, 0 = hidden) allows it and, with `causal`, rel <= 0.  A row without a
+ * visible key: out = 0, lse = -inf, no gradient.  K / V rows of hidden keys are never used, whatever they hold.
+ * Padded form (cu_q == cu_k == NULL): B sequences of Lq query and Lk key rows; k_lens (optional, int32 [B]) = keys held of each (a cache).
+ * Packed form: sequence b = rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. of k (int32 [B + 1], device); Tq, Tk = rows of the buffers, Lq, Lk = the longest
+ * sequence (a launch hint: too small a value costs time, not rows).  Rows outside every sequence: written as zeros (lse -inf) with zero_tail, else left alone.
+ * Values of cu_* / k_lens / map out of range are clamped on the device: wrong rows, never an access outside the buffers.
+ * Strides are in elements, {sequence, row, head}, the last dimension contiguous; rows start on 16 bytes (pointers and strides).  heads a multiple of
+ * kv_heads (each kv head serves heads / kv_heads query heads), D % 8 == 0, D <= 128, span <= 1024.  dtype: AMDSEG_BF16 or AMDSEG_F32 (products of
+ * fp32 tensors in exact fp32); table_dtype independent; softmax, lse and every sum fp32.
+ * lse: [B, heads, Lq] or, packed, [heads, Tq]; may be NULL in forward.  Backward: dq, dk, dv (strides of their own), dtable [buckets, heads] in
+ * table_dtype (NULL: not computed); sums are taken in a fixed order (bit-reproducible), gradients of shared kv heads include all their query heads.
+ * ws: amdseg_relpos_attn_ws_bytes(cfg, backward) bytes of scratch on 16 bytes (0 bytes: NULL allowed). */
+struct amdseg_relpos_cfg {
+    int32_t dtype, table_dtype, B, Lq, Lk, Tq, Tk, heads, kv_heads, D, span, buckets, causal, align_end, zero_tail;
+    float scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+    const int32_t *cu_q, *cu_k, *k_lens;
+    const uint8_t* key_mask;                /* [B, Lk], rows mask_stride bytes apart; packed: [Tk] */
+    int64_t mask_stride;
+    const int32_t* map;                     /* [2 span + 1] */
+    const void* table;                      /* [buckets, heads] */
+};
+size_t amdseg_relpos_attn_ws_bytes(const struct amdseg_relpos_cfg* cfg, int backward);
+int amdseg_relpos_attn_fwd(const struct amdseg_relpos_cfg* cfg, const void* q, const void* k, const void* v, void* out, float* lse, void* ws,
+                           size_t ws_bytes, amdseg_stream_t stream);
+int amdseg_relpos_attn_bwd(const struct amdseg_relpos_cfg* cfg, const void* q, const void* k, const void* v, const void* out, const void* dout,
+                           const float* lse, void* dq, void* dk, void* dv, void* dtable, void* ws, size_t ws_bytes, amdseg_stream_t stream);
+/* the bias as a dense tensor [heads, Lq, Lk] (query row i stands at position i + q_offset) and the gradient of the table, fp32 [buckets, heads], from the
+ * gradient of that tensor for each of B sequences [B, heads, Lq, Lk] (summed over them).  All contiguous, tensors on 16 bytes. */
+int amdseg_relpos_bias_fwd(const void* table, int table_dtype, const int32_t* map, int span, int buckets, int heads, int Lq, int Lk, int q_offset,
+                           void* out, int dtype, amdseg_stream_t stream);
+size_t amdseg_relpos_bias_ws_bytes(int B, int heads, int Lq, int span);
+int amdseg_relpos_bias_bwd(const void* dbias, int dtype, const int32_t* map, int span, int buckets, int B, int heads, int Lq, int Lk, int q_offset,
+                           float* dtable, void* ws, size_t ws_bytes, amdseg_stream_t stream);
+
 /* ---- the explicit library context (ABI 13; csrc/prof.hip).  EVERYTHING libamdseg remembers between two calls lives in an amdseg_ctx the
  * caller creates: (1) the CU budget of the launch-geometry rules -- a process whose backward overlaps an RCCL all-reduce sets it to (CUs - RCCL
  * channels): the GEMM tile width is chosen by rounds of workgroups against this number (a 256-tile grid on 240 free CUs is two rounds);

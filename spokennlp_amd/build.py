@@ -11,7 +11,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
-SOURCES = ["gemm.hip", "gemm_dp.hip", "attention.hip", "attention_split.hip", "elementwise.hip", "optim.hip", "gemm_f32.hip", "longformer.hip", "ponet.hip", "ponet_global.hip", "prof.hip", "parity.hip", "heads.hip", "lf_global.hip", "comm.hip", "api.hip"]
+SOURCES = ["gemm.hip", "gemm_dp.hip", "attention.hip", "attention_split.hip", "elementwise.hip", "optim.hip", "gemm_f32.hip", "longformer.hip", "ponet.hip", "ponet_global.hip", "prof.hip", "parity.hip", "heads.hip", "lf_global.hip", "comm.hip", "relpos_fwd.hip", "relpos_bwd.hip", "relpos_bias.hip", "api.hip"]
 OUT = os.path.join(HERE, "libamdseg.so")
 # -packed-fp32-ops: no v_pk_add / v_pk_mul / v_pk_fma_f32, neither from float2 code nor by the vectoriser: some of their forms have given wrong results
 # now and then on this hardware, silently.  (The host pass does not know the feature and says so: harmless.)

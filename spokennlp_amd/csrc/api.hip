@@ -3,6 +3,7 @@
 #include "amdseg_internal.h"
 #include <algorithm>
 #include "common.h"
+#include "relpos_launch.h"
 #include "keepmask.h"      // km_pairs_with_rows: where layer li + 1's keep masks ride in layer li's LayerNorm launch
 
 #define S(x) ((hipStream_t)(x))
@@ -673,4 +674,104 @@ int amdseg_bert_layer_bwd(const amdseg_bert_cfg* c, const amdseg_bert_layer_para
     return AMDSEG_OK;
 }
 
+// ---- attention under a learned relative position bias (csrc/relpos_*.hip)
+static bool relpos_rows_ok(const void* p, const int64_t st[3], int esize, bool empty) {
+    return (empty || p) && !((uintptr_t)p & 15) && !((st[0] | st[1] | st[2]) * esize & 15);
+}
+static int relpos_args(const struct amdseg_relpos_cfg* c, RpArgs& a) {
+    if (!c || (c->dtype != AMDSEG_BF16 && c->dtype != AMDSEG_F32) || (c->table_dtype != AMDSEG_BF16 && c->table_dtype != AMDSEG_F32)) return AMDSEG_ERR_ARG;
+    if (!c->map || !c->table || (c->cu_q == nullptr) != (c->cu_k == nullptr) || (c->cu_q && c->k_lens)) return AMDSEG_ERR_ARG;
+    if (!(c->scale > 1e-6f && c->scale < 1e6f)) return AMDSEG_ERR_ARG;
+    const int lim = 1 << 30;
+    if (c->B < 0 || c->Lq < 0 || c->Lk < 0 || c->Tq < 0 || c->Tk < 0 || c->B > lim || c->Lq > lim || c->Lk > lim || c->Tq > lim || c->Tk > lim) return AMDSEG_ERR_SHAPE;
+    if (c->heads < 1 || c->heads > 65535 || c->kv_heads < 1 || c->heads % c->kv_heads || c->D < 8 || c->D > 128 || c->D % 8 || c->span < 0 ||
+        c->span > RP_MAX_SPAN || c->buckets < 1 || c->buckets > (1 << 20)) return AMDSEG_ERR_SHAPE;
+    if (c->cu_q && ((c->Tq > 0 && c->Lq < 1) || (c->Tk > 0 && c->Lk < 1))) return AMDSEG_ERR_SHAPE;
+    a = RpArgs{};
+    auto st = [](const int64_t* x) { return RpTensor{x[0], x[1], x[2]}; };
+    a.sq = st(c->q_stride); a.sk = st(c->k_stride); a.sv = st(c->v_stride); a.so = st(c->out_stride); a.sdo = st(c->dout_stride);
+    a.sdq = st(c->dq_stride); a.sdk = st(c->dk_stride); a.sdv = st(c->dv_stride);
+    if (c->cu_q) a.sq.sb = a.sk.sb = a.sv.sb = a.so.sb = a.sdo.sb = a.sdq.sb = a.sdk.sb = a.sdv.sb = 0;
+    a.cu_q = c->cu_q; a.cu_k = c->cu_k; a.k_lens = c->k_lens; a.key_mask = c->key_mask; a.mask_sb = c->mask_stride;
+    a.map = c->map; a.table = c->table; a.table_bf16 = c->table_dtype == AMDSEG_BF16;
+    a.B = c->B; a.Lq = c->Lq; a.Lk = c->Lk; a.heads = c->heads; a.kv_heads = c->kv_heads; a.D = c->D; a.Tq = c->Tq; a.Tk = c->Tk;
+    a.span = c->span; a.buckets = c->buckets; a.causal = c->causal != 0; a.align_end = c->align_end != 0; a.zero_tail = c->cu_q && c->zero_tail;
+    a.scale = c->scale; a.nsplit = 1;
+    return AMDSEG_OK;
+}
+static size_t relpos_up(size_t n) { return (n + 255) / 256 * 256; }
+static size_t relpos_rows(const RpArgs& a) { return a.cu_q ? (size_t)a.heads * a.Tq : (size_t)a.B * a.heads * a.Lq; }
+static size_t relpos_bwd_ws(const RpArgs& a, int dtype, size_t* sums_at, size_t* part_at) {
+    const size_t nd = 2 * ((size_t)a.span + RP_PAD) + 1, bk = 64 * rp_dkv_qt(a, dtype), nrb = (a.Lk + bk - 1) / bk;
+    *sums_at = relpos_up(4 * relpos_rows(a));
+    *part_at = *sums_at + relpos_up(4 * nd * a.heads);
+    return *part_at + relpos_up(4 * nd * a.heads * a.B * nrb);
+}
+size_t amdseg_relpos_attn_ws_bytes(const struct amdseg_relpos_cfg* c, int backward) {
+    RpArgs a;
+    if (relpos_args(c, a)) return 0;
+    size_t x, y;
+    if (backward) return relpos_bwd_ws(a, c->dtype, &x, &y);
+    const size_t n = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
+    return n > 1 ? n * relpos_rows(a) * (a.D + 2) * 4 : 0;
+}
+int amdseg_relpos_attn_fwd(const struct amdseg_relpos_cfg* c, const void* q, const void* k, const void* v, void* out, float* lse, void* ws,
+                           size_t ws_bytes, amdseg_stream_t stream) {
+    RpArgs a;
+    RET_IF(relpos_args(c, a));
+    const int es = c->dtype == AMDSEG_F32 ? 4 : 2;
+    const bool noq = (a.cu_q ? a.Tq : a.Lq) == 0 || (a.B == 0 && !a.cu_q), nok = (a.cu_q ? a.Tk : a.Lk) == 0;
+    if (noq) return AMDSEG_OK;
+    if (!relpos_rows_ok(q, c->q_stride, es, false) || !relpos_rows_ok(k, c->k_stride, es, nok) || !relpos_rows_ok(v, c->v_stride, es, nok) ||
+        !relpos_rows_ok(out, c->out_stride, es, false)) return AMDSEG_ERR_ARG;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse;
+    a.nsplit = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
+    if (a.nsplit > 1) {
+        if (!ws || ((uintptr_t)ws & 15) || ws_bytes < amdseg_relpos_attn_ws_bytes(c, 0)) return AMDSEG_ERR_ARG;
+        a.part_o = (float*)ws;
+        a.part_ml = a.part_o + (size_t)a.nsplit * relpos_rows(a) * a.D;
+    }
+    return amdseg_relpos_fwd_impl(a, c->dtype, S(stream));
+}
+int amdseg_relpos_attn_bwd(const struct amdseg_relpos_cfg* c, const void* q, const void* k, const void* v, const void* out, const void* dout,
+                           const float* lse, void* dq, void* dk, void* dv, void* dtable, void* ws, size_t ws_bytes, amdseg_stream_t stream) {
+    RpArgs a;
+    RET_IF(relpos_args(c, a));
+    const int es = c->dtype == AMDSEG_F32 ? 4 : 2;
+    const bool noq = (a.cu_q ? a.Tq : a.Lq) == 0 || (a.B == 0 && !a.cu_q), nok = (a.cu_q ? a.Tk : a.Lk) == 0 || (a.B == 0 && !a.cu_q);
+    if (!relpos_rows_ok(q, c->q_stride, es, noq) || !relpos_rows_ok(k, c->k_stride, es, nok) || !relpos_rows_ok(v, c->v_stride, es, nok) ||
+        !relpos_rows_ok(out, c->out_stride, es, noq) || !relpos_rows_ok(dout, c->dout_stride, es, noq) || !relpos_rows_ok(dq, c->dq_stride, es, noq) ||
+        !relpos_rows_ok(dk, c->dk_stride, es, nok) || !relpos_rows_ok(dv, c->dv_stride, es, nok) || (!noq && !lse)) return AMDSEG_ERR_ARG;
+    size_t sums_at, part_at;
+    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < relpos_bwd_ws(a, c->dtype, &sums_at, &part_at)) return AMDSEG_ERR_ARG;
+    a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.lse = (float*)lse; a.dq = dq; a.dk = dk; a.dv = dv;
+    a.delta = (float*)ws;
+    a.part_d = dtable ? (float*)((char*)ws + part_at) : nullptr;
+    return amdseg_relpos_bwd_impl(a, c->dtype, dtable, (float*)((char*)ws + sums_at), S(stream));
+}
+static bool relpos_bias_ok(int dtype, const int32_t* map, int span, int buckets, int B, int heads, int Lq, int Lk, int q_offset) {
+    const int lim = 1 << 30;
+    return (dtype == AMDSEG_BF16 || dtype == AMDSEG_F32) && map && span >= 0 && span <= RP_MAX_SPAN && buckets >= 1 && buckets <= (1 << 20) && B >= 0 &&
+           B <= 65535 && heads >= 1 && heads <= 65535 && Lq >= 0 && Lq <= lim && Lk >= 0 && Lk <= lim - 1024 && q_offset > -lim / 2 && q_offset < lim / 2;
+}
+int amdseg_relpos_bias_fwd(const void* table, int table_dtype, const int32_t* map, int span, int buckets, int heads, int Lq, int Lk, int q_offset,
+                           void* out, int dtype, amdseg_stream_t stream) {
+    if (!relpos_bias_ok(dtype, map, span, buckets, 1, heads, Lq, Lk, q_offset) || !table || (table_dtype != AMDSEG_BF16 && table_dtype != AMDSEG_F32)) return AMDSEG_ERR_ARG;
+    if (Lq == 0 || Lk == 0) return AMDSEG_OK;
+    if (!out || ((uintptr_t)out & 15)) return AMDSEG_ERR_ARG;
+    RpArgs a{};
+    a.map = map; a.table = table; a.table_bf16 = table_dtype == AMDSEG_BF16; a.span = span; a.buckets = buckets; a.heads = heads; a.Lq = Lq; a.Lk = Lk; a.out = out;
+    return amdseg_relpos_bias_fwd_impl(a, q_offset, dtype, S(stream));
+}
+size_t amdseg_relpos_bias_ws_bytes(int B, int heads, int Lq, int span) {
+    return B < 0 || heads < 1 || Lq < 0 || span < 0 ? 0 : amdseg_relpos_bias_ws_impl(B, heads, Lq, span);
+}
+int amdseg_relpos_bias_bwd(const void* dbias, int dtype, const int32_t* map, int span, int buckets, int B, int heads, int Lq, int Lk, int q_offset,
+                           float* dtable, void* ws, size_t ws_bytes, amdseg_stream_t stream) {
+    if (!relpos_bias_ok(dtype, map, span, buckets, B, heads, Lq, Lk, q_offset) || !dtable || !ws || ((uintptr_t)ws & 15) ||
+        ws_bytes < amdseg_relpos_bias_ws_bytes(B, heads, Lq, span)) return AMDSEG_ERR_ARG;
+    const bool none = B == 0 || Lq == 0 || Lk == 0;
+    if (!none && (!dbias || ((uintptr_t)dbias & 15))) return AMDSEG_ERR_ARG;
+    return amdseg_relpos_bias_bwd_impl(dbias, dtype, map, span, buckets, none ? 0 : B, heads, Lq, Lk, q_offset, dtable, (float*)ws, S(stream));
+}
 }  // extern "C"

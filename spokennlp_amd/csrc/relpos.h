@@ -1,0 +1,202 @@
+// Shared by the kernels of attention under a learned relative position bias (relpos_fwd.hip, relpos_bwd.hip): arguments, [64 rows] LDS tiles of both
+// element types, fragment products, key visibility, the bias table of a workgroup.
+//
+//   s_ij = scale q_i . k_j + table[map[clamp(rel, -span, span) + span], h],   rel = j - (i + off)
+//
+// The bias depends on (i, j) through rel alone, so it is no [Lq, Lk] operand but a vector of 2 span + 1 floats per head.  A workgroup writes it into LDS
+// once, extended by RP_PAD copies of the end values on both sides: a 64-row tile that touches |rel| < span then indexes without clamping, and a tile
+// wholly beyond one end (almost all of a long sequence) starts from a constant and costs nothing.  It is kept divided by `scale`: MFMA accumulators START from
+// it and scale * log2 e multiplies the finished score inside the exponent's fma.
+#pragma once
+#include <math.h>
+#include "common.h"
+#include "tile64.h"
+
+#define RP_PAD 112              // 63 (tile rows) + 32 (columns of a wave) + 15 lanes of the gradient's diagonal registers
+#define RP_MAX_SPAN 1024
+#define RP_SPLIT_KEYS 512       // keys of one split of the few-rows form
+#define RP_LOG2E 1.4426950408889634f
+#define RP_LN2 0.6931471805599453f
+
+struct RpTensor { int64_t sb, st, sh; };     // element strides: sequence, token, head (last dimension contiguous)
+
+struct RpArgs {
+    const void *q, *k, *v; void* out; float* lse;
+    const void *o, *dout; void *dq, *dk, *dv;
+    RpTensor sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    const int *cu_q, *cu_k, *k_lens; const uint8_t* key_mask; int64_t mask_sb;
+    const int* map; const void* table; int table_bf16;
+    int B, Lq, Lk, heads, kv_heads, D, Tq, Tk, span, buckets, causal, align_end, zero_tail;
+    float scale;
+    int nrb;                    // row blocks of a sequence (grid); a workgroup steps by it, so a wrong `longest` hint costs time, never rows
+    int nsplit;                 // forward: splits over the keys
+    float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
+    float* delta;               // backward: sum_j p_ij dp_ij
+    float* part_d;              // backward: [heads][B * nrb][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
+};
+
+// one sequence: where its rows start and how many there are.  The values of cu_q / cu_k / k_lens come from device memory that the host has not seen:
+// they are clamped to the buffers here, so a wrong one gives wrong rows but no access outside.
+struct RpSeq { int q0, qn, k0, kn, off; };
+__device__ __forceinline__ int rp_clamp(int x, int lo, int hi) { return min(max(x, lo), hi); }
+__device__ __forceinline__ RpSeq rp_seq(const RpArgs& a, int b) {
+    RpSeq s;
+    if (a.cu_q) {
+        s.q0 = rp_clamp(a.cu_q[b], 0, a.Tq); s.qn = rp_clamp(a.cu_q[b + 1], s.q0, a.Tq) - s.q0;
+        s.k0 = rp_clamp(a.cu_k[b], 0, a.Tk); s.kn = rp_clamp(a.cu_k[b + 1], s.k0, a.Tk) - s.k0;
+    } else {
+        s.q0 = 0; s.qn = a.Lq; s.k0 = 0;
+        s.kn = a.k_lens ? rp_clamp(a.k_lens[b], 0, a.Lk) : a.Lk;
+    }
+    s.off = a.align_end ? s.kn - s.qn : 0;
+    return s;
+}
+// index of (sequence b, head h, row i) in lse / delta
+__device__ __forceinline__ int64_t rp_row(const RpArgs& a, const RpSeq& s, int b, int h, int i) {
+    return a.cu_q ? (int64_t)h * a.Tq + s.q0 + i : ((int64_t)b * a.heads + h) * a.Lq + i;
+}
+
+// workgroup id -> (row block, head, sequence).  The row blocks (and the heads of a group) that stream the same K / V go to ONE XCD (ids are dealt round
+// robin over the 8), so that its L2 fetches them once; with a number of (sequence, kv head) pairs that is no multiple of 8 the plain order balances better.
+__device__ __forceinline__ void rp_place(int id, int nrb, int B, int heads, int kv_heads, int& rb, int& h, int& b) {
+    const int pairs = B * kv_heads, G = heads / kv_heads;
+    int pair, rest;
+    if ((pairs & 7) == 0) {
+        const int t = id >> 3;
+        pair = (t / (nrb * G)) * 8 + (id & 7); rest = t % (nrb * G);
+    } else { pair = id / (nrb * G); rest = id % (nrb * G); }
+    b = pair / kv_heads;
+    h = (pair % kv_heads) * G + rest / nrb;
+    rb = rest % nrb;
+}
+
+// ------------------------------------------------------------------------------------------------ tiles and products
+// RpTile<T, DT>: [64 rows][DT * 16 columns] in LDS.  A row fragment is the operand whose contraction runs along the columns (K of S^T = K Q^T), a
+// column fragment the one whose contraction runs along the rows (V^T of O^T = V^T P^T).  PF(): accumulator registers of the score tiles as the other
+// operand of that product -- the row order inside a contraction step is the accumulators' own, so the probabilities never move between lanes.
+template <typename T, int DT> struct RpTile;
+template <int DT> struct RpTile<bf16_t, DT> {
+    typedef bf16x8 frag;
+    static constexpr int BYTES = ((DT + 3) / 4) * 8192, KB = DT / 2, EPU = 8, UNITS = DT * 2;   // units = 16 bytes of a row
+    static constexpr int KSTEP = 32, RPS = 2;                                                   // rows of a contraction step, 16-row tiles of it
+    static __device__ __forceinline__ char* at(char* t, int row, int c) { return t + (c >> 3) * 8192 + row * 128 + (((c & 7) ^ swz(row)) << 4); }
+    static __device__ __forceinline__ frag rowf(const char* t, int row, int kb, int g) { return at_frag(t + (kb >> 1) * 8192, row, (kb & 1) * 4 + g); }
+    static __device__ __forceinline__ frag colf(const char* t, int step, int dt, int l) {
+        const int g = l >> 4;
+        return at_frag_tr(t + (dt >> 2) * 8192, step * 32 + g * 4, step * 32 + 16 + g * 4, (dt & 3) * 16, l);
+    }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ frag pf(const f32x4* s) { return pack8(s[0], s[1]); }
+    // the columns kb * 32 + g * 8 .. + 7 of one row of a global tensor, zero beyond D
+    static __device__ __forceinline__ frag gfrag(const bf16_t* row, int kb, int g, int D, bool ok) {
+        frag f = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (ok && kb * 32 + g * 8 < D) f = *reinterpret_cast<const frag*>(row + kb * 32 + g * 8);
+        return f;
+    }
+    static __device__ __forceinline__ float dot(frag a, frag b) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += bf2f((bf16_t)a[e]) * bf2f((bf16_t)b[e]);
+        return s;
+    }
+    static __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
+};
+template <int DT> struct RpTile<float, DT> {
+    typedef f32x4 frag;
+    static constexpr int BYTES = 64 * DT * 64, KB = DT, EPU = 4, UNITS = DT * 4;
+    static constexpr int KSTEP = 16, RPS = 1;
+    static __device__ __forceinline__ char* at(char* t, int row, int c) { return t + row * (DT * 64) + ((c ^ (row & 7)) << 4); }
+    static __device__ __forceinline__ frag rowf(const char* t, int row, int kb, int g) {
+        return *reinterpret_cast<const frag*>(t + row * (DT * 64) + (((kb * 4 + g) ^ (row & 7)) << 4));
+    }
+    static __device__ __forceinline__ frag colf(const char* t, int step, int dt, int l) {
+        const int g = l >> 4, i16 = l & 15;
+        frag f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = step * 16 + g * 4 + r;
+            f[r] = *reinterpret_cast<const float*>(t + row * (DT * 64) + (((dt * 4 + (i16 >> 2)) ^ (row & 7)) << 4) + (i16 & 3) * 4);
+        }
+        return f;
+    }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ frag pf(const f32x4* s) { return s[0]; }
+    static __device__ __forceinline__ frag gfrag(const float* row, int kb, int g, int D, bool ok) {
+        frag f = {0.f, 0.f, 0.f, 0.f};
+        if (ok && kb * 16 + g * 4 < D) f = *reinterpret_cast<const frag*>(row + kb * 16 + g * 4);
+        return f;
+    }
+    static __device__ __forceinline__ float dot(frag a, frag b) { return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]; }
+    static __device__ __forceinline__ void st4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+};
+
+// 64 rows of a tensor global -> registers -> LDS by a workgroup of 256.  Rows whose bit is clear and columns from D on become zeros: what stands in
+// masked rows (infinities, NaN) reaches no product.
+template <typename T, int DT> struct RpStage {
+    typedef RpTile<T, DT> Ti;
+    static constexpr int N = 64 * Ti::UNITS / 256;
+    uint4 r[N];
+    __device__ __forceinline__ void load(const T* base, int64_t st, uint64_t bits, int D, int tid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = n * 256 + tid, row = u / Ti::UNITS, c = u % Ti::UNITS;
+            r[n] = make_uint4(0u, 0u, 0u, 0u);
+            if (((bits >> row) & 1) && c * Ti::EPU < D) r[n] = *reinterpret_cast<const uint4*>(base + row * st + c * Ti::EPU);
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = n * 256 + tid;
+            *reinterpret_cast<uint4*>(Ti::at(tile, u / Ti::UNITS, u % Ti::UNITS)) = r[n];
+        }
+    }
+};
+
+// visible keys of a 64-key chunk as a wave-uniform word; the mask byte of the chunk after it is in flight
+struct RpKeys {
+    const uint8_t* m; int kn, lane; uint32_t nxt;
+    __device__ __forceinline__ uint32_t byte(int c) const {
+        const int key = c * 64 + lane;
+        return key < kn ? (m ? (uint32_t)m[key] : 1u) : 0u;
+    }
+    __device__ __forceinline__ void init(const RpArgs& a, const RpSeq& s, int b, int lane_, int c) {
+        m = a.key_mask ? a.key_mask + (a.cu_k ? (int64_t)s.k0 : (int64_t)b * a.mask_sb) : nullptr;
+        kn = s.kn; lane = lane_; nxt = byte(c);
+    }
+    __device__ __forceinline__ uint64_t next(int c) {       // the word of chunk c; the loads of chunk c + 1 go out
+        const uint64_t w = __ballot(nxt != 0);
+        nxt = byte(c + 1);
+        return w;
+    }
+};
+__device__ __forceinline__ uint64_t rp_low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+__device__ __forceinline__ float rp_table(const RpArgs& a, int rel, int h) {
+    const int bk = rp_clamp(a.map[rp_clamp(rel, -a.span, a.span) + a.span], 0, a.buckets - 1);
+    const int64_t at = (int64_t)bk * a.heads + h;
+    return a.table_bf16 ? bf2f(((const bf16_t*)a.table)[at]) : ((const float*)a.table)[at];
+}
+// LDS floats [2 (span + RP_PAD) + 1]: entry x = bias of rel = sign * (x - span - RP_PAD), divided by the scale
+__device__ __forceinline__ void rp_fill_table(const RpArgs& a, float* tab, int h, int sign, int tid) {
+    const int n = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD;
+    const float inv = 1.0f / a.scale;
+    for (int x = tid; x < n; x += 256) tab[x] = rp_table(a, sign * (x - mid), h) * inv;
+}
+// zero rows [0, lead) and [end, T) of a packed tensor: `which` of `nwg` workgroups
+template <typename T>
+__device__ __forceinline__ void rp_zero_rows(T* p, const RpTensor& s, int heads, int D, int lead, int end, int T_, int which, int nwg, int tid) {
+    const int64_t per = (int64_t)heads * (D / 4), n = (int64_t)(lead + T_ - end) * per;
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t i = (int64_t)which * 256 + tid; i < n; i += (int64_t)nwg * 256) {
+        int64_t row = i / per;
+        const int64_t rest = i % per;
+        if (row >= lead) row += end - lead;
+        RpTile<T, 2>::st4(p + row * s.st + (rest / (D / 4)) * s.sh + (rest % (D / 4)) * 4, z);
+    }
+}
+#define RP_TAIL_WGS 32

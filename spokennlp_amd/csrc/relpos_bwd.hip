@@ -1,0 +1,519 @@
+// Attention under a learned relative position bias, backward (operator and notation: relpos.h).  The probabilities are recomputed from the saved
+// log-sum-exp:  p = exp(s - lse), dp = dout . v, delta = dout . out, ds = p (dp - delta);
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i      dv_j = sum_i p_ij dout_i      dtable[b, h] = sum over rel in bucket b of ds
+// Two kernels, neither with an atomic on a gradient: rp_dq_kernel owns query rows and walks the keys (dq, delta), rp_dkv_kernel owns keys and walks the
+// query rows of every head of its group (dk, dv, the sums for dtable).  Seven products instead of the five of the formulas; results do not depend on
+// any order of arrival.
+//
+// delta.  sum_j ds_ij = 0, so a bucket that holds most of a row's probability has for its gradient what is left of a cancellation; delta taken from the
+// bf16 `out` is off by up to 2^-8 of it, the same way for every element of the row (1 % of dtable measured, 40 queries against 3 .. 1500 keys).  What the
+// ds of a row sum to instead of 0 IS that error (sum_j p_ij = 1): rp_dq_kernel sums them in fp32 on its way and hands the mended delta on.  Its own dq
+// feels the error only where a row's probability sits on a few keys (by 1 / sqrt of their number): row blocks of at most RP_TWICE_KEYS keys walk them
+// twice, the first time for the sum alone (dq of 33-token sequences: 2.5e-3 -> 2.3e-3 of its norm; longer ones 2.4e-3 either way).
+//
+// dtable.  In the accumulator layout lane (g, i16) holds ds of query 4 g + r (register r) and key i16, so -rel = const + 4 g + r - i16.  Moving register r
+// by r lanes inside its 16 (a DPP operand modifier of the add itself) puts equal rel into equal lanes: the 16 x 16 tiles of one block diagonal add
+// up in one register per lane, the lanes that fall off the end belong to the next block diagonal's register.  7 adds per 4 elements, no LDS; the registers go
+// to the wave's own LDS bins once per 64-row chunk.  Chunks beyond the span add into one register per side instead (one add per element).
+#include "relpos.h"
+#include "relpos_launch.h"
+
+#define RP_TWICE_KEYS 128
+
+template <int CTRL>
+__device__ __forceinline__ float rp_dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// acc[k], acc[k + 1] += the sums over equal rel of one 16 x 16 tile (block diagonal k): lane (g, i) of acc[k] stands for rel 16 k + 4 g - i
+__device__ __forceinline__ void rp_diag_add(f32x4 x, float& lo, float& hi) {
+    lo += x[0];
+    lo += rp_dpp<0x101>(x[1]); hi += rp_dpp<0x11f>(x[1]);          // row_shl 1 / row_shr 15
+    lo += rp_dpp<0x102>(x[2]); hi += rp_dpp<0x11e>(x[2]);
+    lo += rp_dpp<0x103>(x[3]); hi += rp_dpp<0x11d>(x[3]);
+}
+
+template <typename T, int DT, int QT>
+__global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
+    typedef RpTile<T, DT> Ti;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int mid = a.span + RP_PAD;
+    char* tK = smem;
+    char* tV = smem + Ti::BYTES;
+    float* tab = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
+    const int nmain = a.B * a.heads * a.nrb;
+    if ((int)blockIdx.x >= nmain) {
+        const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq);
+        rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain, RP_TAIL_WGS, tid);
+        return;
+    }
+    int rb, h, b;
+    rp_place(blockIdx.x, a.nrb, a.B, a.heads, a.kv_heads, rb, h, b);
+    const RpSeq sq = rp_seq(a, b);
+    constexpr int BQ = 64 * QT;
+    if (rb * BQ >= sq.qn) return;
+    rp_fill_table(a, tab, h, 1, tid);
+    const int hk = h / (a.heads / a.kv_heads);
+    const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
+    const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
+    const float c2 = a.scale * RP_LOG2E;
+    const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+    constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums)
+
+    for (; rb * BQ < sq.qn; rb += a.nrb) {
+        const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
+        typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
+        float nd[QT], nl[QT];                               // -delta, -lse in the exponent's units
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int q = qw + ct * 16 + i16;
+            const bool ok = q < sq.qn;
+            const int64_t qt = (int64_t)(sq.q0 + q);
+            float acc = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < Ti::KB; ++kk) {
+                fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
+                fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
+                acc += Ti::dot(fdo[ct][kk], Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok));
+            }
+            acc += __shfl_xor(acc, 16, 64);
+            acc += __shfl_xor(acc, 32, 64);
+            nd[ct] = -acc;
+            float lse = INFINITY;                           // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
+            if (ok) {
+                const int64_t row = rp_row(a, sq, b, h, q);
+                lse = a.lse[row];
+                if (lse == -INFINITY) lse = INFINITY;
+            }
+            nl[ct] = -lse * RP_LOG2E;
+        }
+        f32x4 dq[QT][DT];
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dq[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        float rsum[QT];                                     // sum of a row's ds (each of its four lanes: a quarter of the keys)
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) rsum[ct] = 0.f;
+        int c_end = (sq.kn + 63) / 64, c_128 = c_end;
+        if (a.causal) {
+            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;
+            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
+            const int last128 = min(q0 / 128 * 128 + 128, sq.qn) - 1 + sq.off;  // (the rule must not depend on QT)
+            c_128 = last128 < 0 ? 0 : min(c_128, last128 / 64 + 1);
+        }
+        for (int pass = MEND && c_128 * 64 <= RP_TWICE_KEYS ? 0 : 1; pass < 2; ++pass) {
+        int c = 0;
+        RpKeys keys;
+        keys.init(a, sq, b, l, c);
+        RpStage<T, DT> rk, rv;
+        uint64_t bits = 0;
+        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
+        if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+        while (c < c_end) {
+            __syncthreads();
+            rk.store(tK, tid); rv.store(tV, tid);
+            __syncthreads();
+            const int key0 = c * 64;
+            const uint64_t now = bits;
+            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
+            if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+            const int rel0 = key0 - (qw + sq.off);
+            if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
+            const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
+            const bool cut = a.causal && rel0 + 63 > 0;
+            const float* bt = tab + (rel0 + mid + 4 * g - i16);
+            const float far = rel0 > 0 ? farR : farL;
+#pragma unroll
+            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS];
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const int f = kp * Ti::RPS + j;
+                        if (near) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[ct][j][r] = bt[16 * (f - ct) + r];
+                        } else s[ct][j] = (f32x4){far, far, far, far};
+                        dp[ct][j] = (f32x4){nd[ct], nd[ct], nd[ct], nd[ct]};
+                    }
+#pragma unroll
+                for (int kk = 0; kk < Ti::KB; ++kk)
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const int f = kp * Ti::RPS + j;
+                        const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) {
+                            s[ct][j] = Ti::mma(fk, fq[ct][kk], s[ct][j]);
+                            dp[ct][j] = Ti::mma(fv, fdo[ct][kk], dp[ct][j]);
+                        }
+                    }
+                if (now != ~0ull) {
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const uint32_t nib = (uint32_t)(now >> ((kp * Ti::RPS + j) * 16 + 4 * g));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct) s[ct][j][r] = (nib >> r) & 1 ? s[ct][j][r] : -INFINITY;
+                    }
+                }
+                if (cut) {
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 > 0) s[ct][j][r] = -INFINITY;
+                }
+                typename Ti::frag fds[QT];
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) {
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, nl[ct]));
+                            dp[ct][j][r] *= p;
+                            if (MEND) rsum[ct] += dp[ct][j][r];
+                        }
+                    }
+                    fds[ct] = Ti::pf(dp[ct]);
+                }
+                if (pass == 0) continue;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
+                }
+            }
+        }
+        if (!MEND) break;
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            rsum[ct] += __shfl_xor(rsum[ct], 16, 64);
+            rsum[ct] += __shfl_xor(rsum[ct], 32, 64);
+            nd[ct] -= rsum[ct];
+            rsum[ct] = 0.f;
+        }
+        }
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int q = qw + ct * 16 + i16;
+            if (q >= sq.qn) continue;
+            if (g == 0) a.delta[rp_row(a, sq, b, h, q)] = -nd[ct];
+            T* op = (T*)a.dq + b * a.sdq.sb + (int64_t)(sq.q0 + q) * a.sdq.st + h * a.sdq.sh;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, dq[ct][d] * a.scale);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int DT, int QT>
+__global__ __launch_bounds__(256, 1) void rp_dkv_kernel(RpArgs a) {
+    typedef RpTile<T, DT> Ti;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int ND = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD;
+    char* tQ = smem;
+    char* tO = smem + Ti::BYTES;
+    float* rowl = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);       // -lse and -delta of the 64 query rows
+    float* rowd = rowl + 64;
+    float* tab = rowd + 64;                                 // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
+    float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
+    const int nmain = a.B * a.kv_heads * a.nrb;
+    if ((int)blockIdx.x >= nmain) {
+        const int lead = rp_clamp(a.cu_k[0], 0, a.Tk), end = rp_clamp(a.cu_k[a.B], lead, a.Tk);
+        rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
+        rp_zero_rows((T*)a.dv, a.sdv, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
+        return;
+    }
+    int rb, hk, b;
+    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads, a.kv_heads, rb, hk, b);
+    const RpSeq sq = rp_seq(a, b);
+    constexpr int BK = 64 * QT;
+    const int G = a.heads / a.kv_heads;
+    const float c2 = a.scale * RP_LOG2E;
+    const int rows_k = a.cu_k ? sq.kn : a.Lk;               // padded: rows past k_lens are gradients of zero, and written
+    float* part = a.part_d ? a.part_d + ((int64_t)hk * G * a.B * a.nrb + (int64_t)b * a.nrb + rb) * ND : nullptr;     // of the group's first head
+    const int64_t part_h = (int64_t)a.B * a.nrb * ND;
+    if (part && rb * BK >= rows_k)
+        for (int gi = 0; gi < G; ++gi)
+            for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
+    float* bw = bins + w * ND;
+    bool again = false;                                     // (a second row block of a sequence longer than the hint adds to the first one's sums)
+
+    for (; rb * BK < rows_k; rb += a.nrb) {
+        const int k0 = rb * BK, kw = k0 + w * 16 * QT;
+        bool seen[QT];
+        bool any = false, all = true;
+        typename Ti::frag fk[QT][Ti::KB], fv[QT][Ti::KB];
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int key = kw + ct * 16 + i16;
+            seen[ct] = key < sq.kn && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
+            any |= seen[ct];
+            all &= seen[ct];
+            const int64_t kt = (int64_t)(sq.k0 + key);
+#pragma unroll
+            for (int kk = 0; kk < Ti::KB; ++kk) {
+                fk[ct][kk] = Ti::gfrag((const T*)a.k + b * a.sk.sb + kt * a.sk.st + hk * a.sk.sh, kk, g, a.D, seen[ct]);
+                fv[ct][kk] = Ti::gfrag((const T*)a.v + b * a.sv.sb + kt * a.sv.st + hk * a.sv.sh, kk, g, a.D, seen[ct]);
+            }
+        }
+        const bool wave_any = __any(any), wave_all = __all(all);
+        const bool wg_any = __syncthreads_or(any);
+        f32x4 dk[QT][DT], dv[QT][DT];
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+        const int n_ch = wg_any ? (sq.qn + 63) / 64 : 0;
+        int c_first = 0;
+        if (a.causal) c_first = max(0, k0 - sq.off) / 64;   // query rows before k0 - off see none of these keys
+        for (int gi = 0; gi < G; ++gi) {
+            const int h = hk * G + gi;
+            const T* qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
+            const T* ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
+            const int64_t row0 = rp_row(a, sq, b, h, 0);
+            __syncthreads();
+            rp_fill_table(a, tab, h, -1, tid);
+            if (part)
+                for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
+            f32x4 sumL = {0.f, 0.f, 0.f, 0.f}, sumR = {0.f, 0.f, 0.f, 0.f};
+            const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+            RpStage<T, DT> rq, ro;
+            float rl = 0.f, rd = 0.f;
+            auto fetch = [&](int c) {
+                const uint64_t ok = rp_low_bits(sq.qn - c * 64);
+                rq.load(qb + (int64_t)c * 64 * a.sq.st, a.sq.st, ok, a.D, tid);
+                ro.load(ob + (int64_t)c * 64 * a.sdo.st, a.sdo.st, ok, a.D, tid);
+                if (tid < 64) {
+                    const bool in = c * 64 + tid < sq.qn;
+                    const float lse = in ? a.lse[row0 + c * 64 + tid] : INFINITY;
+                    rl = lse == -INFINITY ? -INFINITY : -lse * RP_LOG2E;
+                    rd = in ? -a.delta[row0 + c * 64 + tid] : 0.f;
+                }
+            };
+            if (c_first < n_ch) fetch(c_first);
+            for (int c = c_first; c < n_ch; ++c) {
+                __syncthreads();
+                rq.store(tQ, tid); ro.store(tO, tid);
+                if (tid < 64) { rowl[tid] = rl; rowd[tid] = rd; }
+                __syncthreads();
+                if (c + 1 < n_ch) fetch(c + 1);
+                const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
+                if (!wave_any || (a.causal && rel0 + 63 < 0)) continue;
+                const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
+                const bool cut = a.causal && rel0 - (16 * QT - 1) < 0;
+                const float* bt = tab + (rel0 + mid + 4 * g - i16);
+                const float far = rel0 > 0 ? farL : farR;
+                float diag[5 + QT], col[QT];                // block diagonals -(QT - 1) .. 4, and one above; what a far column starts from
+                f32x4 fsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 5 + QT; ++k) diag[k] = 0.f;
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) col[ct] = seen[ct] ? far : -INFINITY;
+#pragma unroll
+                for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS];
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const int f = kp * Ti::RPS + j;
+                        lr[j] = *reinterpret_cast<const f32x4*>(rowl + f * 16 + g * 4);
+                        const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) {
+                            if (near) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) s[ct][j][r] = bt[16 * (f - ct) + r];
+                                if (!wave_all)              // a hidden key's column: p = 0
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) s[ct][j][r] = seen[ct] ? s[ct][j][r] : -INFINITY;
+                            } else s[ct][j] = (f32x4){col[ct], col[ct], col[ct], col[ct]};
+                            dp[ct][j] = d4;
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < Ti::KB; ++kk)
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j) {
+                            const int f = kp * Ti::RPS + j;
+                            const typename Ti::frag fq = Ti::rowf(tQ, f * 16 + i16, kk, g), fo = Ti::rowf(tO, f * 16 + i16, kk, g);
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct) {
+                                s[ct][j] = Ti::mma(fq, fk[ct][kk], s[ct][j]);
+                                dp[ct][j] = Ti::mma(fo, fv[ct][kk], dp[ct][j]);
+                            }
+                        }
+                    if (cut) {
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                            for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 < 0) s[ct][j][r] = -INFINITY;
+                    }
+                    typename Ti::frag fp[QT], fds[QT];
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) {
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, lr[j][r]));
+                                s[ct][j][r] = p;
+                                dp[ct][j][r] *= p;
+                            }
+                        if (part) {
+#pragma unroll
+                            for (int j = 0; j < Ti::RPS; ++j) {
+                                const int k = kp * Ti::RPS + j - ct + QT - 1;
+                                if (near) rp_diag_add(dp[ct][j], diag[k], diag[k + 1]);
+                                else fsum += dp[ct][j];
+                            }
+                        }
+                        fp[ct] = Ti::pf(s[ct]);
+                        fds[ct] = Ti::pf(dp[ct]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const typename Ti::frag fo = Ti::colf(tO, kp, d, l), fq = Ti::colf(tQ, kp, d, l);
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) {
+                            dv[ct][d] = Ti::mma(fo, fp[ct], dv[ct][d]);
+                            dk[ct][d] = Ti::mma(fq, fds[ct], dk[ct][d]);
+                        }
+                    }
+                }
+                if (part) {
+                    if (near) {
+                        // 16 lanes at a time: inside one instruction no two lanes meet in a bin, and a wave's LDS operations complete in order
+                        float* bd = bw + (rel0 - 16 * (QT - 1) + mid + 4 * g - i16);
+#pragma unroll
+                        for (int gg = 0; gg < 4; ++gg)
+                            if (g == gg)
+#pragma unroll
+                                for (int k = 0; k < 4 + QT; ++k) atomicAdd(bd + 16 * k, diag[k]);
+                    } else if (rel0 > 0) sumL += fsum;
+                    else sumR += fsum;
+                }
+            }
+            if (part) {
+                const float L = wave_sum(sumL[0] + sumL[1] + sumL[2] + sumL[3]), R = wave_sum(sumR[0] + sumR[1] + sumR[2] + sumR[3]);
+                if (c_first >= n_ch) __syncthreads();       // (the zeroed bins: no chunk's barrier came in between)
+                if (l == 0) { bw[0] += R; bw[ND - 1] += L; }
+                __syncthreads();
+                for (int x = tid; x < ND; x += 256) {
+                    const float t = (bins[x] + bins[ND + x]) + (bins[2 * ND + x] + bins[3 * ND + x]);
+                    float* o = part + gi * part_h + (ND - 1 - x);
+                    *o = again ? *o + t : t;
+                }
+            }
+        }
+        again = true;
+        // a hidden key's column is zero, whatever dout held
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int key = kw + ct * 16 + i16;
+            if (key >= rows_k) continue;
+            T* kp_ = (T*)a.dk + b * a.sdk.sb + (int64_t)(sq.k0 + key) * a.sdk.st + hk * a.sdk.sh;
+            T* vp_ = (T*)a.dv + b * a.sdv.sb + (int64_t)(sq.k0 + key) * a.sdv.st + hk * a.sdv.sh;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                if (d * 16 + g * 4 < a.D) {
+                    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                    Ti::st4(kp_ + d * 16 + g * 4, seen[ct] ? dk[ct][d] * a.scale : z);
+                    Ti::st4(vp_ + d * 16 + g * 4, seen[ct] ? dv[ct][d] : z);
+                }
+        }
+        __syncthreads();
+    }
+}
+
+// the partial sums of a head over its workgroups, in their order: 64 places of rel per workgroup, 16 interleaved groups of partials
+__global__ __launch_bounds__(1024) void rp_sum_kernel(const float* part, float* sums, int64_t wgs, int nd) {
+    __shared__ float red[16][64];
+    const int x = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6, h = blockIdx.y;
+    float s = 0.f;
+    if (x < nd)
+        for (int64_t i = y; i < wgs; i += 16) s += part[(h * wgs + i) * nd + x];
+    red[y][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (y == 0 && x < nd) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+        sums[(int64_t)h * nd + x] = s;
+    }
+}
+// sums over the places of a bucket: one wave per (bucket, head)
+__global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16) {
+    const int bk = blockIdx.x, h = blockIdx.y, n = 2 * (span + pad) + 1;
+    float s = 0.f;
+    for (int x = threadIdx.x; x < n; x += 64)
+        if (rp_clamp(map[rp_clamp(x - span - pad, -span, span) + span], 0, buckets - 1) == bk) s += sums[(int64_t)h * n + x];
+    s = wave_sum(s);
+    if (threadIdx.x == 0) {
+        if (bf16) ((bf16_t*)dtable)[(int64_t)bk * heads + h] = f2bf(s);
+        else ((float*)dtable)[(int64_t)bk * heads + h] = s;
+    }
+}
+int amdseg_relpos_sums_impl(const float* part, float* sums, int64_t wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16,
+                            hipStream_t s) {
+    const int nd = 2 * (span + pad) + 1;
+    hipLaunchKernelGGL(rp_sum_kernel, dim3((nd + 63) / 64, heads), dim3(1024), 0, s, part, sums, wgs, nd);
+    const int rc = amdseg_launch_status();
+    if (rc) return rc;
+    hipLaunchKernelGGL(rp_bucket_kernel, dim3(buckets, heads), dim3(64), 0, s, sums, map, span, pad, buckets, heads, dtable, bf16);
+    return amdseg_launch_status();
+}
+
+template <typename T, int DT>
+static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStream_t s) {
+    const int ND = 2 * (a.span + RP_PAD) + 1;
+    const int tail = a.zero_tail ? RP_TAIL_WGS : 0;
+    const int qt = rp_fwd_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
+    a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
+    const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
+    if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    const int lds = 2 * RpTile<T, DT>::BYTES + ND * 4;
+    int rc;
+    if (n == 0) {
+    } else if (sizeof(T) == 4 || qt == 1) {
+        if ((rc = rp_allow_lds((const void*)rp_dq_kernel<T, DT, 1>, lds))) return rc;
+        hipLaunchKernelGGL((rp_dq_kernel<T, DT, 1>), dim3((unsigned)n), dim3(256), lds, s, a);
+    } else if constexpr (sizeof(T) == 2) {
+        if ((rc = rp_allow_lds((const void*)rp_dq_kernel<T, DT, 2>, lds))) return rc;
+        hipLaunchKernelGGL((rp_dq_kernel<T, DT, 2>), dim3((unsigned)n), dim3(256), lds, s, a);
+    }
+    if ((rc = amdseg_launch_status())) return rc;
+    a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
+    const int64_t m = (int64_t)a.B * a.kv_heads * a.nrb + tail;
+    if (m > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    const int lds2 = 2 * RpTile<T, DT>::BYTES + 512 + ND * 4 * (a.part_d ? 5 : 1);
+    if (m == 0) {
+    } else if (sizeof(T) == 4 || kt == 1) {
+        if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 1>, lds2))) return rc;
+        hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 1>), dim3((unsigned)m), dim3(256), lds2, s, a);
+    } else if constexpr (sizeof(T) == 2) {
+        if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 2>, lds2))) return rc;
+        hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 2>), dim3((unsigned)m), dim3(256), lds2, s, a);
+    }
+    if ((rc = amdseg_launch_status()) || !a.part_d) return rc;
+    return amdseg_relpos_sums_impl(a.part_d, sums, (int64_t)a.B * a.nrb, a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
+}
+template <typename T>
+static int rp_bwd_d(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {
+    return a.D <= 32 ? rp_bwd_launch<T, 2>(a, dtype, dtable, sums, s) : a.D <= 64 ? rp_bwd_launch<T, 4>(a, dtype, dtable, sums, s)
+                                                                              : rp_bwd_launch<T, 8>(a, dtype, dtable, sums, s);
+}
+int amdseg_relpos_bwd_impl(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {
+    return dtype == 1 ? rp_bwd_d<float>(a, dtype, dtable, sums, s) : rp_bwd_d<bf16_t>(a, dtype, dtable, sums, s);
+}

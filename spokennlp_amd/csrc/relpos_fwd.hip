@@ -1,0 +1,247 @@
+// Attention under a learned relative position bias, forward (operator and notation: relpos.h).  The framework's other attention kernels
+// (attention.hip) take one interleaved projection with head_dim 64, whole 64-token blocks and an additive key mask.
+//
+// One workgroup = 4 waves x QT * 16 query rows of one (sequence, head); the keys stream through LDS in chunks of 64 with an online softmax.  S^T = K Q^T
+// keeps a query in a lane (its maximum and sum are lane scalars, the probabilities are the second operand of O^T += V^T P^T as they stand).
+#include "relpos.h"
+#include "relpos_launch.h"
+
+template <typename T, int DT, int QT>
+__global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
+    typedef RpTile<T, DT> Ti;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char* tK = smem;
+    char* tV = smem + Ti::BYTES;
+    float* tab = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
+    int id = blockIdx.x;
+    const int nmain = a.B * a.heads * a.nrb;
+    const int split = id / nmain;
+    if (split >= a.nsplit) {                                // the buffer rows outside every sequence
+        const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq), which = id - nmain * a.nsplit;
+        rp_zero_rows((T*)a.out, a.so, a.heads, a.D, lead, end, a.Tq, which, RP_TAIL_WGS, tid);
+        if (a.lse)
+            for (int h = 0; h < a.heads; ++h)
+                for (int r = which * 256 + tid; r < lead + a.Tq - end; r += RP_TAIL_WGS * 256)
+                    a.lse[(int64_t)h * a.Tq + (r < lead ? r : r - lead + end)] = -INFINITY;
+        return;
+    }
+    id -= split * nmain;
+    int rb, h, b;
+    rp_place(id, a.nrb, a.B, a.heads, a.kv_heads, rb, h, b);
+    const RpSeq sq = rp_seq(a, b);
+    constexpr int BQ = 64 * QT;
+    if (rb * BQ >= sq.qn) return;
+    rp_fill_table(a, tab, h, 1, tid);
+    const int hk = h / (a.heads / a.kv_heads);
+    const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
+    const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
+    const T* qbase = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
+    const float c2 = a.scale * RP_LOG2E;
+    const int mid = a.span + RP_PAD;
+    const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+
+    for (; rb * BQ < sq.qn; rb += a.nrb) {
+        const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
+        typename Ti::frag fq[QT][Ti::KB];
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int q = qw + ct * 16 + i16;
+#pragma unroll
+            for (int kk = 0; kk < Ti::KB; ++kk) fq[ct][kk] = Ti::gfrag(qbase + (int64_t)q * a.sq.st, kk, g, a.D, q < sq.qn);
+        }
+        f32x4 o[QT][DT];
+        float m_run[QT], l_part[QT];
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            m_run[ct] = -INFINITY; l_part[ct] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+        int c = 0, c_end = (sq.kn + 63) / 64;
+        if (a.causal) {
+            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;                  // the last key any row of the block sees
+            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
+        }
+        if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
+        RpKeys keys;
+        keys.init(a, sq, b, l, c);
+        RpStage<T, DT> rk, rv;
+        uint64_t bits = 0;
+        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
+        if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+        while (c < c_end) {
+            __syncthreads();                                // the chunk before has been read (and the table written)
+            rk.store(tK, tid); rv.store(tV, tid);
+            __syncthreads();
+            const int key0 = c * 64;
+            const uint64_t now = bits;
+            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
+            if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+            const int rel0 = key0 - (qw + sq.off);          // rel of the tile's first key and the wave's first query
+            if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
+            f32x4 s[QT][4];
+            if (rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span) {
+                const float* bt = tab + (rel0 + mid + 4 * g - i16);
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[ct][f][r] = bt[16 * (f - ct) + r];
+            } else {
+                const float x = rel0 > 0 ? farR : farL;
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) s[ct][f] = (f32x4){x, x, x, x};
+            }
+#pragma unroll
+            for (int kk = 0; kk < Ti::KB; ++kk)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g);
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) s[ct][f] = Ti::mma(fk, fq[ct][kk], s[ct][f]);
+                }
+            if (now != ~0ull) {
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) s[ct][f][r] = (nib >> r) & 1 ? s[ct][f][r] : -INFINITY;
+                }
+            }
+            if (a.causal && rel0 + 63 > 0) {
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) s[ct][f][r] = -INFINITY;
+            }
+#pragma unroll
+            for (int ct = 0; ct < QT; ++ct) {
+                float mx = s[ct][0][0];
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[ct][f][r]);
+                mx *= c2;
+                if (__any(mx > m_run[ct])) {                // wave-uniform: some row's running maximum grows
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    const float m_new = fmaxf(m_run[ct], mx);
+                    const float al = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[ct] - m_new);
+                    m_run[ct] = m_new;
+                    l_part[ct] *= al;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[ct][d][r] *= al;
+                }
+                const float mu = m_run[ct] == -INFINITY ? 0.f : m_run[ct];
+                float sum = 0.f;
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[ct][f][r], c2, -mu));
+                        s[ct][f][r] = e;
+                        sum += e;
+                    }
+                l_part[ct] += sum;
+            }
+#pragma unroll
+            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                typename Ti::frag fp[QT];
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) fp[ct] = Ti::pf(&s[ct][kp * Ti::RPS]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const typename Ti::frag fv = Ti::colf(tV, kp, d, l);
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) o[ct][d] = Ti::mma(fv, fp[ct], o[ct][d]);
+                }
+            }
+        }
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            const int q = qw + ct * 16 + i16;
+            float ls = l_part[ct];
+            ls += __shfl_xor(ls, 16, 64);
+            ls += __shfl_xor(ls, 32, 64);
+            if (q >= sq.qn) continue;
+            const int64_t row = rp_row(a, sq, b, h, q);
+            if (a.nsplit > 1) {
+                const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
+                float* po = a.part_o + (split * rows + row) * a.D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(po + d * 16 + g * 4) = o[ct][d];
+                if (g == 0) { a.part_ml[(split * rows + row) * 2] = m_run[ct]; a.part_ml[(split * rows + row) * 2 + 1] = ls; }
+                continue;
+            }
+            const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);    // a row that saw no key: zero; NaN stays
+            T* op = (T*)a.out + b * a.so.sb + (int64_t)(sq.q0 + q) * a.so.st + h * a.so.sh;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, o[ct][d] * inv);
+            if (a.lse && g == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m_run[ct] + __builtin_amdgcn_logf(ls)) * RP_LN2;
+        }
+        __syncthreads();                                    // (another row block of a packed sequence longer than the hint)
+    }
+}
+
+// the splits of a row joined in their order: one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void rp_join_kernel(RpArgs a) {
+    const int l = threadIdx.x & 63;
+    const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    float m = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float ls = 0.f, x0 = 0.f, x1 = 0.f;
+    const int d = l * 2;
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - mu);
+        ls += f * a.part_ml[(s * rows + row) * 2 + 1];
+        if (d < a.D) { const float* p = a.part_o + (s * rows + row) * a.D + d; x0 += f * p[0]; x1 += f * p[1]; }
+    }
+    const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
+    const int i = (int)(row % a.Lq), h = (int)(row / a.Lq % a.heads), b = (int)(row / a.Lq / a.heads);
+    T* op = (T*)a.out + b * a.so.sb + (int64_t)i * a.so.st + h * a.so.sh;
+    if (d < a.D) { Act<T>::st(op + d, x0 * inv); Act<T>::st(op + d + 1, x1 * inv); }
+    if (a.lse && l == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(ls)) * RP_LN2;
+}
+
+template <typename T, int DT, int QT>
+static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
+    const int lds = 2 * RpTile<T, DT>::BYTES + (2 * (a.span + RP_PAD) + 1) * 4;
+    const int rc = rp_allow_lds((const void*)rp_fwd_kernel<T, DT, QT>, lds);
+    if (rc) return rc;
+    const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
+    if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    hipLaunchKernelGGL((rp_fwd_kernel<T, DT, QT>), dim3((unsigned)n), dim3(256), lds, s, a);
+    if (a.nsplit > 1) {
+        const int64_t rows = (int64_t)a.B * a.heads * a.Lq;
+        hipLaunchKernelGGL((rp_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    }
+    return amdseg_launch_status();
+}
+template <typename T, int QT>
+static int rp_fwd_d(const RpArgs& a, hipStream_t s) {
+    return a.D <= 32 ? rp_fwd_launch<T, 2, QT>(a, s) : a.D <= 64 ? rp_fwd_launch<T, 4, QT>(a, s) : rp_fwd_launch<T, 8, QT>(a, s);
+}
+int amdseg_relpos_fwd_impl(const RpArgs& a0, int dtype, hipStream_t s) {
+    RpArgs a = a0;
+    const int qt = rp_fwd_qt(a, dtype);
+    a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
+    if (dtype == 1) return rp_fwd_d<float, 1>(a, s);
+    return qt == 1 ? rp_fwd_d<bf16_t, 1>(a, s) : rp_fwd_d<bf16_t, 2>(a, s);
+}

@@ -1,0 +1,27 @@
+// Launch geometry of the relative-position attention kernels (host side).
+#pragma once
+#include "relpos.h"
+
+int amdseg_relpos_fwd_impl(const RpArgs& a, int dtype, hipStream_t s);
+int amdseg_relpos_bwd_impl(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s);
+
+int amdseg_relpos_sums_impl(const float* part, float* sums, int64_t wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16,
+                            hipStream_t s);
+size_t amdseg_relpos_bias_ws_impl(int B, int heads, int Lq, int span);
+int amdseg_relpos_bias_fwd_impl(const RpArgs& a, int off, int dtype, hipStream_t s);
+int amdseg_relpos_bias_bwd_impl(const void* d, int dtype, const int* map, int span, int buckets, int B, int heads, int Lq, int Lk, int off, float* dtable,
+                                float* ws, hipStream_t s);
+
+// dynamic LDS beyond 64 KiB has to be asked for per kernel and device
+static inline int rp_allow_lds(const void* kernel, int bytes) {
+    if (bytes <= 65536) return 0;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e == hipSuccess ? 0 : (int)e;
+}
+// 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products) unless that leaves CUs without a workgroup
+static inline int rp_qt(int64_t wgs_of_two, int dtype) { return dtype == 1 ? 1 : wgs_of_two < 256 ? 1 : 2; }
+static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return rp_qt((int64_t)((a.Lq + 127) / 128) * a.B * a.heads, dtype); }
+static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, dtype); }
+// splits over the keys: few query rows against many keys (single tokens against a cache).  A fixed number of keys per split: a sequence's sums do not
+// depend on the batch around it.
+static inline int rp_nsplit(int Lq, int Lk, bool packed) { return !packed && Lq <= 16 && Lk > RP_SPLIT_KEYS ? (Lk + RP_SPLIT_KEYS - 1) / RP_SPLIT_KEYS : 1; }

@@ -46,6 +46,17 @@ class LayerWs(C.Structure):
                                   "d_out_s", "du_s", "d_ao_s", "dqkv_s", "dctx_s")]
 
 
+_strides = C.c_int64 * 3
+
+
+class RelposCfg(C.Structure):
+    """struct amdseg_relpos_cfg (include/amdseg.h)"""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "table_dtype", "B", "Lq", "Lk", "Tq", "Tk", "heads", "kv_heads", "D", "span", "buckets", "causal",
+                                         "align_end", "zero_tail")] + [("scale", f32)] + \
+               [(n + "_stride", _strides) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + \
+               [(n, vp) for n in ("cu_q", "cu_k", "k_lens", "key_mask")] + [("mask_stride", C.c_int64), ("map", vp), ("table", vp)]
+
+
 # name -> argtypes (restype is always int unless listed in _RESTYPE); mirrors include/amdseg.h one for one
 _PROTOS = {
     "amdseg_abi_version": [],
@@ -146,11 +157,18 @@ _PROTOS = {
     "amdseg_sumsq": [vp, sz, vp, vp, i32, vp],
     "amdseg_clip_coef": [vp, f32, f32, vp, vp, vp],
     "amdseg_scale": [vp, sz, vp, vp],
+    "amdseg_relpos_attn_ws_bytes": [C.POINTER(RelposCfg), i32],
+    "amdseg_relpos_attn_fwd": [C.POINTER(RelposCfg), vp, vp, vp, vp, vp, vp, sz, vp],
+    "amdseg_relpos_attn_bwd": [C.POINTER(RelposCfg), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp],
+    "amdseg_relpos_bias_fwd": [vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, i32, vp],
+    "amdseg_relpos_bias_ws_bytes": [i32, i32, i32, i32],
+    "amdseg_relpos_bias_bwd": [vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, sz, vp],
     "amdseg_bert_layer_fwd": [C.POINTER(BertCfg), C.POINTER(LayerParams), C.POINTER(LayerActs), vp, i32, vp],
     "amdseg_bert_layer_bwd": [C.POINTER(BertCfg), C.POINTER(LayerParams), C.POINTER(LayerGrads), C.POINTER(LayerActs),
                               C.POINTER(LayerWs), vp, vp, vp, i32, vp],
 }
-_RESTYPE = {"amdseg_error_string": C.c_char_p, "amdseg_attn_keepmask_bytes": C.c_size_t, "amdseg_ponet_global_scratch_floats": C.c_size_t}
+_RESTYPE = {"amdseg_error_string": C.c_char_p, "amdseg_attn_keepmask_bytes": C.c_size_t, "amdseg_ponet_global_scratch_floats": C.c_size_t,
+            "amdseg_relpos_attn_ws_bytes": C.c_size_t, "amdseg_relpos_bias_ws_bytes": C.c_size_t}
 
 EXPORTS = tuple(_PROTOS)
 _lib = None

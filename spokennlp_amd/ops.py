@@ -500,3 +500,229 @@ def pattn_bwd(qkv, mask_bias, ctx, dctx, lse, B, Lq, heads, p=0.0, seed=0):
     rc = L.load().amdseg_pattn_bwd(_p(qkv), _p(mask_bias), _p(ctx), _p(dctx), _p(lse), _p(delta), _p(dqkv), B, Lq, heads, 0.125, p, seed, _s())
     L.check(rc, "amdseg_pattn_bwd")
     return dqkv
+
+
+# ---- attention under a learned relative position bias (csrc/relpos_fwd.hip, relpos_bwd.hip, relpos_bias.hip)
+def relpos_bucket_list(num_buckets=32, max_distance=128, bidirectional=True):
+    """bucket of rel = -max_distance .. max_distance (key position - query position) as a list of 2 * max_distance + 1 ints.  Half of a side's
+    buckets hold one distance each, the others steps that grow with the distance up to max_distance; two sides, or (bidirectional=False) one: keys behind
+    the query share bucket 0 with distance 0.  Distances are compared as whole numbers (n >= m (M / m)^(k / steps)  <=>  n^steps >= m^(steps - k) M^k), so
+    no rounding of a logarithm moves one over a bucket's edge."""
+    half = num_buckets // 2 if bidirectional else num_buckets
+    m = half // 2
+    steps = half - m
+    if num_buckets < 1 or m < 1 or max_distance <= m:
+        raise ValueError(f"num_buckets = {num_buckets}, max_distance = {max_distance}: a side needs two buckets and max_distance beyond its first half")
+    near, k = list(range(m)), 0
+    for n in range(m, max_distance + 1):
+        while k + 1 < steps and n ** steps >= m ** (steps - k - 1) * max_distance ** (k + 1):
+            k += 1
+        near.append(m + k)
+    if bidirectional:
+        return near[:0:-1] + [near[0]] + [half + b for b in near[1:]]
+    return near[:0:-1] + [near[0]] * (max_distance + 1)
+
+
+def relpos_bucket_map(num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+    """relpos_bucket_list as the device tensor that the relpos_* functions take (build it once per model)"""
+    return torch.tensor(relpos_bucket_list(num_buckets, max_distance, bidirectional), dtype=torch.int32, device=device)
+
+
+def _rp_strides(t, name, esize):
+    """element strides (sequence, row, head) of [B, L, heads, D] or packed [T, heads, D]"""
+    st = t.stride()
+    if t.numel() and st[-1] != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous, strides are {st}")
+    st = [0 if n == 1 else s for n, s in zip(t.shape[:-1], st[:-1])]
+    if (t.data_ptr() | (st[-1] * esize) | (st[-2] * esize) | (st[0] * esize)) & 15:
+        raise ValueError(f"{name}: rows must start on 16 bytes (strides {t.stride()}, element size {esize})")
+    return (st[0] if len(st) == 3 else 0, st[-2], st[-1])
+
+
+def _rp_int(t, name, n, dev):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {dev}")
+    return t.data_ptr()
+
+
+def _rp_table(c, table, bucket_map, heads, dev):
+    if table.device != dev or bucket_map.device != dev:
+        raise ValueError(f"table and bucket_map must be on {dev}")
+    if table.dim() != 2 or table.shape[1] != heads or table.shape[0] < 1 or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous [buckets, {heads}] tensor, not {tuple(table.shape)}")
+    n = bucket_map.numel()
+    if n % 2 == 0 or n > 2049:
+        raise ValueError(f"bucket_map must hold 2 * span + 1 entries with span <= 1024, not {n}")
+    c.map, c.span = _rp_int(bucket_map, "bucket_map", n, dev), n // 2
+    c.table, c.table_dtype, c.buckets = table.data_ptr(), _dt(table), table.shape[0]
+
+
+def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end):
+    packed = cu_q is not None
+    if packed != (cu_k is not None):
+        raise ValueError("cu_q and cu_k come together")
+    nd = 3 if packed else 4
+    if q.dim() != nd or k.dim() != nd or v.shape != k.shape:
+        raise ValueError(f"q, k, v must be {'[tokens, heads, D]' if packed else '[B, L, heads, D]'}, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    dev = q.device
+    if dev.type != "cuda" or k.device != dev or v.device != dev:
+        raise ValueError("q, k, v must be on one GPU")
+    c = L.RelposCfg()
+    c.dtype = _dt(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v must share a dtype, not {q.dtype}, {k.dtype}, {v.dtype}")
+    heads, D = q.shape[-2:]
+    kv_heads = k.shape[-2]
+    if k.shape[-1] != D or D < 8 or D > 128 or D % 8:
+        raise ValueError(f"head dimension {D} (keys: {k.shape[-1]}): a multiple of 8 up to 128, the same for q, k, v")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are no multiple of {kv_heads} key / value heads")
+    c.heads, c.kv_heads, c.D = heads, kv_heads, D
+    es = q.element_size()
+    c.q_stride[:] = _rp_strides(q, "q", es)
+    c.k_stride[:] = _rp_strides(k, "k", es)
+    c.v_stride[:] = _rp_strides(v, "v", es)
+    if packed:
+        if k_lens is not None:
+            raise ValueError("k_lens belongs to the padded form; packed sequences have cu_k")
+        c.B, c.Tq, c.Tk = cu_q.numel() - 1, q.shape[0], k.shape[0]
+        if c.B < 0:
+            raise ValueError("cu_q needs at least one element")
+        c.cu_q, c.cu_k = _rp_int(cu_q, "cu_q", c.B + 1, dev), _rp_int(cu_k, "cu_k", c.B + 1, dev)
+        for n in (max_q, max_k):
+            if n is not None and n < 0:
+                raise ValueError("max_q / max_k must not be negative")
+        c.Lq = max(1, min(c.Tq, c.Tq if max_q is None else int(max_q)))
+        c.Lk = max(1, min(c.Tk, c.Tk if max_k is None else int(max_k)))
+    else:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError(f"q holds {q.shape[0]} sequences, k {k.shape[0]}")
+        c.B, c.Lq, c.Lk = q.shape[0], q.shape[1], k.shape[1]
+        if k_lens is not None:
+            c.k_lens = _rp_int(k_lens, "k_lens", c.B, dev)
+    if key_mask is not None:
+        want = (c.Tk,) if packed else (c.B, c.Lk)
+        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != want or key_mask.device != dev:
+            raise ValueError(f"key_mask must be a bool or uint8 tensor {want} on {dev}, not {key_mask.dtype} {tuple(key_mask.shape)}")
+        if key_mask.numel() and key_mask.shape[-1] > 1 and key_mask.stride(-1) != 1:
+            raise ValueError("key_mask: the last dimension must be contiguous")
+        c.key_mask, c.mask_stride = key_mask.data_ptr(), 0 if packed or key_mask.shape[0] == 1 else key_mask.stride(0)
+    _rp_table(c, table, bucket_map, heads, dev)
+    c.scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-6 < c.scale < 1e6:
+        raise ValueError(f"scale = {scale}: a positive number")
+    c.causal, c.align_end = int(bool(causal)), int(bool(align_end))
+    return c
+
+
+def _rp_out(t, like, name, es):
+    """a caller's output tensor: shape, dtype, device, and no two elements in one place"""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
+    at = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < at:
+            raise ValueError(f"{name}: elements overlap (strides {t.stride()})")
+        at = s * n if s * n > at else at
+    return _rp_strides(t, name, es)
+
+
+def _rp_ws(n, dev):
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
+
+
+def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None, causal=False,
+                    align_end=False, need_lse=True, out=None):
+    """softmax(scale q k^T + table[bucket_map[clamp(rel) + span]]) v with rel = key position - query position (amdseg_relpos_attn_fwd).
+
+    Padded: q [B, Lq, heads, D], k / v [B, Lk, kv_heads, D] (any strides with a contiguous last dimension and rows on 16 bytes: column blocks of a fused
+    projection, a cache), k_lens int32 [B] = keys held, key_mask bool / uint8 [B, Lk].  Packed: q [tokens, heads, D], cu_q / cu_k int32 [B + 1],
+    max_q / max_k = longest sequence (launch hints), key_mask [tokens].  bf16 or fp32; table [buckets, heads] of either; scale: D ** -0.5.
+    Query i stands at position i, or (align_end) so that the last query stands at the last key.  A row that sees no key: zero, lse -inf.
+    Returns (out, lse); lse fp32 [B, heads, Lq] / [heads, tokens], None unless need_lse.  `out`: rows outside every packed sequence are left as they were
+    (a fresh tensor has zeros there)."""
+    c = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+    dev = q.device
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            c.zero_tail = 1
+        c.out_stride[:] = _rp_out(out, q, "out", q.element_size())
+        lse = torch.empty((c.heads, c.Tq) if cu_q is not None else (c.B, c.heads, c.Lq), dtype=torch.float32, device=dev) if need_lse else None
+        lib = L.load()
+        n = lib.amdseg_relpos_attn_ws_bytes(C.byref(c), 0)
+        ws = _rp_ws(n, dev) if n else None
+        L.check(lib.amdseg_relpos_attn_fwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(ws), n, _s()), "amdseg_relpos_attn_fwd")
+    return out, lse
+
+
+def relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale=None, key_mask=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None,
+                    causal=False, align_end=False, need_dtable=True, dq=None, dk=None, dv=None):
+    """gradients of relpos_attn_fwd from its `out` and `lse` (amdseg_relpos_attn_bwd): (dq, dk, dv, dtable), the last in the table's dtype or None.
+    dq / dk / dv may be given (column blocks of one buffer): rows outside every packed sequence are left as they were in all three or, if none is given,
+    zero.  Sums are taken in a fixed order: the same call gives the same bits."""
+    c = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+    dev, es = q.device, q.element_size()
+    if (dq is None) != (dk is None) or (dq is None) != (dv is None):
+        raise ValueError("dq, dk, dv: give all three or none")
+    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype or out.device != dev or dout.device != dev:
+        raise ValueError(f"out and dout must be {tuple(q.shape)} {q.dtype} on {dev}")
+    want = (c.heads, c.Tq) if cu_q is not None else (c.B, c.heads, c.Lq)
+    if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError(f"lse must be the contiguous fp32 {want} of relpos_attn_fwd")
+    with torch.cuda.device(dev):
+        if dq is None:
+            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+            c.zero_tail = 1
+        c.out_stride[:] = _rp_strides(out, "out", es)
+        c.dout_stride[:] = _rp_strides(dout, "dout", es)
+        c.dq_stride[:] = _rp_out(dq, q, "dq", es)
+        c.dk_stride[:] = _rp_out(dk, k, "dk", es)
+        c.dv_stride[:] = _rp_out(dv, v, "dv", es)
+        dtable = torch.empty_like(table) if need_dtable else None
+        lib = L.load()
+        n = lib.amdseg_relpos_attn_ws_bytes(C.byref(c), 1)
+        ws = _rp_ws(n, dev)
+        L.check(lib.amdseg_relpos_attn_bwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable), _p(ws),
+                                           ws.numel(), _s()), "amdseg_relpos_attn_bwd")
+    return dq, dk, dv, dtable
+
+
+def relpos_bias_fwd(table, bucket_map, Lq, Lk, q_offset=0, out_dtype=torch.float32):
+    """the bias of relpos_attn_fwd as a dense [heads, Lq, Lk] tensor: for attention composed from single operations (probabilities that are dropped out
+    or returned)"""
+    if table.dim() != 2 or Lq < 0 or Lk < 0:
+        raise ValueError(f"table [buckets, heads], Lq and Lk >= 0, not {tuple(table.shape)}, {Lq}, {Lk}")
+    c, dev, heads = L.RelposCfg(), table.device, table.shape[1]
+    if dev.type != "cuda":
+        raise ValueError("table must be on a GPU")
+    _rp_table(c, table, bucket_map, heads, dev)
+    with torch.cuda.device(dev):
+        out = torch.empty((heads, Lq, Lk), dtype=out_dtype, device=dev)
+        L.check(L.load().amdseg_relpos_bias_fwd(c.table, c.table_dtype, c.map, c.span, c.buckets, heads, Lq, Lk, q_offset, _p(out), _dt(out), _s()),
+                "amdseg_relpos_bias_fwd")
+    return out
+
+
+def relpos_bias_bwd(dbias, bucket_map, buckets, q_offset=0):
+    """gradient of the table, fp32 [buckets, heads], from dbias [B, heads, Lq, Lk] (or [heads, Lq, Lk]), summed over the sequences, the queries and the
+    distances of a bucket in a fixed order"""
+    if dbias.dim() == 3:
+        dbias = dbias.unsqueeze(0)
+    if dbias.dim() != 4:
+        raise ValueError(f"dbias must be [B, heads, Lq, Lk], not {tuple(dbias.shape)}")
+    _chk(dbias, "dbias")
+    B, heads, Lq, Lk = dbias.shape
+    dev, n = dbias.device, bucket_map.numel()
+    if n % 2 == 0 or n > 2049 or buckets < 1:
+        raise ValueError(f"bucket_map must hold 2 * span + 1 entries with span <= 1024, not {n}; buckets = {buckets}")
+    if dbias.data_ptr() & 15:
+        raise ValueError("dbias must start on 16 bytes")
+    m = _rp_int(bucket_map, "bucket_map", n, dev)
+    with torch.cuda.device(dev):
+        dtable = torch.empty((buckets, heads), dtype=torch.float32, device=dev)
+        lib = L.load()
+        ws = _rp_ws(lib.amdseg_relpos_bias_ws_bytes(B, heads, Lq, n // 2), dev)
+        L.check(lib.amdseg_relpos_bias_bwd(_p(dbias), _dt(dbias), m, n // 2, buckets, B, heads, Lq, Lk, q_offset, _p(dtable), _p(ws), ws.numel(), _s()),
+                "amdseg_relpos_bias_bwd")
+    return dtable
