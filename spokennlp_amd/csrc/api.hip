@@ -675,7 +675,9 @@ int amdseg_bert_layer_bwd(const amdseg_bert_cfg* c, const amdseg_bert_layer_para
 }
 
 // ---- attention under a learned relative position bias (csrc/relpos_*.hip)
+// rows on 16 bytes, and 63 of them within the 31 bits of a chunk's lane offsets
 static bool relpos_rows_ok(const void* p, const int64_t st[3], int esize, bool empty) {
+    if (st[1] < 0 || st[1] * esize > (1 << 24)) return false;
     return (empty || p) && !((uintptr_t)p & 15) && !((st[0] | st[1] | st[2]) * esize & 15);
 }
 static int relpos_args(const struct amdseg_relpos_cfg* c, RpArgs& a) {

@@ -79,7 +79,8 @@ template <int DT> struct RpTile<bf16_t, DT> {
     typedef bf16x8 frag;
     static constexpr int BYTES = ((DT + 3) / 4) * 8192, KB = DT / 2, EPU = 8, UNITS = DT * 2;   // units = 16 bytes of a row
     static constexpr int KSTEP = 32, RPS = 2;                                                   // rows of a contraction step, 16-row tiles of it
-    static __device__ __forceinline__ char* at(char* t, int row, int c) { return t + (c >> 3) * 8192 + row * 128 + (((c & 7) ^ swz(row)) << 4); }
+    // piece p of 1 KiB: which row and 16-byte unit lane l's slot holds
+    static __device__ __forceinline__ void piece(int p, int l, int& row, int& c) { row = (p & 7) * 8 + (l >> 3); c = (p >> 3) * 8 + ((l & 7) ^ swz(row)); }
     static __device__ __forceinline__ frag rowf(const char* t, int row, int kb, int g) { return at_frag(t + (kb >> 1) * 8192, row, (kb & 1) * 4 + g); }
     static __device__ __forceinline__ frag colf(const char* t, int step, int dt, int l) {
         const int g = l >> 4;
@@ -105,7 +106,7 @@ template <int DT> struct RpTile<float, DT> {
     typedef f32x4 frag;
     static constexpr int BYTES = 64 * DT * 64, KB = DT, EPU = 4, UNITS = DT * 4;
     static constexpr int KSTEP = 16, RPS = 1;
-    static __device__ __forceinline__ char* at(char* t, int row, int c) { return t + row * (DT * 64) + ((c ^ (row & 7)) << 4); }
+    static __device__ __forceinline__ void piece(int p, int l, int& row, int& c) { row = p * (16 / DT) + l / (DT * 4); c = (l % (DT * 4)) ^ (row & 7); }
     static __device__ __forceinline__ frag rowf(const char* t, int row, int kb, int g) {
         return *reinterpret_cast<const frag*>(t + row * (DT * 64) + (((kb * 4 + g) ^ (row & 7)) << 4));
     }
@@ -134,28 +135,57 @@ template <int DT> struct RpTile<float, DT> {
     static __device__ __forceinline__ void st4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
 };
 
-// 64 rows of a tensor global -> registers -> LDS by a workgroup of 256.  Rows whose bit is clear and columns from D on become zeros: what stands in
-// masked rows (infinities, NaN) reaches no product.
+// 64 lanes x 16 bytes from base + lane offset to LDS.  The base may come straight from v_readfirstlane: a vector instruction's SGPR result needs five wait
+// states before a memory instruction reads it, and the compiler does not look for them inside an asm statement
+__device__ __forceinline__ void rp_glds16(const void* uniform_base, uint32_t lane_byte_offset, uint32_t lds_wave_addr) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(lane_byte_offset), "s"(uniform_base), "{m0}"(lds_wave_addr) : "memory");
+}
+
+// chunk buffers: two (the next chunk lands under this one's products), one where two would leave a CU a single workgroup (fp32, D > 64: the other
+// workgroup's products hide the wait)
+template <typename T, int DT> constexpr int rp_nb = DT * sizeof(T) >= 32 ? 1 : 2;
+
+// 64 rows of a tensor global -> LDS by the DMA path, 1 KiB a wave and instruction, no register in between.  The swizzle sits on the global side (lane l
+// fetches what its fixed LDS slot holds).  Rows whose bit is clear and columns from D on are not fetched: their places keep what they held -- the zeros of
+// rp_clear_lds or a visible row of an earlier chunk -- so what stands in hidden rows (infinities, NaN) reaches no product, and a probability of exactly 0 meets
+// a finite number.
 template <typename T, int DT> struct RpStage {
     typedef RpTile<T, DT> Ti;
-    static constexpr int N = 64 * Ti::UNITS / 256;
-    uint4 r[N];
-    __device__ __forceinline__ void load(const T* base, int64_t st, uint64_t bits, int D, int tid) {
+    static constexpr int N = Ti::BYTES / 4096;              // pieces of a wave
+    uint32_t off[N];                                        // byte offset of this lane's 16 bytes from the chunk's first row; ~0: beyond D
+    bool full;
+    __device__ __forceinline__ void init(int64_t st, int D, int w, int l) {
+        full = D == DT * 16;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + tid, row = u / Ti::UNITS, c = u % Ti::UNITS;
-            r[n] = make_uint4(0u, 0u, 0u, 0u);
-            if (((bits >> row) & 1) && c * Ti::EPU < D) r[n] = *reinterpret_cast<const uint4*>(base + row * st + c * Ti::EPU);
+            int row, c;
+            Ti::piece(w * N + n, l, row, c);
+            off[n] = c < Ti::UNITS && c * Ti::EPU < D ? (uint32_t)(row * st * (int64_t)sizeof(T) + c * 16) : ~0u;
         }
     }
-    __device__ __forceinline__ void store(char* tile, int tid) const {
+    __device__ __forceinline__ void load(const T* base, uint64_t bits, char* tile, int w, int l) const {
+        const uint32_t lds = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(char, tile)) + w * N * 1024;
+        const uint64_t u = (uint64_t)base;
+        // (readfirstlane returns a signed int: without the casts the low half's sign bit would run into the high half)
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)u), hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+        const void* ub = (const void*)(((uint64_t)hi << 32) | lo);
+        if (bits == ~0ull && full && DT % 4 == 0) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + tid;
-            *reinterpret_cast<uint4*>(Ti::at(tile, u / Ti::UNITS, u % Ti::UNITS)) = r[n];
+            for (int n = 0; n < N; ++n) rp_glds16(ub, off[n], lds + n * 1024);
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                int row, c;
+                Ti::piece(w * N + n, l, row, c);
+                if (((bits >> row) & 1) && off[n] != ~0u) rp_glds16(ub, off[n], lds + n * 1024);
+            }
         }
     }
 };
+__device__ __forceinline__ void rp_clear_lds(char* p, int bytes, int tid) {
+    for (int x = tid * 16; x < bytes; x += 4096) *reinterpret_cast<uint4*>(p + x) = make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ void rp_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); __syncthreads(); }
 
 // visible keys of a 64-key chunk as a wave-uniform word; the mask byte of the chunk after it is in flight
 struct RpKeys {

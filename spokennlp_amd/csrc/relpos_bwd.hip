@@ -35,11 +35,10 @@ __device__ __forceinline__ void rp_diag_add(f32x4 x, float& lo, float& hi) {
 template <typename T, int DT, int QT>
 __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
+    constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int mid = a.span + RP_PAD;
-    char* tK = smem;
-    char* tV = smem + Ti::BYTES;
-    float* tab = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);
+    float* tab = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.heads * a.nrb;
     if ((int)blockIdx.x >= nmain) {
@@ -53,6 +52,9 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
     rp_fill_table(a, tab, h, 1, tid);
+    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
+    RpStage<T, DT> rk, rv;
+    rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
@@ -106,18 +108,24 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         int c = 0;
         RpKeys keys;
         keys.init(a, sq, b, l, c);
-        RpStage<T, DT> rk, rv;
         uint64_t bits = 0;
+        int buf = 0;
+        auto fetch = [&](int at) {
+            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
+            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        };
         while (c < c_end && (bits = keys.next(c)) == 0) ++c;
-        if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
-        while (c < c_end) {
-            __syncthreads();
-            rk.store(tK, tid); rv.store(tV, tid);
-            __syncthreads();
+        __syncthreads();                                    // the table is written, the buffers are clear, nobody is left in them
+        if (NB == 2 && c < c_end) fetch(0);
+        for (; c < c_end; buf ^= NB - 1) {
+            if (NB == 1) { __syncthreads(); fetch(0); }
+            rp_landed();                                    // this chunk is there, and nobody reads the buffer of the one before it any more
+            const char* tK = smem + buf * 2 * Ti::BYTES;
+            const char* tV = tK + Ti::BYTES;
             const int key0 = c * 64;
             const uint64_t now = bits;
             do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-            if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+            if (NB == 2 && c < c_end) fetch(buf ^ 1);
             const int rel0 = key0 - (qw + sq.off);
             if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
             const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
@@ -216,15 +224,13 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
 }
 
 template <typename T, int DT, int QT>
-__global__ __launch_bounds__(256, 1) void rp_dkv_kernel(RpArgs a) {
+__global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
+    constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int ND = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD;
-    char* tQ = smem;
-    char* tO = smem + Ti::BYTES;
-    float* rowl = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);       // -lse and -delta of the 64 query rows
-    float* rowd = rowl + 64;
-    float* tab = rowd + 64;                                 // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
+    float* rows = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);       // after the buffers of Q and dout chunks: -lse, -delta of their 64 rows, twice
+    float* tab = rows + 256;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.kv_heads * a.nrb;
@@ -247,6 +253,9 @@ __global__ __launch_bounds__(256, 1) void rp_dkv_kernel(RpArgs a) {
         for (int gi = 0; gi < G; ++gi)
             for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
     float* bw = bins + w * ND;
+    RpStage<T, DT> rq, ro;
+    rq.init(a.sq.st, a.D, w, l); ro.init(a.sdo.st, a.D, w, l);
+    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
     bool again = false;                                     // (a second row block of a sequence longer than the hint adds to the first one's sums)
 
     for (; rb * BK < rows_k; rb += a.nrb) {
@@ -288,12 +297,13 @@ __global__ __launch_bounds__(256, 1) void rp_dkv_kernel(RpArgs a) {
                 for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
             f32x4 sumL = {0.f, 0.f, 0.f, 0.f}, sumR = {0.f, 0.f, 0.f, 0.f};
             const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
-            RpStage<T, DT> rq, ro;
             float rl = 0.f, rd = 0.f;
-            auto fetch = [&](int c) {
+            auto fetch = [&](int c, int at) {
                 const uint64_t ok = rp_low_bits(sq.qn - c * 64);
-                rq.load(qb + (int64_t)c * 64 * a.sq.st, a.sq.st, ok, a.D, tid);
-                ro.load(ob + (int64_t)c * 64 * a.sdo.st, a.sdo.st, ok, a.D, tid);
+                rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + at * 2 * Ti::BYTES, w, l);
+                ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+            };
+            auto fetch_rows = [&](int c) {                  // (through registers: rows that are not there need -inf)
                 if (tid < 64) {
                     const bool in = c * 64 + tid < sq.qn;
                     const float lse = in ? a.lse[row0 + c * 64 + tid] : INFINITY;
@@ -301,13 +311,19 @@ __global__ __launch_bounds__(256, 1) void rp_dkv_kernel(RpArgs a) {
                     rd = in ? -a.delta[row0 + c * 64 + tid] : 0.f;
                 }
             };
-            if (c_first < n_ch) fetch(c_first);
-            for (int c = c_first; c < n_ch; ++c) {
-                __syncthreads();
-                rq.store(tQ, tid); ro.store(tO, tid);
-                if (tid < 64) { rowl[tid] = rl; rowd[tid] = rd; }
-                __syncthreads();
-                if (c + 1 < n_ch) fetch(c + 1);
+            auto put_rows = [&](int at) {
+                if (tid < 64) { rows[at * 128 + tid] = rl; rows[at * 128 + 64 + tid] = rd; }
+            };
+            int buf = 0;
+            if (c_first < n_ch) { fetch_rows(c_first); put_rows(0); fetch_rows(c_first + 1); if (NB == 2) fetch(c_first, 0); }
+            for (int c = c_first; c < n_ch; ++c, buf ^= 1) {
+                if (NB == 1) { __syncthreads(); fetch(c, 0); }
+                rp_landed();
+                const char* tQ = smem + buf * (NB - 1) * 2 * Ti::BYTES;
+                const char* tO = tQ + Ti::BYTES;
+                const float* rowl = rows + buf * 128;
+                const float* rowd = rowl + 64;
+                if (c + 1 < n_ch) { put_rows(buf ^ 1); fetch_rows(c + 2); if (NB == 2) fetch(c + 1, buf ^ 1); }
                 const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
                 if (!wave_any || (a.causal && rel0 + 63 < 0)) continue;
                 const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
@@ -483,7 +499,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
     const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
     if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
-    const int lds = 2 * RpTile<T, DT>::BYTES + ND * 4;
+    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + ND * 4;
     int rc;
     if (n == 0) {
     } else if (sizeof(T) == 4 || qt == 1) {
@@ -497,7 +513,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
     const int64_t m = (int64_t)a.B * a.kv_heads * a.nrb + tail;
     if (m > 0x7fffffff) return AMDSEG_ERR_SHAPE;
-    const int lds2 = 2 * RpTile<T, DT>::BYTES + 512 + ND * 4 * (a.part_d ? 5 : 1);
+    const int lds2 = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + 1024 + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
     } else if (sizeof(T) == 4 || kt == 1) {
         if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 1>, lds2))) return rc;

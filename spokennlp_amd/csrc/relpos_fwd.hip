@@ -9,10 +9,9 @@
 template <typename T, int DT, int QT>
 __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
+    constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* tK = smem;
-    char* tV = smem + Ti::BYTES;
-    float* tab = reinterpret_cast<float*>(smem + 2 * Ti::BYTES);
+    float* tab = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     int id = blockIdx.x;
     const int nmain = a.B * a.heads * a.nrb;
@@ -33,6 +32,9 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
     rp_fill_table(a, tab, h, 1, tid);
+    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
+    RpStage<T, DT> rk, rv;
+    rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
@@ -66,18 +68,24 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
         if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
         RpKeys keys;
         keys.init(a, sq, b, l, c);
-        RpStage<T, DT> rk, rv;
         uint64_t bits = 0;
+        int buf = 0;
+        auto fetch = [&](int at) {
+            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
+            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        };
         while (c < c_end && (bits = keys.next(c)) == 0) ++c;
-        if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
-        while (c < c_end) {
-            __syncthreads();                                // the chunk before has been read (and the table written)
-            rk.store(tK, tid); rv.store(tV, tid);
-            __syncthreads();
+        __syncthreads();                                    // the table is written, the buffers are clear
+        if (NB == 2 && c < c_end) fetch(0);
+        for (; c < c_end; buf ^= NB - 1) {
+            if (NB == 1) { __syncthreads(); fetch(0); }
+            rp_landed();                                    // this chunk is there, and nobody reads the buffer of the one before it any more
+            const char* tK = smem + buf * 2 * Ti::BYTES;
+            const char* tV = tK + Ti::BYTES;
             const int key0 = c * 64;
             const uint64_t now = bits;
             do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-            if (c < c_end) { rk.load(kb + (int64_t)c * 64 * a.sk.st, a.sk.st, bits, a.D, tid); rv.load(vb + (int64_t)c * 64 * a.sv.st, a.sv.st, bits, a.D, tid); }
+            if (NB == 2 && c < c_end) fetch(buf ^ 1);
             const int rel0 = key0 - (qw + sq.off);          // rel of the tile's first key and the wave's first query
             if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
             f32x4 s[QT][4];
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(256) void rp_join_kernel(RpArgs a) {
 
 template <typename T, int DT, int QT>
 static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
-    const int lds = 2 * RpTile<T, DT>::BYTES + (2 * (a.span + RP_PAD) + 1) * 4;
+    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + (2 * (a.span + RP_PAD) + 1) * 4;
     const int rc = rp_allow_lds((const void*)rp_fwd_kernel<T, DT, QT>, lds);
     if (rc) return rc;
     const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);

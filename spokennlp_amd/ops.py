@@ -536,6 +536,8 @@ def _rp_strides(t, name, esize):
     st = [0 if n == 1 else s for n, s in zip(t.shape[:-1], st[:-1])]
     if (t.data_ptr() | (st[-1] * esize) | (st[-2] * esize) | (st[0] * esize)) & 15:
         raise ValueError(f"{name}: rows must start on 16 bytes (strides {t.stride()}, element size {esize})")
+    if not 0 <= st[-2] * esize <= 1 << 24:
+        raise ValueError(f"{name}: rows at most 16 MiB apart (strides {t.stride()}, element size {esize})")
     return (st[0] if len(st) == 3 else 0, st[-2], st[-1])
 
 
