@@ -9,6 +9,7 @@
 // it and scale * log2 e multiplies the finished score inside the exponent's fma.
 #pragma once
 #include <math.h>
+#include <type_traits>
 #include "common.h"
 #include "tile64.h"
 
@@ -74,6 +75,15 @@ __device__ __forceinline__ void rp_place(int id, int nrb, int B, int heads, int 
 // RpTile<T, DT>: [64 rows][DT * 16 columns] in LDS.  A row fragment is the operand whose contraction runs along the columns (K of S^T = K Q^T), a
 // column fragment the one whose contraction runs along the rows (V^T of O^T = V^T P^T).  PF(): accumulator registers of the score tiles as the other
 // operand of that product -- the row order inside a contraction step is the accumulators' own, so the probabilities never move between lanes.
+// two fp32 -> bf16 x 2 (round to nearest even).  The compiler's conversion, not inline asm: an asm statement that reads the result of a transcendental (or
+// matrix) instruction right behind it gets no wait states from the compiler -- v_exp_f32 straight into an asm v_cvt_pk gave now and then the value of before
+typedef __bf16 rp_bf2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t rp_pack2(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, rp_bf2));
+}
+
 template <typename T, int DT> struct RpTile;
 template <int DT> struct RpTile<bf16_t, DT> {
     typedef bf16x8 frag;
@@ -87,7 +97,10 @@ template <int DT> struct RpTile<bf16_t, DT> {
         return at_frag_tr(t + (dt >> 2) * 8192, step * 32 + g * 4, step * 32 + 16 + g * 4, (dt & 3) * 16, l);
     }
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ frag pf(const f32x4* s) { return pack8(s[0], s[1]); }
+    static __device__ __forceinline__ frag pf(const f32x4* s) {
+        const uint4 u = make_uint4(rp_pack2(s[0][0], s[0][1]), rp_pack2(s[0][2], s[0][3]), rp_pack2(s[1][0], s[1][1]), rp_pack2(s[1][2], s[1][3]));
+        return __builtin_bit_cast(frag, u);
+    }
     // the columns kb * 32 + g * 8 .. + 7 of one row of a global tensor, zero beyond D
     static __device__ __forceinline__ frag gfrag(const bf16_t* row, int kb, int g, int D, bool ok) {
         frag f = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -100,7 +113,7 @@ template <int DT> struct RpTile<bf16_t, DT> {
         for (int e = 0; e < 8; ++e) s += bf2f((bf16_t)a[e]) * bf2f((bf16_t)b[e]);
         return s;
     }
-    static __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
+    static __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(rp_pack2(v[0], v[1]), rp_pack2(v[2], v[3])); }
 };
 template <int DT> struct RpTile<float, DT> {
     typedef f32x4 frag;
@@ -182,10 +195,28 @@ template <typename T, int DT> struct RpStage {
         }
     }
 };
-__device__ __forceinline__ void rp_clear_lds(char* p, int bytes, int tid) {
-    for (int x = tid * 16; x < bytes; x += 4096) *reinterpret_cast<uint4*>(p + x) = make_uint4(0u, 0u, 0u, 0u);
+// zeros into the pieces that this wave's own RpStage::load fills, before its first one (no barrier: nobody else writes there)
+template <typename T, int DT>
+__device__ __forceinline__ void rp_clear_own(char* tile, int w, int l) {
+    constexpr int N = RpStage<T, DT>::N;
+#pragma unroll
+    for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(tile + (w * N + n) * 1024 + l * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
+__device__ __forceinline__ void rp_cleared() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void rp_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); __syncthreads(); }
+
+// the bias values of the score tiles whose block diagonal (row tile - column tile) is k0, k0 + 1, ...: lane (g, i16), register r = rel 16 k + 4 g + r - i16
+// (or zeros, where the whole tile is beyond the span)
+template <int N>
+__device__ __forceinline__ void rp_bias_or_zero(bool near, const float* bt, int k0, f32x4 (&z)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (near)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[k][r] = bt[16 * (k0 + k) + r];
+}
 
 // visible keys of a 64-key chunk as a wave-uniform word; the mask byte of the chunk after it is in flight
 struct RpKeys {

@@ -32,12 +32,29 @@ __device__ __forceinline__ void rp_diag_add(f32x4 x, float& lo, float& hi) {
     lo += rp_dpp<0x103>(x[3]); hi += rp_dpp<0x11d>(x[3]);
 }
 
+
+// acc[0..3] are complete block diagonals: their four 16-lane rows (g) hold overlapping rel, so the 4 x 4 rows are exchanged -- afterwards register g holds
+// the g rows of all four diagonals, 64 different bins -- and four adds carry them into the wave's bins (a wave's LDS operations complete in order)
+__device__ __forceinline__ void rp_swap32(float& x, float& y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    x = __uint_as_float(r[0]); y = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void rp_swap16(float& x, float& y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    x = __uint_as_float(r[0]); y = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void rp_flush4(float* bin, float x0, float x1, float x2, float x3, int l) {
+    rp_swap32(x0, x2); rp_swap32(x1, x3);
+    rp_swap16(x0, x1); rp_swap16(x2, x3);
+    bin += 16 * (l >> 4) - (l & 15);
+    atomicAdd(bin, x0); atomicAdd(bin + 4, x1); atomicAdd(bin + 8, x2); atomicAdd(bin + 12, x3);
+}
+
 template <typename T, int DT, int QT>
 __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int mid = a.span + RP_PAD;
     float* tab = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.heads * a.nrb;
@@ -51,175 +68,171 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
-    rp_fill_table(a, tab, h, 1, tid);
-    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
     RpStage<T, DT> rk, rv;
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
+    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    rp_cleared();
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
     const float c2 = a.scale * RP_LOG2E;
-    const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+    const int mid = a.span + RP_PAD, span = a.span;
+    const bool causal = a.causal;
     constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums)
+    bool first = true;
 
     for (; rb * BQ < sq.qn; rb += a.nrb) {
         const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
-        typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
-        float nd[QT], nl[QT];                               // -delta, -lse in the exponent's units
-#pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            const int q = qw + ct * 16 + i16;
-            const bool ok = q < sq.qn;
-            const int64_t qt = (int64_t)(sq.q0 + q);
-            float acc = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < Ti::KB; ++kk) {
-                fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
-                fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
-                acc += Ti::dot(fdo[ct][kk], Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok));
-            }
-            acc += __shfl_xor(acc, 16, 64);
-            acc += __shfl_xor(acc, 32, 64);
-            nd[ct] = -acc;
-            float lse = INFINITY;                           // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
-            if (ok) {
-                const int64_t row = rp_row(a, sq, b, h, q);
-                lse = a.lse[row];
-                if (lse == -INFINITY) lse = INFINITY;
-            }
-            nl[ct] = -lse * RP_LOG2E;
-        }
-        f32x4 dq[QT][DT];
-#pragma unroll
-        for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dq[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        float rsum[QT];                                     // sum of a row's ds (each of its four lanes: a quarter of the keys)
-#pragma unroll
-        for (int ct = 0; ct < QT; ++ct) rsum[ct] = 0.f;
         int c_end = (sq.kn + 63) / 64, c_128 = c_end;
-        if (a.causal) {
+        if (causal) {
             const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
             const int last128 = min(q0 / 128 * 128 + 128, sq.qn) - 1 + sq.off;  // (the rule must not depend on QT)
             c_128 = last128 < 0 ? 0 : min(c_128, last128 / 64 + 1);
         }
-        for (int pass = MEND && c_128 * 64 <= RP_TWICE_KEYS ? 0 : 1; pass < 2; ++pass) {
-        int c = 0;
-        RpKeys keys;
-        keys.init(a, sq, b, l, c);
-        uint64_t bits = 0;
-        int buf = 0;
-        auto fetch = [&](int at) {
-            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
-            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
-        };
-        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
-        __syncthreads();                                    // the table is written, the buffers are clear, nobody is left in them
-        if (NB == 2 && c < c_end) fetch(0);
-        for (; c < c_end; buf ^= NB - 1) {
-            if (NB == 1) { __syncthreads(); fetch(0); }
-            rp_landed();                                    // this chunk is there, and nobody reads the buffer of the one before it any more
-            const char* tK = smem + buf * 2 * Ti::BYTES;
-            const char* tV = tK + Ti::BYTES;
-            const int key0 = c * 64;
-            const uint64_t now = bits;
-            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-            if (NB == 2 && c < c_end) fetch(buf ^ 1);
-            const int rel0 = key0 - (qw + sq.off);
-            if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
-            const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
-            const bool cut = a.causal && rel0 + 63 > 0;
-            const float* bt = tab + (rel0 + mid + 4 * g - i16);
-            const float far = rel0 > 0 ? farR : farL;
+        typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
+        float nl[QT], rsum[QT];                             // -lse in the exponent's units; sum of a row's ds (each of its four lanes: a quarter of the keys)
+        f32x4 nd[QT];                                       // -delta, as what the product dout . v starts from
+        f32x4 dq[QT][DT];
 #pragma unroll
-            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
-                f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS];
+        for (int ct = 0; ct < QT; ++ct) {
+            rsum[ct] = 0.f;
 #pragma unroll
-                for (int ct = 0; ct < QT; ++ct)
+            for (int d = 0; d < DT; ++d) dq[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+        const int pass0 = MEND && c_128 * 64 <= RP_TWICE_KEYS ? 0 : 1;
+        for (int pass = pass0; pass < 2; ++pass) {
+            int c = 0;
+            RpKeys keys;
+            keys.init(a, sq, b, l, c);
+            uint64_t bits = 0;
+            int buf = 0;
+            auto fetch = [&](int at) {
+                rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
+                rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+            };
+            while (c < c_end && (bits = keys.next(c)) == 0) ++c;
+            if (!first) __syncthreads();                    // (nobody is left in the buffers)
+            if (NB == 2 && c < c_end) fetch(0);             // on its way before anything else is waited for
+            if (first) rp_fill_table(a, tab, h, 1, tid);
+            if (pass == pass0) {
 #pragma unroll
-                    for (int j = 0; j < Ti::RPS; ++j) {
-                        const int f = kp * Ti::RPS + j;
-                        if (near) {
+                for (int ct = 0; ct < QT; ++ct) {
+                    const int q = qw + ct * 16 + i16;
+                    const bool ok = q < sq.qn;
+                    const int64_t qt = (int64_t)(sq.q0 + q);
+                    float acc = 0.f;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) s[ct][j][r] = bt[16 * (f - ct) + r];
-                        } else s[ct][j] = (f32x4){far, far, far, far};
-                        dp[ct][j] = (f32x4){nd[ct], nd[ct], nd[ct], nd[ct]};
+                    for (int kk = 0; kk < Ti::KB; ++kk) {
+                        fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
+                        fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
+                        acc += Ti::dot(fdo[ct][kk], Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok));
                     }
+                    acc += __shfl_xor(acc, 16, 64);
+                    acc += __shfl_xor(acc, 32, 64);
+                    nd[ct] = (f32x4){-acc, -acc, -acc, -acc};
+                    float lse = INFINITY;                   // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
+                    if (ok) {
+                        lse = a.lse[rp_row(a, sq, b, h, q)];
+                        if (lse == -INFINITY) lse = INFINITY;
+                    }
+                    nl[ct] = -lse * RP_LOG2E;
+                }
+            }
+            first = false;
+            const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
+            auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
+                const char* tV = tK + Ti::BYTES;
+                const float fc = near ? 0.f : rel0 > 0 ? farR : farL;
+                float al[QT];
 #pragma unroll
-                for (int kk = 0; kk < Ti::KB; ++kk)
+                for (int ct = 0; ct < QT; ++ct) al[ct] = nl[ct] + fc;
+                const float* bt = tab + (rel0 + mid + 4 * g - i16);
 #pragma unroll
-                    for (int j = 0; j < Ti::RPS; ++j) {
-                        const int f = kp * Ti::RPS + j;
-                        const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
+                for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], z[Ti::RPS + QT - 1];
+                    rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
 #pragma unroll
-                        for (int ct = 0; ct < QT; ++ct) {
-                            s[ct][j] = Ti::mma(fk, fq[ct][kk], s[ct][j]);
-                            dp[ct][j] = Ti::mma(fv, fdo[ct][kk], dp[ct][j]);
+                    for (int kk = 0; kk < Ti::KB; ++kk)
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j) {
+                            const int f = kp * Ti::RPS + j;
+                            const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct) {
+                                const f32x4 start = z[j - ct + QT - 1];
+                                s[ct][j] = Ti::mma(fk, fq[ct][kk], kk == 0 ? start : s[ct][j]);
+                                dp[ct][j] = Ti::mma(fv, fdo[ct][kk], kk == 0 ? nd[ct] : dp[ct][j]);
+                            }
+                        }
+                    if (edge) {
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j) {
+                            const int f = kp * Ti::RPS + j;
+                            const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                                for (int ct = 0; ct < QT; ++ct)
+                                    s[ct][j][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][j][r] : -INFINITY;
                         }
                     }
-                if (now != ~0ull) {
+                    typename Ti::frag fds[QT];
 #pragma unroll
-                    for (int j = 0; j < Ti::RPS; ++j) {
-                        const uint32_t nib = (uint32_t)(now >> ((kp * Ti::RPS + j) * 16 + 4 * g));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int ct = 0; ct < QT; ++ct) s[ct][j][r] = (nib >> r) & 1 ? s[ct][j][r] : -INFINITY;
-                    }
-                }
-                if (cut) {
-#pragma unroll
-                    for (int ct = 0; ct < QT; ++ct)
+                    for (int ct = 0; ct < QT; ++ct) {
+                        float sum = 0.f;
 #pragma unroll
                         for (int j = 0; j < Ti::RPS; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 > 0) s[ct][j][r] = -INFINITY;
-                }
-                typename Ti::frag fds[QT];
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct) {
-#pragma unroll
-                    for (int j = 0; j < Ti::RPS; ++j) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, nl[ct]));
-                            dp[ct][j][r] *= p;
-                            if (MEND) rsum[ct] += dp[ct][j][r];
-                        }
+                            for (int r = 0; r < 4; ++r) {
+                                dp[ct][j][r] *= __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, al[ct]));
+                                if (MEND) sum += dp[ct][j][r];
+                            }
+                        rsum[ct] += sum;
+                        fds[ct] = Ti::pf(dp[ct]);
                     }
-                    fds[ct] = Ti::pf(dp[ct]);
-                }
-                if (pass == 0) continue;
+                    if (pass == 0) continue;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
+                    for (int d = 0; d < DT; ++d) {
+                        const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
 #pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
+                        for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
+                    }
                 }
+            };
+            for (; c < c_end; buf ^= NB - 1) {
+                if (NB == 1) { __syncthreads(); fetch(0); }
+                rp_landed();                                // this chunk is there, nobody reads the buffer of the one before it any more
+                const char* tK = smem + buf * 2 * Ti::BYTES;
+                const int rel0 = c * 64 - (qw + sq.off);
+                const uint64_t now = bits;
+                do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
+                if (NB == 2 && c < c_end) fetch(buf ^ 1);
+                if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
+                const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+                chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
             }
-        }
-        if (!MEND) break;
+            if (!MEND) break;
 #pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            rsum[ct] += __shfl_xor(rsum[ct], 16, 64);
-            rsum[ct] += __shfl_xor(rsum[ct], 32, 64);
-            nd[ct] -= rsum[ct];
-            rsum[ct] = 0.f;
-        }
+            for (int ct = 0; ct < QT; ++ct) {
+                float rho = rsum[ct];
+                rho += __shfl_xor(rho, 16, 64);
+                rho += __shfl_xor(rho, 32, 64);
+                const float x = nd[ct][0] - rho;
+                nd[ct] = (f32x4){x, x, x, x};
+                rsum[ct] = 0.f;
+            }
         }
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
             if (q >= sq.qn) continue;
-            if (g == 0) a.delta[rp_row(a, sq, b, h, q)] = -nd[ct];
+            if (g == 0) a.delta[rp_row(a, sq, b, h, q)] = -nd[ct][0];
             T* op = (T*)a.dq + b * a.sdq.sb + (int64_t)(sq.q0 + q) * a.sdq.st + h * a.sdq.sh;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, dq[ct][d] * a.scale);
         }
-        __syncthreads();
     }
 }
 
@@ -228,7 +241,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int ND = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD;
+    const int ND = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD, span = a.span;
     float* rows = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);       // after the buffers of Q and dout chunks: -lse, -delta of their 64 rows, twice
     float* tab = rows + 256;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
@@ -246,6 +259,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     constexpr int BK = 64 * QT;
     const int G = a.heads / a.kv_heads;
     const float c2 = a.scale * RP_LOG2E;
+    const bool causal = a.causal;
     const int rows_k = a.cu_k ? sq.kn : a.Lk;               // padded: rows past k_lens are gradients of zero, and written
     float* part = a.part_d ? a.part_d + ((int64_t)hk * G * a.B * a.nrb + (int64_t)b * a.nrb + rb) * ND : nullptr;     // of the group's first head
     const int64_t part_h = (int64_t)a.B * a.nrb * ND;
@@ -255,7 +269,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     float* bw = bins + w * ND;
     RpStage<T, DT> rq, ro;
     rq.init(a.sq.st, a.D, w, l); ro.init(a.sdo.st, a.D, w, l);
-    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
+    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    rp_cleared();
     bool again = false;                                     // (a second row block of a sequence longer than the hint adds to the first one's sums)
 
     for (; rb * BK < rows_k; rb += a.nrb) {
@@ -285,18 +300,13 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
         const int n_ch = wg_any ? (sq.qn + 63) / 64 : 0;
         int c_first = 0;
-        if (a.causal) c_first = max(0, k0 - sq.off) / 64;   // query rows before k0 - off see none of these keys
+        if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
         for (int gi = 0; gi < G; ++gi) {
             const int h = hk * G + gi;
             const T* qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
             const T* ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
-            const int64_t row0 = rp_row(a, sq, b, h, 0);
-            __syncthreads();
-            rp_fill_table(a, tab, h, -1, tid);
-            if (part)
-                for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
-            f32x4 sumL = {0.f, 0.f, 0.f, 0.f}, sumR = {0.f, 0.f, 0.f, 0.f};
-            const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+            const float* lse_h = a.lse + rp_row(a, sq, b, h, 0);
+            const float* delta_h = a.delta + rp_row(a, sq, b, h, 0);
             float rl = 0.f, rd = 0.f;
             auto fetch = [&](int c, int at) {
                 const uint64_t ok = rp_low_bits(sq.qn - c * 64);
@@ -306,54 +316,52 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             auto fetch_rows = [&](int c) {                  // (through registers: rows that are not there need -inf)
                 if (tid < 64) {
                     const bool in = c * 64 + tid < sq.qn;
-                    const float lse = in ? a.lse[row0 + c * 64 + tid] : INFINITY;
+                    const float lse = in ? lse_h[c * 64 + tid] : INFINITY;
                     rl = lse == -INFINITY ? -INFINITY : -lse * RP_LOG2E;
-                    rd = in ? -a.delta[row0 + c * 64 + tid] : 0.f;
+                    rd = in ? -delta_h[c * 64 + tid] : 0.f;
                 }
             };
             auto put_rows = [&](int at) {
                 if (tid < 64) { rows[at * 128 + tid] = rl; rows[at * 128 + 64 + tid] = rd; }
             };
             int buf = 0;
-            if (c_first < n_ch) { fetch_rows(c_first); put_rows(0); fetch_rows(c_first + 1); if (NB == 2) fetch(c_first, 0); }
-            for (int c = c_first; c < n_ch; ++c, buf ^= 1) {
-                if (NB == 1) { __syncthreads(); fetch(c, 0); }
-                rp_landed();
-                const char* tQ = smem + buf * (NB - 1) * 2 * Ti::BYTES;
+            __syncthreads();                                // (nobody is left in the buffers, the table, the bins)
+            if (c_first < n_ch) {
+                if (NB == 2) fetch(c_first, 0);
+                fetch_rows(c_first);
+            }
+            rp_fill_table(a, tab, h, -1, tid);
+            if (part)
+                for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
+            const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
+            f32x4 far_sum = {0.f, 0.f, 0.f, 0.f};           // one side at a time: the chunks come in the order of -rel
+            auto commit = [&](int at) {
+                const float t = wave_sum(far_sum[0] + far_sum[1] + far_sum[2] + far_sum[3]);
+                if (l == 0) bw[at] += t;
+                far_sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+            };
+            int side = 0;                                   // -1: rel >= span summed so far, 1: rel <= -span
+            float diag[4 + QT];                             // block diagonals 1 - QT .. 4 of the chunk
+#pragma unroll
+            for (int k = 0; k < 4 + QT; ++k) diag[k] = 0.f;
+            if (c_first < n_ch) { put_rows(0); fetch_rows(c_first + 1); }
+            auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0) __attribute__((always_inline)) {
                 const char* tO = tQ + Ti::BYTES;
-                const float* rowl = rows + buf * 128;
                 const float* rowd = rowl + 64;
-                if (c + 1 < n_ch) { put_rows(buf ^ 1); fetch_rows(c + 2); if (NB == 2) fetch(c + 1, buf ^ 1); }
-                const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
-                if (!wave_any || (a.causal && rel0 + 63 < 0)) continue;
-                const bool near = rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span;
-                const bool cut = a.causal && rel0 - (16 * QT - 1) < 0;
                 const float* bt = tab + (rel0 + mid + 4 * g - i16);
-                const float far = rel0 > 0 ? farL : farR;
-                float diag[5 + QT], col[QT];                // block diagonals -(QT - 1) .. 4, and one above; what a far column starts from
-                f32x4 fsum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < 5 + QT; ++k) diag[k] = 0.f;
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct) col[ct] = seen[ct] ? far : -INFINITY;
+                const float fc = near ? 0.f : rel0 > 0 ? farL : farR;
 #pragma unroll
                 for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
-                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS];
+                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS], dr[Ti::RPS], z[Ti::RPS + QT - 1];
+                    rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
 #pragma unroll
                     for (int j = 0; j < Ti::RPS; ++j) {
                         const int f = kp * Ti::RPS + j;
                         lr[j] = *reinterpret_cast<const f32x4*>(rowl + f * 16 + g * 4);
-                        const f32x4 d4 = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
+                        dr[j] = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
+                        if (!near) {
 #pragma unroll
-                        for (int ct = 0; ct < QT; ++ct) {
-                            if (near) {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) s[ct][j][r] = bt[16 * (f - ct) + r];
-                                if (!wave_all)              // a hidden key's column: p = 0
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) s[ct][j][r] = seen[ct] ? s[ct][j][r] : -INFINITY;
-                            } else s[ct][j] = (f32x4){col[ct], col[ct], col[ct], col[ct]};
-                            dp[ct][j] = d4;
+                            for (int r = 0; r < 4; ++r) lr[j][r] += fc;
                         }
                     }
 #pragma unroll
@@ -364,18 +372,19 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                             const typename Ti::frag fq = Ti::rowf(tQ, f * 16 + i16, kk, g), fo = Ti::rowf(tO, f * 16 + i16, kk, g);
 #pragma unroll
                             for (int ct = 0; ct < QT; ++ct) {
-                                s[ct][j] = Ti::mma(fq, fk[ct][kk], s[ct][j]);
-                                dp[ct][j] = Ti::mma(fo, fv[ct][kk], dp[ct][j]);
+                                const f32x4 start = z[j - ct + QT - 1];
+                                s[ct][j] = Ti::mma(fq, fk[ct][kk], kk == 0 ? start : s[ct][j]);
+                                dp[ct][j] = Ti::mma(fo, fv[ct][kk], kk == 0 ? dr[j] : dp[ct][j]);
                             }
                         }
-                    if (cut) {
+                    if (edge) {                             // a hidden key's column, rel > 0 with `causal`: p = 0
 #pragma unroll
                         for (int ct = 0; ct < QT; ++ct)
 #pragma unroll
                             for (int j = 0; j < Ti::RPS; ++j)
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 < 0) s[ct][j][r] = -INFINITY;
+                                    s[ct][j][r] = seen[ct] && !(causal && rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 < 0) ? s[ct][j][r] : -INFINITY;
                     }
                     typename Ti::frag fp[QT], fds[QT];
 #pragma unroll
@@ -388,16 +397,35 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                                 s[ct][j][r] = p;
                                 dp[ct][j][r] *= p;
                             }
-                        if (part) {
-#pragma unroll
-                            for (int j = 0; j < Ti::RPS; ++j) {
-                                const int k = kp * Ti::RPS + j - ct + QT - 1;
-                                if (near) rp_diag_add(dp[ct][j], diag[k], diag[k + 1]);
-                                else fsum += dp[ct][j];
-                            }
-                        }
                         fp[ct] = Ti::pf(s[ct]);
                         fds[ct] = Ti::pf(dp[ct]);
+                    }
+                    if (part) {
+                        if (near) {
+                            // tiles of one block diagonal first add up element by element
+#pragma unroll
+                            for (int k = 0; k < Ti::RPS + QT - 1; ++k) {
+                                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                                bool have = false;
+#pragma unroll
+                                for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                                    for (int ct = 0; ct < QT; ++ct)
+                                        if (j - ct + QT - 1 == k) {
+                                            if (have) {
+#pragma unroll
+                                                for (int r = 0; r < 4; ++r) x[r] += dp[ct][j][r];
+                                            } else x = dp[ct][j];
+                                            have = true;
+                                        }
+                                rp_diag_add(x, diag[kp * Ti::RPS + k], diag[kp * Ti::RPS + k + 1]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                                for (int j = 0; j < Ti::RPS; ++j) far_sum += dp[ct][j];
+                        }
                     }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
@@ -409,23 +437,42 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                         }
                     }
                 }
-                if (part) {
-                    if (near) {
-                        // 16 lanes at a time: inside one instruction no two lanes meet in a bin, and a wave's LDS operations complete in order
-                        float* bd = bw + (rel0 - 16 * (QT - 1) + mid + 4 * g - i16);
+            };
+            for (int c = c_first; c < n_ch; ++c, buf ^= 1) {
+                if (NB == 1) { __syncthreads(); fetch(c, 0); }
+                rp_landed();
+                const char* tQ = smem + buf * (NB - 1) * 2 * Ti::BYTES;
+                const float* rowl = rows + buf * 128;
+                if (c + 1 < n_ch) { put_rows(buf ^ 1); fetch_rows(c + 2); if (NB == 2) fetch(c + 1, buf ^ 1); }
+                const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
+                if (!wave_any || (causal && rel0 + 63 < 0)) continue;
+                const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+                if (part && side < 0 && rel0 > 0) { commit(0); side = 0; }
+                if (part && !near) side = rel0 > 0 ? 1 : -1;
+                chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0), tQ, rowl, rel0);
+                if (part && near) {
+                    float* bd = bw + (rel0 - 16 * (QT - 1) + mid);
+                    rp_flush4(bd, diag[0], diag[1], diag[2], diag[3], l);
+                    // the upper ones go on into the next chunk, 64 rel further; after the last near chunk they are flushed too (rows of 16 lanes one at a
+                    // time: they overlap)
+#pragma unroll
+                    for (int k = 0; k < QT; ++k) diag[k] = diag[4 + k];
+#pragma unroll
+                    for (int k = QT; k < 4 + QT; ++k) diag[k] = 0.f;
+                    if (c + 1 >= n_ch || rel0 + 64 - (16 * QT - 1) >= span) {
 #pragma unroll
                         for (int gg = 0; gg < 4; ++gg)
                             if (g == gg)
 #pragma unroll
-                                for (int k = 0; k < 4 + QT; ++k) atomicAdd(bd + 16 * k, diag[k]);
-                    } else if (rel0 > 0) sumL += fsum;
-                    else sumR += fsum;
+                                for (int k = 0; k < QT; ++k) atomicAdd(bd + 64 + 16 * k + 4 * g - i16, diag[k]);
+#pragma unroll
+                        for (int k = 0; k < QT; ++k) diag[k] = 0.f;
+                    }
                 }
             }
             if (part) {
-                const float L = wave_sum(sumL[0] + sumL[1] + sumL[2] + sumL[3]), R = wave_sum(sumR[0] + sumR[1] + sumR[2] + sumR[3]);
                 if (c_first >= n_ch) __syncthreads();       // (the zeroed bins: no chunk's barrier came in between)
-                if (l == 0) { bw[0] += R; bw[ND - 1] += L; }
+                if (side) commit(side < 0 ? 0 : ND - 1);
                 __syncthreads();
                 for (int x = tid; x < ND; x += 256) {
                     const float t = (bins[x] + bins[ND + x]) + (bins[2 * ND + x] + bins[3 * ND + x]);
@@ -450,7 +497,6 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                     Ti::st4(vp_ + d * 16 + g * 4, seen[ct] ? dv[ct][d] : z);
                 }
         }
-        __syncthreads();
     }
 }
 

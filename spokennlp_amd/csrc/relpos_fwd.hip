@@ -31,20 +31,40 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
-    rp_fill_table(a, tab, h, 1, tid);
-    rp_clear_lds(smem, NB * 2 * Ti::BYTES, tid);
     RpStage<T, DT> rk, rv;
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
+    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    rp_cleared();
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
     const T* qbase = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
     const float c2 = a.scale * RP_LOG2E;
-    const int mid = a.span + RP_PAD;
-    const float farL = rp_table(a, -a.span, h) / a.scale, farR = rp_table(a, a.span, h) / a.scale;
+    const int mid = a.span + RP_PAD, span = a.span;
+    const bool causal = a.causal;
+    bool first = true;
 
     for (; rb * BQ < sq.qn; rb += a.nrb) {
         const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
+        int c = 0, c_end = (sq.kn + 63) / 64;
+        if (causal) {
+            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;                  // the last key any row of the block sees
+            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
+        }
+        if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
+        RpKeys keys;
+        keys.init(a, sq, b, l, c);
+        uint64_t bits = 0;
+        int buf = 0;
+        auto fetch = [&](int at) {
+            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
+            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        };
+        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
+        if (NB == 2 && c < c_end) fetch(0);                 // on its way before anything else is waited for
+        if (first) rp_fill_table(a, tab, h, 1, tid);
+        first = false;
+        const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
         typename Ti::frag fq[QT][Ti::KB];
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
@@ -60,77 +80,33 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
-        int c = 0, c_end = (sq.kn + 63) / 64;
-        if (a.causal) {
-            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;                  // the last key any row of the block sees
-            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
-        }
-        if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
-        RpKeys keys;
-        keys.init(a, sq, b, l, c);
-        uint64_t bits = 0;
-        int buf = 0;
-        auto fetch = [&](int at) {
-            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
-            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
-        };
-        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
-        __syncthreads();                                    // the table is written, the buffers are clear
-        if (NB == 2 && c < c_end) fetch(0);
-        for (; c < c_end; buf ^= NB - 1) {
-            if (NB == 1) { __syncthreads(); fetch(0); }
-            rp_landed();                                    // this chunk is there, and nobody reads the buffer of the one before it any more
-            const char* tK = smem + buf * 2 * Ti::BYTES;
+        // one chunk: `near` = some |rel| < span (scores start from the table; else from 0, and the constant joins in the exponent), `edge` = some (i, j) hidden
+        auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
             const char* tV = tK + Ti::BYTES;
-            const int key0 = c * 64;
-            const uint64_t now = bits;
-            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-            if (NB == 2 && c < c_end) fetch(buf ^ 1);
-            const int rel0 = key0 - (qw + sq.off);          // rel of the tile's first key and the wave's first query
-            if (qw >= sq.qn || (a.causal && rel0 - (16 * QT - 1) > 0)) continue;
-            f32x4 s[QT][4];
-            if (rel0 + 63 > -a.span && rel0 - (16 * QT - 1) < a.span) {
-                const float* bt = tab + (rel0 + mid + 4 * g - i16);
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) s[ct][f][r] = bt[16 * (f - ct) + r];
-            } else {
-                const float x = rel0 > 0 ? farR : farL;
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) s[ct][f] = (f32x4){x, x, x, x};
-            }
+            f32x4 s[QT][4], z[3 + QT];
+            rp_bias_or_zero(near, tab + (rel0 + mid + 4 * g - i16), 1 - QT, z);
 #pragma unroll
             for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
                 for (int f = 0; f < 4; ++f) {
                     const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g);
 #pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) s[ct][f] = Ti::mma(fk, fq[ct][kk], s[ct][f]);
+                    for (int ct = 0; ct < QT; ++ct) {
+                        s[ct][f] = Ti::mma(fk, fq[ct][kk], kk == 0 ? z[f - ct + QT - 1] : s[ct][f]);
+                    }
                 }
-            if (now != ~0ull) {
+            if (edge) {
 #pragma unroll
                 for (int f = 0; f < 4; ++f) {
                     const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int ct = 0; ct < QT; ++ct) s[ct][f][r] = (nib >> r) & 1 ? s[ct][f][r] : -INFINITY;
+                        for (int ct = 0; ct < QT; ++ct)
+                            s[ct][f][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][f][r] : -INFINITY;
                 }
             }
-            if (a.causal && rel0 + 63 > 0) {
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) s[ct][f][r] = -INFINITY;
-            }
+            const float fc = near ? 0.f : rel0 > 0 ? farR : farL;
 #pragma unroll
             for (int ct = 0; ct < QT; ++ct) {
                 float mx = s[ct][0][0];
@@ -138,7 +114,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                 for (int f = 0; f < 4; ++f)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[ct][f][r]);
-                mx *= c2;
+                mx = fmaf(mx, c2, fc);
                 if (__any(mx > m_run[ct])) {                // wave-uniform: some row's running maximum grows
                     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -151,13 +127,13 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) o[ct][d][r] *= al;
                 }
-                const float mu = m_run[ct] == -INFINITY ? 0.f : m_run[ct];
+                const float mu = fc - (m_run[ct] == -INFINITY ? 0.f : m_run[ct]);
                 float sum = 0.f;
 #pragma unroll
                 for (int f = 0; f < 4; ++f)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[ct][f][r], c2, -mu));
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[ct][f][r], c2, mu));
                         s[ct][f][r] = e;
                         sum += e;
                     }
@@ -175,6 +151,18 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                     for (int ct = 0; ct < QT; ++ct) o[ct][d] = Ti::mma(fv, fp[ct], o[ct][d]);
                 }
             }
+        };
+        for (; c < c_end; buf ^= NB - 1) {
+            if (NB == 1) { __syncthreads(); fetch(0); }
+            rp_landed();                                    // this chunk is there (and the table), nobody reads the buffer of the one before it any more
+            const char* tK = smem + buf * 2 * Ti::BYTES;
+            const int rel0 = c * 64 - (qw + sq.off);        // rel of the chunk's first key and the wave's first query
+            const uint64_t now = bits;
+            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
+            if (NB == 2 && c < c_end) fetch(buf ^ 1);
+            if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
+            const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+            chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
         }
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
