@@ -705,7 +705,7 @@ static size_t relpos_up(size_t n) { return (n + 255) / 256 * 256; }
 static size_t relpos_rows(const RpArgs& a) { return a.cu_q ? (size_t)a.heads * a.Tq : (size_t)a.B * a.heads * a.Lq; }
 static size_t relpos_bwd_ws(const RpArgs& a, int dtype, size_t* sums_at, size_t* part_at) {
     const size_t nd = 2 * ((size_t)a.span + RP_PAD) + 1, bk = 64 * rp_dkv_qt(a, dtype), nrb = (a.Lk + bk - 1) / bk;
-    *sums_at = relpos_up(4 * relpos_rows(a));
+    *sums_at = relpos_up(8 * relpos_rows(a));
     *part_at = *sums_at + relpos_up(4 * nd * a.heads);
     return *part_at + relpos_up(4 * nd * a.heads * a.B * nrb);
 }
@@ -747,7 +747,7 @@ int amdseg_relpos_attn_bwd(const struct amdseg_relpos_cfg* c, const void* q, con
     size_t sums_at, part_at;
     if (!ws || ((uintptr_t)ws & 15) || ws_bytes < relpos_bwd_ws(a, c->dtype, &sums_at, &part_at)) return AMDSEG_ERR_ARG;
     a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.lse = (float*)lse; a.dq = dq; a.dk = dk; a.dv = dv;
-    a.delta = (float*)ws;
+    a.stat = (float*)ws;
     a.part_d = dtable ? (float*)((char*)ws + part_at) : nullptr;
     return amdseg_relpos_bwd_impl(a, c->dtype, dtable, (float*)((char*)ws + sums_at), S(stream));
 }

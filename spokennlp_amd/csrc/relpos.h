@@ -9,7 +9,7 @@
 // it and scale * log2 e multiplies the finished score inside the exponent's fma.
 #pragma once
 #include <math.h>
-#include <type_traits>
+#include <algorithm>
 #include "common.h"
 #include "tile64.h"
 
@@ -30,9 +30,10 @@ struct RpArgs {
     int B, Lq, Lk, heads, kv_heads, D, Tq, Tk, span, buckets, causal, align_end, zero_tail;
     float scale;
     int nrb;                    // row blocks of a sequence (grid); a workgroup steps by it, so a wrong `longest` hint costs time, never rows
+    int mask_words;             // 8-byte words of the key mask in LDS
     int nsplit;                 // forward: splits over the keys
     float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
-    float* delta;               // backward: sum_j p_ij dp_ij
+    float* stat;                // backward: what the dK / dV kernel needs of a row: -lse in the exponent's units [rows], -sum_j p_ij dp_ij [rows]
     float* part_d;              // backward: [heads][B * nrb][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
 };
 
@@ -155,7 +156,7 @@ __device__ __forceinline__ void rp_glds16(const void* uniform_base, uint32_t lan
 }
 
 // chunk buffers: two (the next chunk lands under this one's products), one where two would leave a CU a single workgroup (fp32, D > 64: the other
-// workgroup's products hide the wait)
+// workgroup's products hide the wait).  A third one, two chunks of lead, measured no faster at any length: 32 x 512 backward 83 + 147 us against 77 + 135.
 template <typename T, int DT> constexpr int rp_nb = DT * sizeof(T) >= 32 ? 1 : 2;
 
 // 64 rows of a tensor global -> LDS by the DMA path, 1 KiB a wave and instruction, no register in between.  The swizzle sits on the global side (lane l
@@ -218,36 +219,73 @@ __device__ __forceinline__ void rp_bias_or_zero(bool near, const float* bt, int 
             for (int r = 0; r < 4; ++r) z[k][r] = bt[16 * (k0 + k) + r];
 }
 
-// visible keys of a 64-key chunk as a wave-uniform word; the mask byte of the chunk after it is in flight
-struct RpKeys {
-    const uint8_t* m; int kn, lane; uint32_t nxt;
-    __device__ __forceinline__ uint32_t byte(int c) const {
-        const int key = c * 64 + lane;
-        return key < kn ? (m ? (uint32_t)m[key] : 1u) : 0u;
-    }
-    __device__ __forceinline__ void init(const RpArgs& a, const RpSeq& s, int b, int lane_, int c) {
-        m = a.key_mask ? a.key_mask + (a.cu_k ? (int64_t)s.k0 : (int64_t)b * a.mask_sb) : nullptr;
-        kn = s.kn; lane = lane_; nxt = byte(c);
-    }
-    __device__ __forceinline__ uint64_t next(int c) {       // the word of chunk c; the loads of chunk c + 1 go out
-        const uint64_t w = __ballot(nxt != 0);
-        nxt = byte(c + 1);
-        return w;
-    }
-};
 __device__ __forceinline__ uint64_t rp_low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
-__device__ __forceinline__ float rp_table(const RpArgs& a, int rel, int h) {
-    const int bk = rp_clamp(a.map[rp_clamp(rel, -a.span, a.span) + a.span], 0, a.buckets - 1);
-    const int64_t at = (int64_t)bk * a.heads + h;
+// visible keys of a 64-key chunk as a wave-uniform word.  A key mask is turned into words in LDS by the workgroup before its first chunk (the chunk loop
+// then has no load of its own whose wait would drain the chunks under way); only chunks beyond RP_MASK_WORDS (or a packed batch's hint) are looked up as
+// they come.
+#define RP_MASK_WORDS 1024
+struct RpKeys {
+    const uint8_t* m; const uint64_t* words; int kn, lane, nw;
+    __device__ __forceinline__ void init(const RpArgs& a, const RpSeq& s, int b, int lane_, uint64_t* lds) {
+        m = a.key_mask ? a.key_mask + (a.cu_k ? (int64_t)s.k0 : (int64_t)b * a.mask_sb) : nullptr;
+        words = lds; kn = s.kn; lane = lane_; nw = a.mask_words;
+    }
+    __device__ __forceinline__ uint64_t look(int c) const { const int key = c * 64 + lane; return __ballot(key < kn && m[key] != 0); }
+    __device__ __forceinline__ void build(uint64_t* lds, int w) const {       // (only with a mask; a barrier follows)
+        const int n = min((kn + 63) / 64, nw);
+        for (int c = w; c < n; c += 16) {
+            uint32_t v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { const int key = (c + 4 * u) * 64 + lane; v[u] = key < kn ? m[key] : 0; }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t x = __ballot(v[u] != 0);
+                if (lane == 0 && c + 4 * u < n) lds[c + 4 * u] = x;
+            }
+        }
+    }
+    __device__ __forceinline__ uint64_t bits(int c) const {
+        if (!m) return rp_low_bits(kn - c * 64);
+        if (c >= nw) return look(c);
+        const uint64_t x = words[c];
+        return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
+    }
+    // the next chunk from c on that holds a visible key
+    __device__ __forceinline__ int seek(int c, int c_end, uint64_t& w) const {
+        w = 0;
+        while (c < c_end && (w = bits(c)) == 0) ++c;
+        return c;
+    }
+};
+static inline int rp_mask_bytes(const RpArgs& a) { return a.key_mask ? 8 * std::min((a.Lk + 63) / 64, RP_MASK_WORDS) : 0; }
+
+// LDS floats [2 (span + RP_PAD) + 1]: entry x = bias of rel = sign * (x - span - RP_PAD), divided by the scale.  Two dependent loads an entry: the first goes
+// out with everything else a workgroup begins with (start), the second with its rows (finish), so that a workgroup pays two latencies before its
+// first product and not one per load -- of 55 us for 32 x 512 forward 20 were such waits.
+__device__ __forceinline__ float rp_table(const RpArgs& a, int bk, int h) {
+    const int64_t at = (int64_t)rp_clamp(bk, 0, a.buckets - 1) * a.heads + h;
     return a.table_bf16 ? bf2f(((const bf16_t*)a.table)[at]) : ((const float*)a.table)[at];
 }
-// LDS floats [2 (span + RP_PAD) + 1]: entry x = bias of rel = sign * (x - span - RP_PAD), divided by the scale
-__device__ __forceinline__ void rp_fill_table(const RpArgs& a, float* tab, int h, int sign, int tid) {
-    const int n = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD;
-    const float inv = 1.0f / a.scale;
-    for (int x = tid; x < n; x += 256) tab[x] = rp_table(a, sign * (x - mid), h) * inv;
-}
+struct RpTable {
+    int bk[2], n, mid, sign, tid;
+    __device__ __forceinline__ int map(const RpArgs& a, int x) const { return a.map[rp_clamp(sign * (x - mid), -a.span, a.span) + a.span]; }
+    __device__ __forceinline__ void start(const RpArgs& a, int sign_, int tid_) {
+        mid = a.span + RP_PAD; n = 2 * mid + 1; sign = sign_; tid = tid_;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) bk[u] = tid + 256 * u < n ? map(a, tid + 256 * u) : 0;
+    }
+    __device__ __forceinline__ void finish(const RpArgs& a, float* tab, int h) const {
+        const float inv = 1.0f / a.scale;
+        float v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) v[u] = rp_table(a, bk[u], h);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (tid + 256 * u < n) tab[tid + 256 * u] = v[u] * inv;
+        for (int x = tid + 512; x < n; x += 256) tab[x] = rp_table(a, map(a, x), h) * inv;
+    }
+};
 // zero rows [0, lead) and [end, T) of a packed tensor: `which` of `nwg` workgroups
 template <typename T>
 __device__ __forceinline__ void rp_zero_rows(T* p, const RpTensor& s, int heads, int D, int lead, int end, int T_, int which, int nwg, int tid) {

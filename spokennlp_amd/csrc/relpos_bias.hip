@@ -11,7 +11,7 @@ __global__ __launch_bounds__(256) void rp_bias_kernel(RpArgs a, int off, int row
     extern __shared__ float val[];
     constexpr int E = 16 / sizeof(T);
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, h = blockIdx.y;
-    for (int x = tid; x <= 2 * a.span; x += 256) val[x + (x >> 3)] = rp_table(a, x - a.span, h);
+    for (int x = tid; x <= 2 * a.span; x += 256) val[x + (x >> 3)] = rp_table(a, a.map[x], h);
     __syncthreads();
     const int i0 = blockIdx.x * rows_per_wg, i1 = min(i0 + rows_per_wg, a.Lq);
     for (int i = i0 + w; i < i1; i += 4) {

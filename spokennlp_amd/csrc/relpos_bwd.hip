@@ -55,7 +55,8 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* tab = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks
+    uint64_t* words = reinterpret_cast<uint64_t*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks: the mask's words, the table
+    float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.heads * a.nrb;
     if ((int)blockIdx.x >= nmain) {
@@ -68,10 +69,16 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
+    RpTable table;
+    table.start(a, 1, tid);
     RpStage<T, DT> rk, rv;
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
-    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    RpKeys keys;
+    keys.init(a, sq, b, l, words);
+    if (keys.m || sq.kn % 64 || a.D != DT * 16)             // (something of a chunk is not fetched)
+        for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
     rp_cleared();
+    if (keys.m) { keys.build(words, w); __syncthreads(); }
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
@@ -79,6 +86,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     const int mid = a.span + RP_PAD, span = a.span;
     const bool causal = a.causal;
     constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums)
+    const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
     bool first = true;
 
     for (; rb * BQ < sq.qn; rb += a.nrb) {
@@ -102,48 +110,46 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         }
         const int pass0 = MEND && c_128 * 64 <= RP_TWICE_KEYS ? 0 : 1;
         for (int pass = pass0; pass < 2; ++pass) {
-            int c = 0;
-            RpKeys keys;
-            keys.init(a, sq, b, l, c);
-            uint64_t bits = 0;
-            int buf = 0;
-            auto fetch = [&](int at) {
-                rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
-                rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+            auto fetch = [&](int at, int buf, uint64_t bits) {
+                rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
+                rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
             };
-            while (c < c_end && (bits = keys.next(c)) == 0) ++c;
+            uint64_t bits;
+            int c = keys.seek(0, c_end, bits), buf = 0;
             if (!first) __syncthreads();                    // (nobody is left in the buffers)
-            if (NB == 2 && c < c_end) fetch(0);             // on its way before anything else is waited for
-            if (first) rp_fill_table(a, tab, h, 1, tid);
+            if (NB == 2 && c < c_end) fetch(c, 0, bits);    // on its way before anything else is waited for
             if (pass == pass0) {
+                typename Ti::frag fo[QT][Ti::KB];
+                float lse[QT];                              // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
 #pragma unroll
                 for (int ct = 0; ct < QT; ++ct) {
                     const int q = qw + ct * 16 + i16;
                     const bool ok = q < sq.qn;
                     const int64_t qt = (int64_t)(sq.q0 + q);
-                    float acc = 0.f;
 #pragma unroll
                     for (int kk = 0; kk < Ti::KB; ++kk) {
                         fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
                         fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
-                        acc += Ti::dot(fdo[ct][kk], Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok));
+                        fo[ct][kk] = Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok);
                     }
+                    lse[ct] = ok ? a.lse[rp_row(a, sq, b, h, q)] : INFINITY;
+                }
+                if (first) table.finish(a, tab, h);
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) {
+                    float acc = 0.f;
+#pragma unroll
+                    for (int kk = 0; kk < Ti::KB; ++kk) acc += Ti::dot(fdo[ct][kk], fo[ct][kk]);
                     acc += __shfl_xor(acc, 16, 64);
                     acc += __shfl_xor(acc, 32, 64);
                     nd[ct] = (f32x4){-acc, -acc, -acc, -acc};
-                    float lse = INFINITY;                   // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
-                    if (ok) {
-                        lse = a.lse[rp_row(a, sq, b, h, q)];
-                        if (lse == -INFINITY) lse = INFINITY;
-                    }
-                    nl[ct] = -lse * RP_LOG2E;
+                    nl[ct] = lse[ct] == -INFINITY ? -INFINITY : -lse[ct] * RP_LOG2E;
                 }
             }
             first = false;
-            const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
             auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
                 const char* tV = tK + Ti::BYTES;
-                const float fc = near ? 0.f : rel0 > 0 ? farR : farL;
+                const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
                 float al[QT];
 #pragma unroll
                 for (int ct = 0; ct < QT; ++ct) al[ct] = nl[ct] + fc;
@@ -200,14 +206,15 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                     }
                 }
             };
-            for (; c < c_end; buf ^= NB - 1) {
-                if (NB == 1) { __syncthreads(); fetch(0); }
+            while (c < c_end) {
+                if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
                 rp_landed();                                // this chunk is there, nobody reads the buffer of the one before it any more
                 const char* tK = smem + buf * 2 * Ti::BYTES;
                 const int rel0 = c * 64 - (qw + sq.off);
                 const uint64_t now = bits;
-                do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-                if (NB == 2 && c < c_end) fetch(buf ^ 1);
+                c = keys.seek(c + 1, c_end, bits);
+                buf ^= NB - 1;
+                if (NB == 2 && c < c_end) fetch(c, buf, bits);
                 if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
                 const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
                 chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
@@ -227,7 +234,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
             if (q >= sq.qn) continue;
-            if (g == 0) a.delta[rp_row(a, sq, b, h, q)] = -nd[ct][0];
+            if (g == 0) { a.stat[rp_row(a, sq, b, h, q)] = nl[ct]; a.stat[rows + rp_row(a, sq, b, h, q)] = nd[ct][0]; }
             T* op = (T*)a.dq + b * a.sdq.sb + (int64_t)(sq.q0 + q) * a.sdq.st + h * a.sdq.sh;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -242,8 +249,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int ND = 2 * (a.span + RP_PAD) + 1, mid = a.span + RP_PAD, span = a.span;
-    float* rows = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);       // after the buffers of Q and dout chunks: -lse, -delta of their 64 rows, twice
-    float* tab = rows + 256;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
+    float* rows = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);       // after the buffers of Q and dout chunks: the stat of their 64 rows
+    float* tab = rows + NB * 128;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.kv_heads * a.nrb;
@@ -267,73 +274,84 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
         for (int gi = 0; gi < G; ++gi)
             for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
     float* bw = bins + w * ND;
+    RpTable table;
+    table.start(a, -1, tid);
     RpStage<T, DT> rq, ro;
     rq.init(a.sq.st, a.D, w, l); ro.init(a.sdo.st, a.D, w, l);
-    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    if (sq.qn % 64 || a.D != DT * 16) {                     // (something of a chunk is not fetched)
+        for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+        if (w == 0)
+            for (int x = l; x < NB * 128; x += 64) rows[x] = 0.f;
+    }
     rp_cleared();
+    const int64_t all_rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
     bool again = false;                                     // (a second row block of a sequence longer than the hint adds to the first one's sums)
 
     for (; rb * BK < rows_k; rb += a.nrb) {
         const int k0 = rb * BK, kw = k0 + w * 16 * QT;
+        int c_first = 0, n_ch = (sq.qn + 63) / 64;
+        if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
+        const T *qb, *ob;
+        const float* stat_h;
+        auto fetch = [&](int c, int buf) {
+            const uint64_t ok = rp_low_bits(sq.qn - c * 64);
+            rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + buf * 2 * Ti::BYTES, w, l);
+            ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
+            if (w == 0 && ((ok >> l) & 1)) {                // 64 rows' stat: 4 bytes a lane
+                amdseg_glds4(stat_h + c * 64 + l, rows + buf * 128);
+                amdseg_glds4(stat_h + all_rows + c * 64 + l, rows + buf * 128 + 64);
+            }
+        };
+        auto head = [&](int gi) {                           // a head's first chunk, on its way before anything else is waited for
+            const int h = hk * G + gi;
+            qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
+            ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
+            stat_h = a.stat + rp_row(a, sq, b, h, 0);
+            if (NB == 2 && c_first < n_ch) fetch(c_first, 0);
+        };
+        if (again) __syncthreads();                         // (nobody is left in the buffers)
+        head(0);
         bool seen[QT];
         bool any = false, all = true;
         typename Ti::frag fk[QT][Ti::KB], fv[QT][Ti::KB];
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int key = kw + ct * 16 + i16;
-            seen[ct] = key < sq.kn && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
-            any |= seen[ct];
-            all &= seen[ct];
+            const bool in = key < sq.kn;
             const int64_t kt = (int64_t)(sq.k0 + key);
+            seen[ct] = in && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
 #pragma unroll
             for (int kk = 0; kk < Ti::KB; ++kk) {
-                fk[ct][kk] = Ti::gfrag((const T*)a.k + b * a.sk.sb + kt * a.sk.st + hk * a.sk.sh, kk, g, a.D, seen[ct]);
-                fv[ct][kk] = Ti::gfrag((const T*)a.v + b * a.sv.sb + kt * a.sv.st + hk * a.sv.sh, kk, g, a.D, seen[ct]);
+                fk[ct][kk] = Ti::gfrag((const T*)a.k + b * a.sk.sb + kt * a.sk.st + hk * a.sk.sh, kk, g, a.D, in);
+                fv[ct][kk] = Ti::gfrag((const T*)a.v + b * a.sv.sb + kt * a.sv.st + hk * a.sv.sh, kk, g, a.D, in);
             }
         }
+#pragma unroll
+        for (int ct = 0; ct < QT; ++ct) {
+            any |= seen[ct];
+            all &= seen[ct];
+        }
         const bool wave_any = __any(any), wave_all = __all(all);
-        const bool wg_any = __syncthreads_or(any);
+        if (!wave_all)                                      // what stands in hidden rows reaches no product
+#pragma unroll
+            for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                for (int kk = 0; kk < Ti::KB; ++kk) {
+                    fk[ct][kk] = seen[ct] ? fk[ct][kk] : (typename Ti::frag){};
+                    fv[ct][kk] = seen[ct] ? fv[ct][kk] : (typename Ti::frag){};
+                }
+        if (!__syncthreads_or(any)) { n_ch = 0; asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // (the chunk under way lands before anybody leaves)
         f32x4 dk[QT][DT], dv[QT][DT];
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct)
 #pragma unroll
             for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
-        const int n_ch = wg_any ? (sq.qn + 63) / 64 : 0;
-        int c_first = 0;
-        if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
         for (int gi = 0; gi < G; ++gi) {
-            const int h = hk * G + gi;
-            const T* qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
-            const T* ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
-            const float* lse_h = a.lse + rp_row(a, sq, b, h, 0);
-            const float* delta_h = a.delta + rp_row(a, sq, b, h, 0);
-            float rl = 0.f, rd = 0.f;
-            auto fetch = [&](int c, int at) {
-                const uint64_t ok = rp_low_bits(sq.qn - c * 64);
-                rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + at * 2 * Ti::BYTES, w, l);
-                ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
-            };
-            auto fetch_rows = [&](int c) {                  // (through registers: rows that are not there need -inf)
-                if (tid < 64) {
-                    const bool in = c * 64 + tid < sq.qn;
-                    const float lse = in ? lse_h[c * 64 + tid] : INFINITY;
-                    rl = lse == -INFINITY ? -INFINITY : -lse * RP_LOG2E;
-                    rd = in ? -delta_h[c * 64 + tid] : 0.f;
-                }
-            };
-            auto put_rows = [&](int at) {
-                if (tid < 64) { rows[at * 128 + tid] = rl; rows[at * 128 + 64 + tid] = rd; }
-            };
-            int buf = 0;
-            __syncthreads();                                // (nobody is left in the buffers, the table, the bins)
-            if (c_first < n_ch) {
-                if (NB == 2) fetch(c_first, 0);
-                fetch_rows(c_first);
-            }
-            rp_fill_table(a, tab, h, -1, tid);
+            if (gi) { __syncthreads(); head(gi); }          // (nobody is left in the buffers, the table, the bins)
+            table.finish(a, tab, hk * G + gi);
             if (part)
                 for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
-            const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
+            int buf = 0;
             f32x4 far_sum = {0.f, 0.f, 0.f, 0.f};           // one side at a time: the chunks come in the order of -rel
             auto commit = [&](int at) {
                 const float t = wave_sum(far_sum[0] + far_sum[1] + far_sum[2] + far_sum[3]);
@@ -344,12 +362,11 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             float diag[4 + QT];                             // block diagonals 1 - QT .. 4 of the chunk
 #pragma unroll
             for (int k = 0; k < 4 + QT; ++k) diag[k] = 0.f;
-            if (c_first < n_ch) { put_rows(0); fetch_rows(c_first + 1); }
-            auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0) __attribute__((always_inline)) {
+            auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0, int there) __attribute__((always_inline)) {
                 const char* tO = tQ + Ti::BYTES;
                 const float* rowd = rowl + 64;
                 const float* bt = tab + (rel0 + mid + 4 * g - i16);
-                const float fc = near ? 0.f : rel0 > 0 ? farL : farR;
+                const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
 #pragma unroll
                 for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
                     f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS], dr[Ti::RPS], z[Ti::RPS + QT - 1];
@@ -377,14 +394,16 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                                 dp[ct][j] = Ti::mma(fo, fv[ct][kk], kk == 0 ? dr[j] : dp[ct][j]);
                             }
                         }
-                    if (edge) {                             // a hidden key's column, rel > 0 with `causal`: p = 0
+                    if (edge) {                             // a hidden key's column, rel > 0 with `causal`, a row behind the sequence: p = 0
 #pragma unroll
-                        for (int ct = 0; ct < QT; ++ct)
+                        for (int j = 0; j < Ti::RPS; ++j)
 #pragma unroll
-                            for (int j = 0; j < Ti::RPS; ++j)
+                            for (int r = 0; r < 4; ++r) {
+                                const int row = (kp * Ti::RPS + j) * 16 + 4 * g + r;
 #pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    s[ct][j][r] = seen[ct] && !(causal && rel0 + 16 * (kp * Ti::RPS + j - ct) + 4 * g + r - i16 < 0) ? s[ct][j][r] : -INFINITY;
+                                for (int ct = 0; ct < QT; ++ct)
+                                    s[ct][j][r] = seen[ct] && row < there && !(causal && rel0 + row - 16 * ct - i16 < 0) ? s[ct][j][r] : -INFINITY;
+                            }
                     }
                     typename Ti::frag fp[QT], fds[QT];
 #pragma unroll
@@ -438,18 +457,18 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                     }
                 }
             };
-            for (int c = c_first; c < n_ch; ++c, buf ^= 1) {
+            for (int c = c_first; c < n_ch; ++c, buf ^= NB - 1) {
                 if (NB == 1) { __syncthreads(); fetch(c, 0); }
                 rp_landed();
-                const char* tQ = smem + buf * (NB - 1) * 2 * Ti::BYTES;
+                const char* tQ = smem + buf * 2 * Ti::BYTES;
                 const float* rowl = rows + buf * 128;
-                if (c + 1 < n_ch) { put_rows(buf ^ 1); fetch_rows(c + 2); if (NB == 2) fetch(c + 1, buf ^ 1); }
+                if (NB == 2 && c + 1 < n_ch) fetch(c + 1, buf ^ 1);
                 const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
                 if (!wave_any || (causal && rel0 + 63 < 0)) continue;
                 const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
                 if (part && side < 0 && rel0 > 0) { commit(0); side = 0; }
                 if (part && !near) side = rel0 > 0 ? 1 : -1;
-                chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0), tQ, rowl, rel0);
+                chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0) || (c + 1) * 64 > sq.qn, tQ, rowl, rel0, sq.qn - c * 64);
                 if (part && near) {
                     float* bd = bw + (rel0 - 16 * (QT - 1) + mid);
                     rp_flush4(bd, diag[0], diag[1], diag[2], diag[3], l);
@@ -500,13 +519,21 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     }
 }
 
-// the partial sums of a head over its workgroups, in their order: 64 places of rel per workgroup, 16 interleaved groups of partials
+// dtable of a head from its workgroups' sums, in a fixed order.  rp_sum_kernel: 64 places of rel a workgroup, 16 interleaved groups of partials; rp_bucket_kernel:
+// one wave per (bucket, head) over the places.  Few partials (short sequences): the second alone, summing as it reads.
 __global__ __launch_bounds__(1024) void rp_sum_kernel(const float* part, float* sums, int64_t wgs, int nd) {
     __shared__ float red[16][64];
     const int x = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6, h = blockIdx.y;
     float s = 0.f;
-    if (x < nd)
-        for (int64_t i = y; i < wgs; i += 16) s += part[(h * wgs + i) * nd + x];
+    if (x < nd) {
+        const float* p = part + (h * wgs + y) * nd + x;
+        int64_t i = y;
+        for (; i + 48 < wgs; i += 64, p += (int64_t)64 * nd) {
+            const float v0 = p[0], v1 = p[(int64_t)16 * nd], v2 = p[(int64_t)32 * nd], v3 = p[(int64_t)48 * nd];
+            s += (v0 + v1) + (v2 + v3);
+        }
+        for (; i < wgs; i += 16, p += (int64_t)16 * nd) s += *p;
+    }
     red[y][threadIdx.x & 63] = s;
     __syncthreads();
     if (y == 0 && x < nd) {
@@ -515,12 +542,13 @@ __global__ __launch_bounds__(1024) void rp_sum_kernel(const float* part, float* 
         sums[(int64_t)h * nd + x] = s;
     }
 }
-// sums over the places of a bucket: one wave per (bucket, head)
-__global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16) {
+__global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, int wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable,
+                                                       int bf16) {
     const int bk = blockIdx.x, h = blockIdx.y, n = 2 * (span + pad) + 1;
     float s = 0.f;
     for (int x = threadIdx.x; x < n; x += 64)
-        if (rp_clamp(map[rp_clamp(x - span - pad, -span, span) + span], 0, buckets - 1) == bk) s += sums[(int64_t)h * n + x];
+        if (rp_clamp(map[rp_clamp(x - span - pad, -span, span) + span], 0, buckets - 1) == bk)
+            for (int i = 0; i < wgs; ++i) s += sums[((int64_t)h * wgs + i) * n + x];
     s = wave_sum(s);
     if (threadIdx.x == 0) {
         if (bf16) ((bf16_t*)dtable)[(int64_t)bk * heads + h] = f2bf(s);
@@ -530,10 +558,13 @@ __global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, const 
 int amdseg_relpos_sums_impl(const float* part, float* sums, int64_t wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16,
                             hipStream_t s) {
     const int nd = 2 * (span + pad) + 1;
-    hipLaunchKernelGGL(rp_sum_kernel, dim3((nd + 63) / 64, heads), dim3(1024), 0, s, part, sums, wgs, nd);
-    const int rc = amdseg_launch_status();
-    if (rc) return rc;
-    hipLaunchKernelGGL(rp_bucket_kernel, dim3(buckets, heads), dim3(64), 0, s, sums, map, span, pad, buckets, heads, dtable, bf16);
+    const bool few = wgs <= 8;
+    if (!few) {
+        hipLaunchKernelGGL(rp_sum_kernel, dim3((nd + 63) / 64, heads), dim3(1024), 0, s, part, sums, wgs, nd);
+        const int rc = amdseg_launch_status();
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(rp_bucket_kernel, dim3(buckets, heads), dim3(64), 0, s, few ? part : sums, few ? (int)wgs : 1, map, span, pad, buckets, heads, dtable, bf16);
     return amdseg_launch_status();
 }
 
@@ -541,11 +572,12 @@ template <typename T, int DT>
 static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStream_t s) {
     const int ND = 2 * (a.span + RP_PAD) + 1;
     const int tail = a.zero_tail ? RP_TAIL_WGS : 0;
+    a.mask_words = rp_mask_bytes(a) / 8;
     const int qt = rp_fwd_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
     const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
     if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
-    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + ND * 4;
+    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
     int rc;
     if (n == 0) {
     } else if (sizeof(T) == 4 || qt == 1) {
@@ -559,7 +591,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
     const int64_t m = (int64_t)a.B * a.kv_heads * a.nrb + tail;
     if (m > 0x7fffffff) return AMDSEG_ERR_SHAPE;
-    const int lds2 = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + 1024 + ND * 4 * (a.part_d ? 5 : 1);
+    const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
     } else if (sizeof(T) == 4 || kt == 1) {
         if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 1>, lds2))) return rc;

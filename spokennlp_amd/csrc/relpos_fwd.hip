@@ -11,7 +11,8 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* tab = reinterpret_cast<float*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks
+    uint64_t* words = reinterpret_cast<uint64_t*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks: the mask's words, the table
+    float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     int id = blockIdx.x;
     const int nmain = a.B * a.heads * a.nrb;
@@ -31,10 +32,16 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
+    RpTable table;
+    table.start(a, 1, tid);
     RpStage<T, DT> rk, rv;
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
-    for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
+    RpKeys keys;
+    keys.init(a, sq, b, l, words);
+    if (keys.m || sq.kn % 64 || a.D != DT * 16)             // (something of a chunk is not fetched)
+        for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
     rp_cleared();
+    if (keys.m) { keys.build(words, w); __syncthreads(); }
     const int hk = h / (a.heads / a.kv_heads);
     const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)sq.k0 * a.sk.st + hk * a.sk.sh;
     const T* vb = (const T*)a.v + b * a.sv.sb + (int64_t)sq.k0 * a.sv.st + hk * a.sv.sh;
@@ -52,19 +59,14 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
         }
         if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
-        RpKeys keys;
-        keys.init(a, sq, b, l, c);
-        uint64_t bits = 0;
-        int buf = 0;
-        auto fetch = [&](int at) {
-            rk.load(kb + (int64_t)c * 64 * a.sk.st, bits, smem + at * 2 * Ti::BYTES, w, l);
-            rv.load(vb + (int64_t)c * 64 * a.sv.st, bits, smem + at * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        auto fetch = [&](int at, int buf, uint64_t bits) {
+            rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
+            rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
         };
-        while (c < c_end && (bits = keys.next(c)) == 0) ++c;
-        if (NB == 2 && c < c_end) fetch(0);                 // on its way before anything else is waited for
-        if (first) rp_fill_table(a, tab, h, 1, tid);
-        first = false;
-        const float farL = rp_table(a, -span, h) * RP_LOG2E, farR = rp_table(a, span, h) * RP_LOG2E;
+        uint64_t bits;
+        c = keys.seek(c, c_end, bits);
+        int buf = 0;
+        if (NB == 2 && c < c_end) fetch(c, 0, bits);        // on its way before anything else is waited for
         typename Ti::frag fq[QT][Ti::KB];
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
@@ -72,6 +74,8 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
 #pragma unroll
             for (int kk = 0; kk < Ti::KB; ++kk) fq[ct][kk] = Ti::gfrag(qbase + (int64_t)q * a.sq.st, kk, g, a.D, q < sq.qn);
         }
+        if (first) table.finish(a, tab, h);
+        first = false;
         f32x4 o[QT][DT];
         float m_run[QT], l_part[QT];
 #pragma unroll
@@ -106,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                             s[ct][f][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][f][r] : -INFINITY;
                 }
             }
-            const float fc = near ? 0.f : rel0 > 0 ? farR : farL;
+            const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
 #pragma unroll
             for (int ct = 0; ct < QT; ++ct) {
                 float mx = s[ct][0][0];
@@ -152,14 +156,15 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                 }
             }
         };
-        for (; c < c_end; buf ^= NB - 1) {
-            if (NB == 1) { __syncthreads(); fetch(0); }
+        while (c < c_end) {
+            if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
             rp_landed();                                    // this chunk is there (and the table), nobody reads the buffer of the one before it any more
             const char* tK = smem + buf * 2 * Ti::BYTES;
             const int rel0 = c * 64 - (qw + sq.off);        // rel of the chunk's first key and the wave's first query
             const uint64_t now = bits;
-            do ++c; while (c < c_end && (bits = keys.next(c)) == 0);
-            if (NB == 2 && c < c_end) fetch(buf ^ 1);
+            c = keys.seek(c + 1, c_end, bits);
+            buf ^= NB - 1;
+            if (NB == 2 && c < c_end) fetch(c, buf, bits);
             if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
             const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
             chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
@@ -218,7 +223,7 @@ __global__ __launch_bounds__(256) void rp_join_kernel(RpArgs a) {
 
 template <typename T, int DT, int QT>
 static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
-    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + (2 * (a.span + RP_PAD) + 1) * 4;
+    const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + (2 * (a.span + RP_PAD) + 1) * 4;
     const int rc = rp_allow_lds((const void*)rp_fwd_kernel<T, DT, QT>, lds);
     if (rc) return rc;
     const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
@@ -238,6 +243,7 @@ int amdseg_relpos_fwd_impl(const RpArgs& a0, int dtype, hipStream_t s) {
     RpArgs a = a0;
     const int qt = rp_fwd_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
+    a.mask_words = rp_mask_bytes(a) / 8;
     if (dtype == 1) return rp_fwd_d<float, 1>(a, s);
     return qt == 1 ? rp_fwd_d<bf16_t, 1>(a, s) : rp_fwd_d<bf16_t, 2>(a, s);
 }

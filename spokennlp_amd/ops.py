@@ -547,28 +547,59 @@ def _rp_int(t, name, n, dev):
     return t.data_ptr()
 
 
-def _rp_table(c, table, bucket_map, heads, dev):
-    if table.device != dev or bucket_map.device != dev:
-        raise ValueError(f"table and bucket_map must be on {dev}")
+def _rp_table(c, table, bucket_map, heads):
     if table.dim() != 2 or table.shape[1] != heads or table.shape[0] < 1 or not table.is_contiguous():
         raise ValueError(f"table must be a contiguous [buckets, {heads}] tensor, not {tuple(table.shape)}")
     n = bucket_map.numel()
     if n % 2 == 0 or n > 2049:
         raise ValueError(f"bucket_map must hold 2 * span + 1 entries with span <= 1024, not {n}")
-    c.map, c.span = _rp_int(bucket_map, "bucket_map", n, dev), n // 2
-    c.table, c.table_dtype, c.buckets = table.data_ptr(), _dt(table), table.shape[0]
+    c.span, c.table_dtype, c.buckets = n // 2, _dt(table), table.shape[0]
 
 
 def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end):
+    """-> (RelposCfg, shape of lse, workspace bytes forward, backward).  What follows from shapes, strides, types and options alone is worked out once per
+    such combination and copied (a call on a few rows is otherwise longer on the host than on the GPU); pointers and devices are looked at every time."""
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, table.shape, table.dtype, bucket_map.shape, scale, max_q, max_k,
+           bool(causal), bool(align_end), cu_q is None or cu_q.shape, cu_k is None or cu_k.shape, k_lens is None,
+           None if key_mask is None else (key_mask.shape, key_mask.stride(), key_mask.dtype))
+    known = _rp_known.get(key)
+    if known is None:
+        known = _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+        if len(_rp_known) >= 256:
+            _rp_known.clear()
+        _rp_known[key] = known
+    c = L.RelposCfg.from_buffer_copy(known[0])
+    dev = q.device
+    if dev.type != "cuda" or k.device != dev or v.device != dev:
+        raise ValueError("q, k, v must be on one GPU")
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.data_ptr() & 15:
+            raise ValueError(f"{n}: rows must start on 16 bytes")
+    if table.device != dev or bucket_map.device != dev or not table.is_contiguous():
+        raise ValueError(f"table (contiguous) and bucket_map must be on {dev}")
+    c.table, c.map = table.data_ptr(), _rp_int(bucket_map, "bucket_map", bucket_map.numel(), dev)
+    if cu_q is not None:
+        c.cu_q, c.cu_k = _rp_int(cu_q, "cu_q", c.B + 1, dev), _rp_int(cu_k, "cu_k", c.B + 1, dev)
+    if k_lens is not None:
+        c.k_lens = _rp_int(k_lens, "k_lens", c.B, dev)
+    if key_mask is not None:
+        if key_mask.device != dev:
+            raise ValueError(f"key_mask must be on {dev}")
+        c.key_mask = key_mask.data_ptr()
+    return c, known[1], known[2], known[3]
+
+
+_rp_known = {}
+
+
+def _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end):
+    """the checks and the part of RelposCfg that depend on no pointer"""
     packed = cu_q is not None
     if packed != (cu_k is not None):
         raise ValueError("cu_q and cu_k come together")
     nd = 3 if packed else 4
     if q.dim() != nd or k.dim() != nd or v.shape != k.shape:
         raise ValueError(f"q, k, v must be {'[tokens, heads, D]' if packed else '[B, L, heads, D]'}, not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    dev = q.device
-    if dev.type != "cuda" or k.device != dev or v.device != dev:
-        raise ValueError("q, k, v must be on one GPU")
     c = L.RelposCfg()
     c.dtype = _dt(q)
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -590,7 +621,6 @@ def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max
         c.B, c.Tq, c.Tk = cu_q.numel() - 1, q.shape[0], k.shape[0]
         if c.B < 0:
             raise ValueError("cu_q needs at least one element")
-        c.cu_q, c.cu_k = _rp_int(cu_q, "cu_q", c.B + 1, dev), _rp_int(cu_k, "cu_k", c.B + 1, dev)
         for n in (max_q, max_k):
             if n is not None and n < 0:
                 raise ValueError("max_q / max_k must not be negative")
@@ -600,21 +630,26 @@ def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max
         if k.shape[0] != q.shape[0]:
             raise ValueError(f"q holds {q.shape[0]} sequences, k {k.shape[0]}")
         c.B, c.Lq, c.Lk = q.shape[0], q.shape[1], k.shape[1]
-        if k_lens is not None:
-            c.k_lens = _rp_int(k_lens, "k_lens", c.B, dev)
     if key_mask is not None:
         want = (c.Tk,) if packed else (c.B, c.Lk)
-        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != want or key_mask.device != dev:
-            raise ValueError(f"key_mask must be a bool or uint8 tensor {want} on {dev}, not {key_mask.dtype} {tuple(key_mask.shape)}")
+        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != want:
+            raise ValueError(f"key_mask must be a bool or uint8 tensor {want}, not {key_mask.dtype} {tuple(key_mask.shape)}")
         if key_mask.numel() and key_mask.shape[-1] > 1 and key_mask.stride(-1) != 1:
             raise ValueError("key_mask: the last dimension must be contiguous")
-        c.key_mask, c.mask_stride = key_mask.data_ptr(), 0 if packed or key_mask.shape[0] == 1 else key_mask.stride(0)
-    _rp_table(c, table, bucket_map, heads, dev)
+        c.mask_stride = 0 if packed or key_mask.shape[0] == 1 else key_mask.stride(0)
+    _rp_table(c, table, bucket_map, heads)
     c.scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-6 < c.scale < 1e6:
         raise ValueError(f"scale = {scale}: a positive number")
     c.causal, c.align_end = int(bool(causal)), int(bool(align_end))
-    return c
+    # the library sizes its workspaces from shapes; the two pointers it asks for (and whether there is a mask or offsets at all) stand in
+    probe = L.RelposCfg.from_buffer_copy(c)
+    probe.map = probe.table = 256
+    if packed:
+        probe.cu_q = probe.cu_k = 256
+    lib = L.load()
+    return (bytes(c), (heads, c.Tq) if packed else (c.B, heads, c.Lq), lib.amdseg_relpos_attn_ws_bytes(C.byref(probe), 0),
+            lib.amdseg_relpos_attn_ws_bytes(C.byref(probe), 1))
 
 
 def _rp_out(t, like, name, es):
@@ -629,8 +664,28 @@ def _rp_out(t, like, name, es):
     return _rp_strides(t, name, es)
 
 
-def _rp_ws(n, dev):
-    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=dev)
+def _rp_dense(shape):
+    """element strides (sequence, row, head) of a contiguous tensor"""
+    st = [shape[-1] * shape[-2], shape[-1]]
+    return (st[0] * shape[1] if len(shape) == 4 else 0, *st)
+
+
+class _rp_on:
+    """the GPU of a call's tensors as the current one (nothing to do where it is), and its current stream's handle"""
+
+    def __init__(self, dev):
+        self.dev = dev
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.dev).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
 
 
 def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None, causal=False,
@@ -643,18 +698,17 @@ def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_len
     Query i stands at position i, or (align_end) so that the last query stands at the last key.  A row that sees no key: zero, lse -inf.
     Returns (out, lse); lse fp32 [B, heads, Lq] / [heads, tokens], None unless need_lse.  `out`: rows outside every packed sequence are left as they were
     (a fresh tensor has zeros there)."""
-    c = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
-    dev = q.device
-    with torch.cuda.device(dev):
+    c, lse_shape, ws_bytes, _ = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+    with _rp_on(q.device) as stream:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out = q.new_empty(q.shape)
             c.zero_tail = 1
-        c.out_stride[:] = _rp_out(out, q, "out", q.element_size())
-        lse = torch.empty((c.heads, c.Tq) if cu_q is not None else (c.B, c.heads, c.Lq), dtype=torch.float32, device=dev) if need_lse else None
-        lib = L.load()
-        n = lib.amdseg_relpos_attn_ws_bytes(C.byref(c), 0)
-        ws = _rp_ws(n, dev) if n else None
-        L.check(lib.amdseg_relpos_attn_fwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(ws), n, _s()), "amdseg_relpos_attn_fwd")
+            c.out_stride[:] = _rp_dense(q.shape)
+        else:
+            c.out_stride[:] = _rp_out(out, q, "out", q.element_size())
+        lse = table.new_empty(lse_shape, dtype=torch.float32) if need_lse else None
+        ws = table.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+        L.check(L.load().amdseg_relpos_attn_fwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(ws), ws_bytes, stream), "amdseg_relpos_attn_fwd")
     return out, lse
 
 
@@ -663,30 +717,30 @@ def relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale=None, key_
     """gradients of relpos_attn_fwd from its `out` and `lse` (amdseg_relpos_attn_bwd): (dq, dk, dv, dtable), the last in the table's dtype or None.
     dq / dk / dv may be given (column blocks of one buffer): rows outside every packed sequence are left as they were in all three or, if none is given,
     zero.  Sums are taken in a fixed order: the same call gives the same bits."""
-    c = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+    c, lse_shape, _, ws_bytes = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
     dev, es = q.device, q.element_size()
     if (dq is None) != (dk is None) or (dq is None) != (dv is None):
         raise ValueError("dq, dk, dv: give all three or none")
     if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype or out.device != dev or dout.device != dev:
         raise ValueError(f"out and dout must be {tuple(q.shape)} {q.dtype} on {dev}")
-    want = (c.heads, c.Tq) if cu_q is not None else (c.B, c.heads, c.Lq)
-    if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
-        raise ValueError(f"lse must be the contiguous fp32 {want} of relpos_attn_fwd")
-    with torch.cuda.device(dev):
-        if dq is None:
-            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
-            c.zero_tail = 1
+    if lse.shape != lse_shape or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError(f"lse must be the contiguous fp32 {lse_shape} of relpos_attn_fwd")
+    with _rp_on(dev) as stream:
         c.out_stride[:] = _rp_strides(out, "out", es)
         c.dout_stride[:] = _rp_strides(dout, "dout", es)
-        c.dq_stride[:] = _rp_out(dq, q, "dq", es)
-        c.dk_stride[:] = _rp_out(dk, k, "dk", es)
-        c.dv_stride[:] = _rp_out(dv, v, "dv", es)
+        if dq is None:
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+            c.zero_tail = 1
+            c.dq_stride[:] = _rp_dense(q.shape)
+            c.dk_stride[:] = c.dv_stride[:] = _rp_dense(k.shape)
+        else:
+            c.dq_stride[:] = _rp_out(dq, q, "dq", es)
+            c.dk_stride[:] = _rp_out(dk, k, "dk", es)
+            c.dv_stride[:] = _rp_out(dv, v, "dv", es)
         dtable = torch.empty_like(table) if need_dtable else None
-        lib = L.load()
-        n = lib.amdseg_relpos_attn_ws_bytes(C.byref(c), 1)
-        ws = _rp_ws(n, dev)
-        L.check(lib.amdseg_relpos_attn_bwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable), _p(ws),
-                                           ws.numel(), _s()), "amdseg_relpos_attn_bwd")
+        ws = table.new_empty(ws_bytes, dtype=torch.uint8)
+        L.check(L.load().amdseg_relpos_attn_bwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable), _p(ws),
+                                                ws_bytes, stream), "amdseg_relpos_attn_bwd")
     return dq, dk, dv, dtable
 
 
@@ -698,10 +752,11 @@ def relpos_bias_fwd(table, bucket_map, Lq, Lk, q_offset=0, out_dtype=torch.float
     c, dev, heads = L.RelposCfg(), table.device, table.shape[1]
     if dev.type != "cuda":
         raise ValueError("table must be on a GPU")
-    _rp_table(c, table, bucket_map, heads, dev)
-    with torch.cuda.device(dev):
-        out = torch.empty((heads, Lq, Lk), dtype=out_dtype, device=dev)
-        L.check(L.load().amdseg_relpos_bias_fwd(c.table, c.table_dtype, c.map, c.span, c.buckets, heads, Lq, Lk, q_offset, _p(out), _dt(out), _s()),
+    _rp_table(c, table, bucket_map, heads)
+    m = _rp_int(bucket_map, "bucket_map", bucket_map.numel(), dev)
+    with _rp_on(dev) as stream:
+        out = table.new_empty((heads, Lq, Lk), dtype=out_dtype)
+        L.check(L.load().amdseg_relpos_bias_fwd(_p(table), c.table_dtype, m, c.span, c.buckets, heads, Lq, Lk, q_offset, _p(out), _dt(out), stream),
                 "amdseg_relpos_bias_fwd")
     return out
 
@@ -721,10 +776,11 @@ def relpos_bias_bwd(dbias, bucket_map, buckets, q_offset=0):
     if dbias.data_ptr() & 15:
         raise ValueError("dbias must start on 16 bytes")
     m = _rp_int(bucket_map, "bucket_map", n, dev)
-    with torch.cuda.device(dev):
-        dtable = torch.empty((buckets, heads), dtype=torch.float32, device=dev)
+    with _rp_on(dev) as stream:
+        dtable = dbias.new_empty((buckets, heads), dtype=torch.float32)
         lib = L.load()
-        ws = _rp_ws(lib.amdseg_relpos_bias_ws_bytes(B, heads, Lq, n // 2), dev)
-        L.check(lib.amdseg_relpos_bias_bwd(_p(dbias), _dt(dbias), m, n // 2, buckets, B, heads, Lq, Lk, q_offset, _p(dtable), _p(ws), ws.numel(), _s()),
+        ws_bytes = lib.amdseg_relpos_bias_ws_bytes(B, heads, Lq, n // 2)
+        ws = dbias.new_empty(ws_bytes, dtype=torch.uint8)
+        L.check(lib.amdseg_relpos_bias_bwd(_p(dbias), _dt(dbias), m, n // 2, buckets, B, heads, Lq, Lk, q_offset, _p(dtable), _p(ws), ws_bytes, stream),
                 "amdseg_relpos_bias_bwd")
     return dtable
