@@ -13,8 +13,9 @@
 //
 // dtable.  In the accumulator layout lane (g, i16) holds ds of query 4 g + r (register r) and key i16, so -rel = const + 4 g + r - i16.  Moving register r
 // by r lanes inside its 16 (a DPP operand modifier of the add itself) puts equal rel into equal lanes: the 16 x 16 tiles of one block diagonal add
-// up in one register per lane, the lanes that fall off the end belong to the next block diagonal's register.  7 adds per 4 elements, no LDS; the registers go
-// to the wave's own LDS bins once per 64-row chunk.  Chunks beyond the span add into one register per side instead (one add per element).
+// up in one register per lane, the lanes that fall off the end belong to the next block diagonal's register.  7 adds per 4 elements, no LDS; the registers
+// live on from chunk to chunk until no later tile reaches their rel, and each sum is STORED once into the wave's own LDS bins (with ds_add_f32 instead,
+// four a chunk, the kernel took 141 us instead of 105 at 32 x 512: LDS float atomics).  Chunks beyond the span add into one register per side instead (one add per element).
 #include "relpos.h"
 #include "relpos_launch.h"
 
@@ -33,8 +34,9 @@ __device__ __forceinline__ void rp_diag_add(f32x4 x, float& lo, float& hi) {
 }
 
 
-// acc[0..3] are complete block diagonals: their four 16-lane rows (g) hold overlapping rel, so the 4 x 4 rows are exchanged -- afterwards register g holds
-// the g rows of all four diagonals, 64 different bins -- and four adds carry them into the wave's bins (a wave's LDS operations complete in order)
+// Four complete block diagonals x0 .. x3 -> one register of 64 sums, lane (row, i) = rel 16 row - i.  A lane's g-row is 4 g further: each register is turned by
+// 4 g lanes inside its rows of 16 (one LDS permute), what goes past the end is the next diagonal's (`past` carries x3's to the next chunk), then the four rows
+// add up in three exchanges.
 __device__ __forceinline__ void rp_swap32(float& x, float& y) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     x = __uint_as_float(r[0]); y = __uint_as_float(r[1]);
@@ -43,11 +45,17 @@ __device__ __forceinline__ void rp_swap16(float& x, float& y) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     x = __uint_as_float(r[0]); y = __uint_as_float(r[1]);
 }
-__device__ __forceinline__ void rp_flush4(float* bin, float x0, float x1, float x2, float x3, int l) {
-    rp_swap32(x0, x2); rp_swap32(x1, x3);
-    rp_swap16(x0, x1); rp_swap16(x2, x3);
-    bin += 16 * (l >> 4) - (l & 15);
-    atomicAdd(bin, x0); atomicAdd(bin + 4, x1); atomicAdd(bin + 8, x2); atomicAdd(bin + 12, x3);
+__device__ __forceinline__ float rp_join4(float x0, float x1, float x2, float x3, float& past, int l) {
+    const int g = l >> 4, i = l & 15, from = ((l & 48) | ((i + 4 * g) & 15)) * 4;
+    const bool wrap = i + 4 * g >= 16;
+    auto turn = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from, __builtin_bit_cast(int, x))); };
+    const float y0 = turn(x0), y1 = turn(x1), y2 = turn(x2), y3 = turn(x3);
+    float z0 = wrap ? past : y0, z1 = wrap ? y0 : y1, z2 = wrap ? y1 : y2, z3 = wrap ? y2 : y3;
+    past = y3;
+    rp_swap32(z0, z2); rp_swap32(z1, z3);
+    float a = z0 + z2, b = z1 + z3;
+    rp_swap16(a, b);
+    return a + b;
 }
 
 template <typename T, int DT, int QT>
@@ -359,7 +367,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                 far_sum = (f32x4){0.f, 0.f, 0.f, 0.f};
             };
             int side = 0;                                   // -1: rel >= span summed so far, 1: rel <= -span
-            float diag[4 + QT];                             // block diagonals 1 - QT .. 4 of the chunk
+            float diag[4 + QT], past = 0.f;                 // block diagonals 1 - QT .. 4 of the chunk
 #pragma unroll
             for (int k = 0; k < 4 + QT; ++k) diag[k] = 0.f;
             auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0, int there) __attribute__((always_inline)) {
@@ -470,20 +478,17 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                 if (part && !near) side = rel0 > 0 ? 1 : -1;
                 chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0) || (c + 1) * 64 > sq.qn, tQ, rowl, rel0, sq.qn - c * 64);
                 if (part && near) {
-                    float* bd = bw + (rel0 - 16 * (QT - 1) + mid);
-                    rp_flush4(bd, diag[0], diag[1], diag[2], diag[3], l);
-                    // the upper ones go on into the next chunk, 64 rel further; after the last near chunk they are flushed too (rows of 16 lanes one at a
-                    // time: they overlap)
+                    float* bd = bw + (rel0 - 16 * (QT - 1) + mid + 16 * g - i16);
+                    *bd = rp_join4(diag[0], diag[1], diag[2], diag[3], past, l);
+                    // the upper ones go on into the next chunk, 64 rel further; after the last near chunk they are stored too (nothing beyond rel0 + 63)
 #pragma unroll
                     for (int k = 0; k < QT; ++k) diag[k] = diag[4 + k];
 #pragma unroll
                     for (int k = QT; k < 4 + QT; ++k) diag[k] = 0.f;
                     if (c + 1 >= n_ch || rel0 + 64 - (16 * QT - 1) >= span) {
-#pragma unroll
-                        for (int gg = 0; gg < 4; ++gg)
-                            if (g == gg)
-#pragma unroll
-                                for (int k = 0; k < QT; ++k) atomicAdd(bd + 64 + 16 * k + 4 * g - i16, diag[k]);
+                        const float rest = rp_join4(diag[0], QT > 1 ? diag[1] : 0.f, 0.f, 0.f, past, l);
+                        if (64 - 16 * (QT - 1) + 16 * g - i16 <= 63) bd[64] = rest;
+                        past = 0.f;
 #pragma unroll
                         for (int k = 0; k < QT; ++k) diag[k] = 0.f;
                     }
@@ -519,8 +524,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     }
 }
 
-// dtable of a head from its workgroups' sums, in a fixed order.  rp_sum_kernel: 64 places of rel a workgroup, 16 interleaved groups of partials; rp_bucket_kernel:
-// one wave per (bucket, head) over the places.  Few partials (short sequences): the second alone, summing as it reads.
+// dtable from the workgroups' sums, in a fixed order: one workgroup per (bucket, head) lists the places of rel that belong to its bucket, then adds those of
+// every partial.  Many partials (long batches): rp_sum_kernel first brings them down to one per head -- 64 places a workgroup, 16 interleaved groups.
 __global__ __launch_bounds__(1024) void rp_sum_kernel(const float* part, float* sums, int64_t wgs, int nd) {
     __shared__ float red[16][64];
     const int x = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6, h = blockIdx.y;
@@ -542,15 +547,43 @@ __global__ __launch_bounds__(1024) void rp_sum_kernel(const float* part, float* 
         sums[(int64_t)h * nd + x] = s;
     }
 }
-__global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, int wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable,
-                                                       int bf16) {
-    const int bk = blockIdx.x, h = blockIdx.y, n = 2 * (span + pad) + 1;
+__global__ __launch_bounds__(256) void rp_bucket_kernel(const float* part, int wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable,
+                                                        int bf16) {
+    __shared__ int list[2 * (RP_MAX_SPAN + RP_PAD) + 1];
+    __shared__ int count[4];
+    __shared__ float red[4];
+    const int bk = blockIdx.x, h = blockIdx.y, nd = 2 * (span + pad) + 1, tid = threadIdx.x, w = tid >> 6, l = tid & 63;
+    int len = 0;
+    for (int x0 = 0; x0 < nd; x0 += 256) {
+        const int x = x0 + tid;
+        const bool mine = x < nd && rp_clamp(map[rp_clamp(x - span - pad, -span, span) + span], 0, buckets - 1) == bk;
+        const uint64_t vote = __ballot(mine);
+        if (l == 0) count[w] = __popcll(vote);
+        __syncthreads();
+        int at = len + __popcll(vote & ((1ull << l) - 1));
+        for (int i = 0; i < w; ++i) at += count[i];
+        if (mine) list[at] = x;
+        len += count[0] + count[1] + count[2] + count[3];
+        __syncthreads();
+    }
     float s = 0.f;
-    for (int x = threadIdx.x; x < n; x += 64)
-        if (rp_clamp(map[rp_clamp(x - span - pad, -span, span) + span], 0, buckets - 1) == bk)
-            for (int i = 0; i < wgs; ++i) s += sums[((int64_t)h * wgs + i) * n + x];
+    const float* p = part + (int64_t)h * wgs * nd;
+    if (len > 0) {
+        const int n = wgs * len;                            // (wgs <= 64)
+        int i = tid / len, k = tid % len;
+        const int di = 256 / len, dk = 256 % len;
+#pragma unroll 4
+        for (int x = tid; x < n; x += 256) {
+            s += p[(int64_t)i * nd + list[k]];
+            i += di; k += dk;
+            if (k >= len) { k -= len; ++i; }
+        }
+    }
     s = wave_sum(s);
-    if (threadIdx.x == 0) {
+    if (l == 0) red[w] = s;
+    __syncthreads();
+    if (tid == 0) {
+        s = (red[0] + red[1]) + (red[2] + red[3]);
         if (bf16) ((bf16_t*)dtable)[(int64_t)bk * heads + h] = f2bf(s);
         else ((float*)dtable)[(int64_t)bk * heads + h] = s;
     }
@@ -558,13 +591,13 @@ __global__ __launch_bounds__(64) void rp_bucket_kernel(const float* sums, int wg
 int amdseg_relpos_sums_impl(const float* part, float* sums, int64_t wgs, const int* map, int span, int pad, int buckets, int heads, void* dtable, int bf16,
                             hipStream_t s) {
     const int nd = 2 * (span + pad) + 1;
-    const bool few = wgs <= 8;
+    const bool few = wgs <= 64;
     if (!few) {
         hipLaunchKernelGGL(rp_sum_kernel, dim3((nd + 63) / 64, heads), dim3(1024), 0, s, part, sums, wgs, nd);
         const int rc = amdseg_launch_status();
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(rp_bucket_kernel, dim3(buckets, heads), dim3(64), 0, s, few ? part : sums, few ? (int)wgs : 1, map, span, pad, buckets, heads, dtable, bf16);
+    hipLaunchKernelGGL(rp_bucket_kernel, dim3(buckets, heads), dim3(256), 0, s, few ? part : sums, few ? (int)wgs : 1, map, span, pad, buckets, heads, dtable, bf16);
     return amdseg_launch_status();
 }
 
