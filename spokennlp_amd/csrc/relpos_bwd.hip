@@ -606,7 +606,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int ND = 2 * (a.span + RP_PAD) + 1;
     const int tail = a.zero_tail ? RP_TAIL_WGS : 0;
     a.mask_words = rp_mask_bytes(a) / 8;
-    const int qt = rp_fwd_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
+    const int qt = rp_dq_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
     const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
     if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
@@ -626,10 +626,10 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     if (m > 0x7fffffff) return AMDSEG_ERR_SHAPE;
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
-    } else if (sizeof(T) == 4 || kt == 1) {
+    } else if (sizeof(T) == 4 || DT > 4 || kt == 1) {
         if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 1>, lds2))) return rc;
         hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 1>), dim3((unsigned)m), dim3(256), lds2, s, a);
-    } else if constexpr (sizeof(T) == 2) {
+    } else if constexpr (sizeof(T) == 2 && DT <= 4) {
         if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 2>, lds2))) return rc;
         hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 2>), dim3((unsigned)m), dim3(256), lds2, s, a);
     }

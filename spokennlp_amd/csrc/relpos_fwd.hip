@@ -197,28 +197,224 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     }
 }
 
-// the splits of a row joined in their order: one wave per row
+// The few-rows form: single tokens (or a handful) against a cache.  HBM-bound, so K and V are read once: the G query heads of a kv head and their Lq rows, at most
+// 16 together, are the 16 columns of one tile.  A workgroup has one split of one (sequence, kv head); its four waves take the split's 64-key chunks in turn and
+// need nothing from each other until the end: K goes straight into registers (its row fragments are 16 contiguous bytes), V through the wave's own LDS piece
+// for the transposed read.  No bias table in LDS (every column has another head): only the chunks within the span of the rows look values up.
+template <typename T, int DT>
+__global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kernel(RpArgs a) {
+    typedef RpTile<T, DT> Ti;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ float ml[4][16][2];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
+    const int split = blockIdx.x, b = blockIdx.y / a.kv_heads, hk = blockIdx.y % a.kv_heads;
+    const int G = a.heads / a.kv_heads;
+    const RpSeq sq = rp_seq(a, b);
+    char* tV = smem + w * Ti::BYTES;
+    const bool col_ok = i16 < G * a.Lq;
+    const int qi = col_ok ? i16 / G : 0, h = hk * G + (col_ok ? i16 % G : 0), pos = qi + sq.off;
+    RpKeys keys;
+    keys.init(a, sq, b, l, nullptr);
+    keys.nw = 0;                                            // (the mask as it comes: a wave sees two or three chunks of it)
+    const bool causal = a.causal;
+    int c_end = (sq.kn + 63) / 64;
+    if (causal) c_end = sq.kn <= 0 || a.Lq - 1 + sq.off < 0 ? 0 : min(c_end, (a.Lq - 1 + sq.off) / 64 + 1);
+    const int c0 = split * (RP_SPLIT_KEYS / 64);
+    c_end = a.nsplit > 1 ? min(c_end, c0 + RP_SPLIT_KEYS / 64) : c_end;
+    typename Ti::frag fq[Ti::KB];
+    {
+        const T* qrow = (const T*)a.q + b * a.sq.sb + (int64_t)qi * a.sq.st + h * a.sq.sh;
+#pragma unroll
+        for (int kk = 0; kk < Ti::KB; ++kk) fq[kk] = Ti::gfrag(qrow, kk, g, a.D, col_ok);
+    }
+    const float c2 = a.scale * RP_LOG2E, farL = rp_table(a, a.map[0], h) * RP_LOG2E, farR = rp_table(a, a.map[2 * a.span], h) * RP_LOG2E;
+    if (keys.m || sq.kn % 64 || a.D != DT * 16) {
+#pragma unroll
+        for (int n = 0; n < Ti::BYTES / 1024; ++n) *reinterpret_cast<uint4*>(tV + n * 1024 + l * 16) = make_uint4(0u, 0u, 0u, 0u);
+        rp_cleared();
+    }
+    f32x4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_part = 0.f;
+    for (int c = c0 + w; c < c_end; c += 4) {
+        const uint64_t now = keys.bits(c);
+        if (now == 0) continue;
+        const T* kb = (const T*)a.k + b * a.sk.sb + (int64_t)c * 64 * a.sk.st + hk * a.sk.sh;
+        const uint64_t va = (uint64_t)((const T*)a.v + b * a.sv.sb + (int64_t)c * 64 * a.sv.st + hk * a.sv.sh);
+        typename Ti::frag fk[4][Ti::KB];
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int kk = 0; kk < Ti::KB; ++kk) fk[f][kk] = Ti::gfrag(kb + (int64_t)(f * 16 + i16) * a.sk.st, kk, g, a.D, (now >> (f * 16 + i16)) & 1);
+        const void* vbase = (const void*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(va >> 32)) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)va));
+        const uint32_t lds = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(char, tV));
+#pragma unroll
+        for (int n = 0; n < Ti::BYTES / 1024; ++n) {
+            int row, u;
+            Ti::piece(n, l, row, u);
+            if (((now >> row) & 1) && u < Ti::UNITS && u * Ti::EPU < a.D)
+                rp_glds16(vbase, (uint32_t)row * (uint32_t)(a.sv.st * (int64_t)sizeof(T)) + u * 16, lds + n * 1024);
+        }
+        const int rel0 = c * 64 + 4 * g - pos;
+        const bool near = c * 64 + 63 - sq.off > -a.span && c * 64 - (sq.off + a.Lq - 1) < a.span;
+        f32x4 s[4];
+        if (near) {
+            const float inv = 1.0f / a.scale;
+            int bk[4][4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bk[f][r] = a.map[rp_clamp(rel0 + 16 * f + r, -a.span, a.span) + a.span];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[f][r] = rp_table(a, bk[f][r], h) * inv;
+        } else
+#pragma unroll
+            for (int f = 0; f < 4; ++f) s[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < Ti::KB; ++kk)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) s[f] = Ti::mma(fk[f][kk], fq[kk], s[f]);
+        const float fc = near ? 0.f : c * 64 > sq.off ? farR : farL;
+        if (now != ~0ull || causal)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[f][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * f + r > 0) ? s[f][r] : -INFINITY;
+            }
+        float mx = s[0][0];
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[f][r]);
+        mx = fmaf(mx, c2, fc);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_run, mx);
+        const float al = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new), mu = fc - (m_new == -INFINITY ? 0.f : m_new);
+        m_run = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[f][r], c2, mu));
+                s[f][r] = e;
+                sum += e;
+            }
+        l_part = l_part * al + sum;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[d][r] *= al;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+            const typename Ti::frag fp = Ti::pf(&s[kp * Ti::RPS]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = Ti::mma(Ti::colf(tV, kp, d, l), fp, o[d]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the piece has been read before the next chunk lands in it)
+    }
+    // the four waves' sums meet in LDS, each in its own piece: [16 columns][D]
+    l_part += __shfl_xor(l_part, 16, 64);
+    l_part += __shfl_xor(l_part, 32, 64);
+    float* mine = reinterpret_cast<float*>(tV);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+        if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(mine + i16 * (DT * 16) + d * 16 + g * 4) = o[d];
+    if (g == 0) { ml[w][i16][0] = m_run; ml[w][i16][1] = l_part; }
+    __syncthreads();
+    const int col = tid >> 4, d0 = (tid & 15) * 8;
+    if (col >= G * a.Lq) return;
+    float m = ml[0][col][0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = fmaxf(m, ml[i][col][0]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float ls = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i][col][0] - mu);
+        ls += f * ml[i][col][1];
+        if (d0 < a.D) {
+            const float* p = reinterpret_cast<const float*>(smem + i * Ti::BYTES) + col * (DT * 16) + d0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += f * p[e];
+        }
+    }
+    const int q = col / G, hh = hk * G + col % G;
+    const int64_t row = rp_row(a, sq, b, hh, q);
+    if (a.nsplit > 1) {
+        const int64_t at = split * ((int64_t)a.B * a.heads * a.Lq) + row;
+        if (d0 < a.D) {
+            *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d0) = (f32x4){x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(a.part_o + at * a.D + d0 + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+        }
+        if (d0 == 0) { a.part_ml[at * 2] = m; a.part_ml[at * 2 + 1] = ls; }
+        return;
+    }
+    const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
+    if (d0 < a.D) {
+        T* op = (T*)a.out + b * a.so.sb + (int64_t)q * a.so.st + hh * a.so.sh + d0;
+        Ti::st4(op, (f32x4){x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
+        Ti::st4(op + 4, (f32x4){x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv});
+    }
+    if (a.lse && d0 == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(ls)) * RP_LN2;
+}
+
+// the splits of a row joined in their order: one wave per row, lane s first has split s's maximum and sum
 template <typename T>
 __global__ __launch_bounds__(256) void rp_join_kernel(RpArgs a) {
     const int l = threadIdx.x & 63;
-    const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
+    const int64_t rows = (int64_t)a.B * a.heads * a.Lq;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
     float m = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+    for (int s = l; s < a.nsplit; s += 64) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+    m = wave_max(m);
     const float mu = m == -INFINITY ? 0.f : m;
     float ls = 0.f, x0 = 0.f, x1 = 0.f;
     const int d = l * 2;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - mu);
-        ls += f * a.part_ml[(s * rows + row) * 2 + 1];
-        if (d < a.D) { const float* p = a.part_o + (s * rows + row) * a.D + d; x0 += f * p[0]; x1 += f * p[1]; }
+    const float* p = a.part_o + row * a.D + (d < a.D ? d : 0);
+    for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+        const int s = s0 + l;
+        const float f = s < a.nsplit ? __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - mu) : 0.f;
+        ls += s < a.nsplit ? f * a.part_ml[(s * rows + row) * 2 + 1] : 0.f;
+        const int n = min(64, a.nsplit - s0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float fi = __shfl(f, i, 64);
+            const float2 v = *reinterpret_cast<const float2*>(p + (s0 + i) * rows * a.D);
+            x0 += fi * v.x; x1 += fi * v.y;
+        }
     }
+    ls = wave_sum(ls);
     const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
     const int i = (int)(row % a.Lq), h = (int)(row / a.Lq % a.heads), b = (int)(row / a.Lq / a.heads);
     T* op = (T*)a.out + b * a.so.sb + (int64_t)i * a.so.st + h * a.so.sh;
     if (d < a.D) { Act<T>::st(op + d, x0 * inv); Act<T>::st(op + d + 1, x1 * inv); }
     if (a.lse && l == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(ls)) * RP_LN2;
+}
+
+template <typename T, int DT>
+static int rp_few_launch(const RpArgs& a, hipStream_t s) {
+    const int lds = 4 * RpTile<T, DT>::BYTES;
+    const int rc = rp_allow_lds((const void*)rp_few_kernel<T, DT>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((rp_few_kernel<T, DT>), dim3(a.nsplit, a.B * a.kv_heads), dim3(256), lds, s, a);
+    return amdseg_launch_status();
+}
+template <typename T>
+static int rp_join_launch(const RpArgs& a, hipStream_t s) {
+    if (a.nsplit > 1) {
+        const int64_t rows = (int64_t)a.B * a.heads * a.Lq;
+        hipLaunchKernelGGL((rp_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    }
+    return amdseg_launch_status();
 }
 
 template <typename T, int DT, int QT>
@@ -229,11 +425,13 @@ static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
     const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
     if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
     hipLaunchKernelGGL((rp_fwd_kernel<T, DT, QT>), dim3((unsigned)n), dim3(256), lds, s, a);
-    if (a.nsplit > 1) {
-        const int64_t rows = (int64_t)a.B * a.heads * a.Lq;
-        hipLaunchKernelGGL((rp_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-    }
-    return amdseg_launch_status();
+    const int rc2 = amdseg_launch_status();
+    return rc2 ? rc2 : rp_join_launch<T>(a, s);
+}
+template <typename T>
+static int rp_few_d(const RpArgs& a, hipStream_t s) {
+    const int rc = a.D <= 32 ? rp_few_launch<T, 2>(a, s) : a.D <= 64 ? rp_few_launch<T, 4>(a, s) : rp_few_launch<T, 8>(a, s);
+    return rc ? rc : rp_join_launch<T>(a, s);
 }
 template <typename T, int QT>
 static int rp_fwd_d(const RpArgs& a, hipStream_t s) {
@@ -241,6 +439,7 @@ static int rp_fwd_d(const RpArgs& a, hipStream_t s) {
 }
 int amdseg_relpos_fwd_impl(const RpArgs& a0, int dtype, hipStream_t s) {
     RpArgs a = a0;
+    if (rp_few(a)) return dtype == 1 ? rp_few_d<float>(a, s) : rp_few_d<bf16_t>(a, s);
     const int qt = rp_fwd_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
     a.mask_words = rp_mask_bytes(a) / 8;

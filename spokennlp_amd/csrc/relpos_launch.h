@@ -18,10 +18,19 @@ static inline int rp_allow_lds(const void* kernel, int bytes) {
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return e == hipSuccess ? 0 : (int)e;
 }
-// 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products) unless that leaves CUs without a workgroup
+// 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products; 32 x 512 forward 54 us against 64, dK / dV 108 against 146) unless that
+// leaves CUs without a workgroup, and in fp32 (registers).  D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a
+// SIMD (16 x 512: 113 us against 104 with one tile), and a forward grid of three rounds or more runs better on three waves a SIMD of one tile (4 x 2048:
+// 177 against 165).
 static inline int rp_qt(int64_t wgs_of_two, int dtype) { return dtype == 1 ? 1 : wgs_of_two < 256 ? 1 : 2; }
-static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return rp_qt((int64_t)((a.Lq + 127) / 128) * a.B * a.heads, dtype); }
-static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, dtype); }
+static inline int64_t rp_wgs_of_two(const RpArgs& a) { return (int64_t)((a.Lq + 127) / 128) * a.B * a.heads; }
+static inline int rp_dq_qt(const RpArgs& a, int dtype) { return rp_qt(rp_wgs_of_two(a), dtype); }
+static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return a.D > 64 && rp_wgs_of_two(a) >= 768 ? 1 : rp_dq_qt(a, dtype); }
+static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, dtype); }
+// the rows of a kv head's query heads fit the 16 columns of one tile
+static inline bool rp_few(const RpArgs& a) {
+    return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;
+}
 // splits over the keys: few query rows against many keys (single tokens against a cache).  A fixed number of keys per split: a sequence's sums do not
 // depend on the batch around it.
 static inline int rp_nsplit(int Lq, int Lk, bool packed) { return !packed && Lq <= 16 && Lk > RP_SPLIT_KEYS ? (Lk + RP_SPLIT_KEYS - 1) / RP_SPLIT_KEYS : 1; }
