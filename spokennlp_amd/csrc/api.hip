@@ -728,6 +728,7 @@ int amdseg_relpos_attn_fwd(const struct amdseg_relpos_cfg* c, const void* q, con
         !relpos_rows_ok(out, c->out_stride, es, false)) return AMDSEG_ERR_ARG;
     a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse;
     a.nsplit = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
+    a.split_keys = rp_split_keys(a.Lq);
     if (a.nsplit > 1) {
         if (!ws || ((uintptr_t)ws & 15) || ws_bytes < amdseg_relpos_attn_ws_bytes(c, 0)) return AMDSEG_ERR_ARG;
         a.part_o = (float*)ws;

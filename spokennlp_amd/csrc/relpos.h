@@ -15,7 +15,6 @@
 
 #define RP_PAD 112              // 63 (tile rows) + 32 (columns of a wave) + 15 lanes of the gradient's diagonal registers
 #define RP_MAX_SPAN 1024
-#define RP_SPLIT_KEYS 512       // keys of one split of the few-rows form
 #define RP_LOG2E 1.4426950408889634f
 #define RP_LN2 0.6931471805599453f
 
@@ -31,7 +30,7 @@ struct RpArgs {
     float scale;
     int nrb;                    // row blocks of a sequence (grid); a workgroup steps by it, so a wrong `longest` hint costs time, never rows
     int mask_words;             // 8-byte words of the key mask in LDS
-    int nsplit;                 // forward: splits over the keys
+    int nsplit, split_keys;     // forward: splits over the keys, keys of one (a multiple of 64)
     float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
     float* stat;                // backward: what the dK / dV kernel needs of a row: -lse in the exponent's units [rows], -sum_j p_ij dp_ij [rows]
     float* part_d;              // backward: [heads][B * nrb][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL

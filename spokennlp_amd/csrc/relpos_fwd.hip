@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
             const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;                  // the last key any row of the block sees
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
         }
-        if (a.nsplit > 1) { c = split * (RP_SPLIT_KEYS / 64); c_end = min(c_end, c + RP_SPLIT_KEYS / 64); }
+        if (a.nsplit > 1) { c = split * (a.split_keys / 64); c_end = min(c_end, c + a.split_keys / 64); }
         auto fetch = [&](int at, int buf, uint64_t bits) {
             rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
             rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
@@ -219,8 +219,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
     const bool causal = a.causal;
     int c_end = (sq.kn + 63) / 64;
     if (causal) c_end = sq.kn <= 0 || a.Lq - 1 + sq.off < 0 ? 0 : min(c_end, (a.Lq - 1 + sq.off) / 64 + 1);
-    const int c0 = split * (RP_SPLIT_KEYS / 64);
-    c_end = a.nsplit > 1 ? min(c_end, c0 + RP_SPLIT_KEYS / 64) : c_end;
+    const int c0 = split * (a.split_keys / 64);
+    c_end = a.nsplit > 1 ? min(c_end, c0 + a.split_keys / 64) : c_end;
     typename Ti::frag fq[Ti::KB];
     {
         const T* qrow = (const T*)a.q + b * a.sq.sb + (int64_t)qi * a.sq.st + h * a.sq.sh;

@@ -31,6 +31,9 @@ static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : 
 static inline bool rp_few(const RpArgs& a) {
     return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;
 }
-// splits over the keys: few query rows against many keys (single tokens against a cache).  A fixed number of keys per split: a sequence's sums do not
-// depend on the batch around it.
-static inline int rp_nsplit(int Lq, int Lk, bool packed) { return !packed && Lq <= 16 && Lk > RP_SPLIT_KEYS ? (Lk + RP_SPLIT_KEYS - 1) / RP_SPLIT_KEYS : 1; }
+// splits over the keys: few query rows against many keys (single tokens, a handful of rows against a cache), joined by rp_join_kernel.  A number of keys that
+// the shapes alone decide: a sequence's sums do not depend on the batch around it.  (3 x 47 rows of 4 heads against 4545 keys, fp32: 449 -> 148 us.)
+static inline int rp_split_keys(int Lq) { return Lq <= 16 ? 512 : 1024; }
+static inline int rp_nsplit(int Lq, int Lk, bool packed) {
+    return !packed && Lq <= 128 && Lk > rp_split_keys(Lq) ? (Lk + rp_split_keys(Lq) - 1) / rp_split_keys(Lq) : 1;
+}
