@@ -119,7 +119,7 @@ template <int DT> struct RpTile<float, DT> {
     typedef f32x4 frag;
     static constexpr int BYTES = 64 * DT * 64, KB = DT, EPU = 4, UNITS = DT * 4;
     static constexpr int KSTEP = 16, RPS = 1;
-    static __device__ __forceinline__ void piece(int p, int l, int& row, int& c) { row = p * (16 / DT) + l / (DT * 4); c = (l % (DT * 4)) ^ (row & 7); }
+    static __device__ __forceinline__ void piece(int p, int l, int& row, int& c) { row = (p * 64 + l) / UNITS; c = ((p * 64 + l) % UNITS) ^ (row & 7); }
     static __device__ __forceinline__ frag rowf(const char* t, int row, int kb, int g) {
         return *reinterpret_cast<const frag*>(t + row * (DT * 64) + (((kb * 4 + g) ^ (row & 7)) << 4));
     }

@@ -34,33 +34,88 @@ __global__ __launch_bounds__(256) void rp_bias_kernel(RpArgs a, int off, int row
     }
 }
 
-// Read-bound.  A workgroup takes a strip of rows of one (sequence, head).  Places with |rel| < span: a thread owns one rel and walks the rows -- neighbours
-// read neighbouring elements, the sum stays in a register, no order of arrival anywhere.  The two far sides are one sum each: 16 lanes a row, 16-byte loads.
+// Read-bound.  A workgroup takes a strip of rows of one (sequence, head).
+//  * Places with |rel| < span, 8 x 8 blocks at a time: a lane owns a block diagonal and walks it down the strip (its wave takes every fourth block of it), so that
+//    equal rel stay in the same one of its 15 registers; 16 bytes a load, 64 lanes side by side.  At the end the lanes lay their registers into LDS, the lower 8
+//    first, then the upper 7, which belong to the next lane's places: one writer each, no order of arrival anywhere.
+//  * The two far sides are one sum each: 16 lanes a row, 16-byte loads, four under way.
+typedef uint32_t rp_u4 __attribute__((ext_vector_type(4), aligned(2)));      // 16 bytes from any element: rows start where they start
+template <typename T> __device__ __forceinline__ void rp_ld8(const T* p, float (&v)[8]);
+template <> __device__ __forceinline__ void rp_ld8<bf16_t>(const bf16_t* p, float (&v)[8]) {
+    const rp_u4 q = *reinterpret_cast<const rp_u4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(q[i] << 16); v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void rp_ld8<float>(const float* p, float (&v)[8]) {
+    const rp_u4 a = *reinterpret_cast<const rp_u4*>(p), b = *reinterpret_cast<const rp_u4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
+}
+__device__ __forceinline__ float rp_sum16(uint4 q, float) {
+    return (__uint_as_float(q.x) + __uint_as_float(q.y)) + (__uint_as_float(q.z) + __uint_as_float(q.w));
+}
+__device__ __forceinline__ float rp_sum16(uint4 q, bf16_t) {
+    const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xffff0000u);
+    return s;
+}
 template <typename T>
 __global__ __launch_bounds__(256) void rp_bias_bwd_kernel(const T* d, float* part, int Lq, int Lk, int span, int off, int rows) {
+    __shared__ float bins[4][64 * 8 + 8];
     __shared__ float red[2][4];
     constexpr int E = 16 / sizeof(T);
-    const int tid = threadIdx.x, nd = 2 * span + 1, h = blockIdx.y, b = blockIdx.z, heads = gridDim.y;
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, nd = 2 * span + 1, h = blockIdx.y, b = blockIdx.z, heads = gridDim.y;
     const int i0 = blockIdx.x * rows, i1 = min(i0 + rows, Lq);
     const int64_t plane = ((int64_t)b * heads + h) * Lq;
     float* out = part + (((int64_t)h * gridDim.z + b) * gridDim.x + blockIdx.x) * nd;
-    for (int x = tid + 1; x < nd - 1; x += 256) {           // rel = x - span strictly inside
-        const int rel = x - span;
-        // rows with 0 <= i + off + rel < Lk
-        const int a0 = max(i0, -off - rel), a1 = min(i1, Lk - off - rel);
-        const T* p = d + (plane + a0) * Lk + (a0 + off + rel);
-        float s = 0.f;
-        int i = a0;
-        for (; i + 8 <= a1; i += 8) {
-            float v[8];
+    // block diagonal n holds rel 8 n - span - 7 .. 8 n - span + 7, register e the e-th of them
+    for (int n0 = 0; n0 * 8 <= 2 * span + 6; n0 += 64) {
+        const int n = n0 + l, rel = 8 * n - span;           // rel of the block's main diagonal
+        float acc[15];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = Act<T>::ld(p + (int64_t)e * (Lk + 1));
+        for (int e = 0; e < 15; ++e) acc[e] = 0.f;
+        if (rel - 7 < span)
+            for (int i = i0 + 8 * w; i < i1; i += 32) {
+                const int j = i + off + rel;                // the block's first column
+                if (j <= -8 || j >= Lk) continue;
+                const T* p = d + (plane + i) * Lk + j;
+                if (j >= 0 && j + 8 <= Lk && i + 8 <= i1) {
+                    float v[8][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += v[e];
-            p += (int64_t)8 * (Lk + 1);
+                    for (int r = 0; r < 8; ++r) rp_ld8<T>(p + (int64_t)r * Lk, v[r]);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[7 + e - r] += v[r][e];
+                } else
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (i + r < i1)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (j + e >= 0 && j + e < Lk) acc[7 + e - r] += Act<T>::ld(p + (int64_t)r * Lk + e);
+            }
+        // place x of `out` is rel x - span; register e of block diagonal n is place 8 n - 7 + e
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bins[w][8 * l + e] = acc[e];
+        if (l == 63)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bins[w][512 + e] = 0.f;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 7; ++e) bins[w][8 * (l + 1) + e] += acc[8 + e];
+        __syncthreads();
+        for (int x = tid; x < 520; x += 256) {
+            const int place = 8 * n0 - 7 + x;
+            if (place >= 1 && place < nd - 1) {
+                const float s = (bins[0][x] + bins[1][x]) + (bins[2][x] + bins[3][x]);
+                // (the first 8 places of a later round of 64 diagonals have had the upper registers of the round before)
+                out[place] = n0 > 0 && x < 8 ? out[place] + s : s;
+            }
         }
-        for (; i < a1; ++i) { s += Act<T>::ld(p); p += Lk + 1; }
-        out[x] = s;
+        __syncthreads();
     }
     float sl = 0.f, sr = 0.f;
     const int l16 = tid & 15;
@@ -73,24 +128,23 @@ __global__ __launch_bounds__(256) void rp_bias_bwd_kernel(const T* d, float* par
         for (int side = 0; side < 2; ++side) {
             const int ja = side ? jr : 0, jb = side ? Lk : jl;
             float s = 0.f;
-            for (int u = (ja + mis) / E + l16; u * E - mis < jb; u += 16) {
-                const int j = u * E - mis;
-                if (j >= ja && j + E <= jb) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(row + j);
-                    const uint32_t v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s += sizeof(T) == 2 ? __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u) : __uint_as_float(v[e]);
-                } else
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (j + e >= ja && j + e < jb) s += Act<T>::ld(row + j + e);
+            const int ua = (ja + mis + E - 1) / E, ub = (jb + mis) / E;           // whole 16-byte units
+            const uint4* unit = reinterpret_cast<const uint4*>(row - mis);
+            int u = ua + l16;
+            for (; u + 48 < ub; u += 64) {
+                const uint4 q0 = unit[u], q1 = unit[u + 16], q2 = unit[u + 32], q3 = unit[u + 48];
+                s += (rp_sum16(q0, T(0)) + rp_sum16(q1, T(0))) + (rp_sum16(q2, T(0)) + rp_sum16(q3, T(0)));
             }
+            for (; u < ub; u += 16) s += rp_sum16(unit[u], T(0));
+            // the elements in front of the first whole unit and behind the last
+            const int h1 = min(ua * E - mis, jb), t0 = max(ub * E - mis, h1);
+            if (ja + l16 < h1) s += Act<T>::ld(row + ja + l16);
+            if (t0 + l16 < jb) s += Act<T>::ld(row + t0 + l16);
             if (side) sr += s; else sl += s;
         }
     }
     sl = wave_sum(sl); sr = wave_sum(sr);
-    if ((tid & 63) == 0) { red[0][tid >> 6] = sl; red[1][tid >> 6] = sr; }
+    if (l == 0) { red[0][w] = sl; red[1][w] = sr; }
     __syncthreads();
     if (tid == 0) {
         const float L = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]), R = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);

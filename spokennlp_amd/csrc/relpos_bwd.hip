@@ -639,7 +639,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
 template <typename T>
 static int rp_bwd_d(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {
     return a.D <= 32 ? rp_bwd_launch<T, 2>(a, dtype, dtable, sums, s) : a.D <= 64 ? rp_bwd_launch<T, 4>(a, dtype, dtable, sums, s)
-                                                                              : rp_bwd_launch<T, 8>(a, dtype, dtable, sums, s);
+                                                                              : a.D <= 96 ? rp_bwd_launch<T, 6>(a, dtype, dtable, sums, s) : rp_bwd_launch<T, 8>(a, dtype, dtable, sums, s);
 }
 int amdseg_relpos_bwd_impl(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {
     return dtype == 1 ? rp_bwd_d<float>(a, dtype, dtable, sums, s) : rp_bwd_d<bf16_t>(a, dtype, dtable, sums, s);

@@ -430,12 +430,13 @@ static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
 }
 template <typename T>
 static int rp_few_d(const RpArgs& a, hipStream_t s) {
-    const int rc = a.D <= 32 ? rp_few_launch<T, 2>(a, s) : a.D <= 64 ? rp_few_launch<T, 4>(a, s) : rp_few_launch<T, 8>(a, s);
+    const int rc = a.D <= 32 ? rp_few_launch<T, 2>(a, s) : a.D <= 64 ? rp_few_launch<T, 4>(a, s) : a.D <= 96 ? rp_few_launch<T, 6>(a, s) : rp_few_launch<T, 8>(a, s);
     return rc ? rc : rp_join_launch<T>(a, s);
 }
 template <typename T, int QT>
 static int rp_fwd_d(const RpArgs& a, hipStream_t s) {
-    return a.D <= 32 ? rp_fwd_launch<T, 2, QT>(a, s) : a.D <= 64 ? rp_fwd_launch<T, 4, QT>(a, s) : rp_fwd_launch<T, 8, QT>(a, s);
+    return a.D <= 32 ? rp_fwd_launch<T, 2, QT>(a, s) : a.D <= 64 ? rp_fwd_launch<T, 4, QT>(a, s) : a.D <= 96 ? rp_fwd_launch<T, 6, QT>(a, s)
+                                                                                          : rp_fwd_launch<T, 8, QT>(a, s);
 }
 int amdseg_relpos_fwd_impl(const RpArgs& a0, int dtype, hipStream_t s) {
     RpArgs a = a0;
