@@ -15,6 +15,7 @@
 
 #define RP_PAD 112              // 63 (tile rows) + 32 (columns of a wave) + 15 lanes of the gradient's diagonal registers
 #define RP_MAX_SPAN 1024
+#define RP_MAX_WGS ((1 << 24) - 1)   // a grid has less than 2^32 threads
 #define RP_LOG2E 1.4426950408889634f
 #define RP_LN2 0.6931471805599453f
 

@@ -166,6 +166,7 @@ size_t amdseg_relpos_bias_ws_impl(int B, int heads, int Lq, int span) {
 int amdseg_relpos_bias_fwd_impl(const RpArgs& a, int off, int dtype, hipStream_t s) {
     const int rows = rp_bias_rows(a.heads, a.Lq), lds = (2 * a.span + 1 + (2 * a.span + 1) / 8 + 1) * 4;
     const dim3 grid((a.Lq + rows - 1) / rows, a.heads);
+    if (grid.x > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     if (dtype == 1) hipLaunchKernelGGL((rp_bias_kernel<float>), grid, dim3(256), lds, s, a, off, rows);
     else hipLaunchKernelGGL((rp_bias_kernel<bf16_t>), grid, dim3(256), lds, s, a, off, rows);
     return amdseg_launch_status();
@@ -174,6 +175,7 @@ int amdseg_relpos_bias_bwd_impl(const void* d, int dtype, const int* map, int sp
                                 float* ws, hipStream_t s) {
     const int rows = rp_bias_rows((int64_t)B * heads, Lq), nd = 2 * span + 1;
     const dim3 grid((Lq + rows - 1) / rows, heads, B);
+    if (grid.x > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     float* part = ws + (size_t)nd * heads;
     if (B == 0) return amdseg_relpos_sums_impl(part, ws, 0, map, span, 0, buckets, heads, dtable, 0, s);       // nothing to sum: zeros
     if (dtype == 1) hipLaunchKernelGGL((rp_bias_bwd_kernel<float>), grid, dim3(256), 0, s, (const float*)d, part, Lq, Lk, span, off, rows);

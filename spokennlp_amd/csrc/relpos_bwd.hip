@@ -609,7 +609,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int qt = rp_dq_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
     const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
-    if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
     int rc;
     if (n == 0) {
@@ -623,7 +623,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     if ((rc = amdseg_launch_status())) return rc;
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
     const int64_t m = (int64_t)a.B * a.kv_heads * a.nrb + tail;
-    if (m > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    if (m > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
     } else if (sizeof(T) == 4 || DT > 4 || kt == 1) {

@@ -412,6 +412,7 @@ template <typename T>
 static int rp_join_launch(const RpArgs& a, hipStream_t s) {
     if (a.nsplit > 1) {
         const int64_t rows = (int64_t)a.B * a.heads * a.Lq;
+        if ((rows + 3) / 4 > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
         hipLaunchKernelGGL((rp_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
     }
     return amdseg_launch_status();
@@ -423,7 +424,7 @@ static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
     const int rc = rp_allow_lds((const void*)rp_fwd_kernel<T, DT, QT>, lds);
     if (rc) return rc;
     const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
-    if (n > 0x7fffffff) return AMDSEG_ERR_SHAPE;
+    if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     hipLaunchKernelGGL((rp_fwd_kernel<T, DT, QT>), dim3((unsigned)n), dim3(256), lds, s, a);
     const int rc2 = amdseg_launch_status();
     return rc2 ? rc2 : rp_join_launch<T>(a, s);

@@ -247,6 +247,69 @@ def test_packed(dev, dtype, causal):
         assert bool((x[end:] == 7.0).all()) and not bool((x[:end] == 7.0).all())
 
 
+def test_packed_rows_in_front(dev):
+    """offsets that do not start at 0: the rows in front belong to no sequence either"""
+    ops = _ops()
+    q, k, v, table, lut, dout = (x[0] if x.dim() == 4 else x for x in make(dev, torch.float32, 1, 90, 90, 4, 2, 64))
+    cu, at0 = torch.tensor([17, 60, 80], dtype=torch.int32, device=dev), torch.tensor([0, 43, 63], dtype=torch.int32, device=dev)
+    out, lse = ops.relpos_attn_fwd(q, k, v, table, lut, cu_q=cu, cu_k=cu)
+    grads = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, cu_q=cu, cu_k=cu)
+    o2, l2 = ops.relpos_attn_fwd(q[17:80], k[17:80], v[17:80], table, lut, cu_q=at0, cu_k=at0)
+    g2 = ops.relpos_attn_bwd(q[17:80], k[17:80], v[17:80], table, lut, o2, dout[17:80], l2, cu_q=at0, cu_k=at0)
+    for x, y in zip((out,) + grads[:3], (o2,) + g2[:3]):
+        assert torch.equal(x[17:80], y) and not x[:17].any() and not x[80:].any()
+    assert torch.equal(lse[:, 17:80], l2) and bool((lse[:, :17] == -math.inf).all()) and rel(grads[3], g2[3]) < 2e-5
+
+
+def test_offsets_past_32_bits(dev):
+    """a cache whose sequences start more than 2^31 elements apart, keys broadcast over heads by a stride of 0"""
+    ops = _ops()
+    cap, Hk, D = 1 << 24, 2, 64                              # 2^31 elements a sequence
+    big = torch.empty(2 * cap * Hk * D, dtype=torch.bfloat16, device=dev)
+    kv = big.view(2, cap, Hk, D)
+    q, k, v, table, lut, dout = make(dev, torch.bfloat16, 2, 3, 700, 4, 2, 64)
+    kv[:, cap - 700:] = k
+    far = kv[:, cap - 700:]
+    assert far.stride(0) == 1 << 31
+    out, lse = ops.relpos_attn_fwd(q, far, v, table, lut)
+    want, wl = ops.relpos_attn_fwd(q, k, v, table, lut)
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    q2 = torch.randn(2, 200, 4, D, device=dev).bfloat16()
+    out, lse = ops.relpos_attn_fwd(q2, far, v, table, lut)
+    want, wl = ops.relpos_attn_fwd(q2, k, v, table, lut)
+    assert torch.equal(out, want)
+    for x, y in zip(ops.relpos_attn_bwd(q2, far, v, table, lut, out, q2, lse), ops.relpos_attn_bwd(q2, k, v, table, lut, want, q2, wl)):
+        assert torch.equal(x, y)
+    del big, kv, far
+    one = k[:, :, :1]
+    a = ops.relpos_attn_fwd(q2, one.expand(-1, -1, 2, -1), v, table, lut)[0]
+    assert torch.equal(a, ops.relpos_attn_fwd(q2, one.expand(-1, -1, 2, -1).contiguous(), v, table, lut)[0])
+
+
+def test_infinite_table_entries_hide_a_bucket(dev):
+    """a bucket at -inf: its keys have p = 0 in forward and backward, near and far, and no gradient; a row whose every key is in it is empty"""
+    ops = _ops()
+    for dtype in (torch.bfloat16, torch.float32):
+        q, k, v, table, lut, dout = make(dev, dtype, 2, 300, 400, 2, 2, 64, buckets=8, max_distance=48)
+        table = table.clone()
+        table[3], table[7, 1] = -math.inf, -math.inf         # far left for both heads, far right for the second
+        finite = torch.isfinite(table)
+        out, lse = ops.relpos_attn_fwd(q, k, v, table, lut)
+        g = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse)
+        r = torch.arange(400, device=dev)[None] - torch.arange(300, device=dev)[:, None]
+        b = table.to(F64)[lut.long()[r.clamp(-48, 48) + 48]].permute(2, 0, 1)
+        qq, kk, vv = (x.to(F64).requires_grad_(True) for x in (q, k, v))
+        p = torch.softmax(torch.einsum("bihd,bjhd->bhij", qq, kk) / 8 + b, -1)
+        o = torch.einsum("bhij,bjhd->bihd", p, vv)
+        o.backward(dout.to(F64))
+        assert max(rel(x, y) for x, y in zip((out,) + g[:3], (o.detach(), qq.grad, kk.grad, vv.grad))) < TOL[dtype]
+        assert not g[3][~finite].any() and bool(torch.isfinite(g[3]).all())
+        table[:] = -math.inf
+        out, lse = ops.relpos_attn_fwd(q, k, v, table, lut)
+        g = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse)
+        assert not any(x.any() for x in (out,) + g) and bool((lse == -math.inf).all())
+
+
 def test_packed_with_bad_offsets_stays_inside(dev):
     """offsets that run backwards or past the buffers are clamped on the device: some rows are wrong, none outside is touched"""
     ops = _ops()
@@ -319,9 +382,9 @@ def test_graph_replay_and_streams(dev):
     """captured and replayed (twice the same graph pool, two graphs alive at once, eager work between), and on a side stream"""
     ops = _ops()
     sets = []
-    for n, (B, L) in enumerate(((2, 200), (1, 700))):
-        q, k, v, table, lut, dout = make(dev, torch.bfloat16, B, L, L, 4, 2, 64, seed=n)
-        tok = torch.randn(B, 1, 4, 64, device=dev).bfloat16()
+    for n, (B, L, D) in enumerate(((2, 200, 64), (1, 700, 64), (2, 300, 128))):        # (D = 128: more than 64 KiB of LDS, asked for at every launch)
+        q, k, v, table, lut, dout = make(dev, torch.bfloat16, B, L, L, 4, 2, D, seed=n)
+        tok = torch.randn(B, 1, 4, D, device=dev).bfloat16()
 
         def step(q=q, k=k, v=v, table=table, lut=lut, dout=dout, tok=tok):
             out, lse = ops.relpos_attn_fwd(q, k, v, table, lut, causal=True)
@@ -391,3 +454,120 @@ def test_empty_calls(dev):
     q = torch.randn(5, 4, 64, device=dev)
     out, lse = ops.relpos_attn_fwd(q, q, q, table, lut, cu_q=cu, cu_k=cu)
     assert not out.any() and not any(x.any() for x in ops.relpos_attn_bwd(q, q, q, table, lut, out, q, lse, cu_q=cu, cu_k=cu))
+
+
+# ------------------------------------------------------------------------------------------------ differentiable surface
+def test_autograd_functions(dev):
+    """gradients through torch autograd: q / k / v leaves, a fused projection (padded, packed with rows outside), the dense bias; dout of any strides"""
+    from spokennlp_amd import relpos as R
+    ops = _ops()
+    q, k, v, table, lut, dout = make(dev, torch.float32, 2, 70, 90, 4, 2, 64)
+    out, lse = ops.relpos_attn_fwd(q, k, v, table, lut)
+    want = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v, table)]
+    R.relpos_attention(*leaves, lut).backward(dout.transpose(1, 3).contiguous().transpose(1, 3))      # last dimension strided
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, want))
+    # an expanded dout (the gradient of a sum)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v, table)]
+    R.relpos_attention(*leaves, lut).sum().backward()
+    ones = ops.relpos_attn_bwd(q, k, v, table, lut, out, torch.ones_like(out), lse)
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, ones))
+    # only some leaves
+    t = table.clone().requires_grad_(True)
+    R.relpos_attention(q, k, v, t, lut).backward(dout)
+    assert torch.equal(t.grad, want[3])
+    with torch.no_grad():
+        assert torch.equal(R.relpos_attention(q, k, v, table, lut), out)
+    # fused, packed
+    lens, H, Hk, D = [33, 0, 70], 4, 2, 64
+    cu = torch.tensor([0, 33, 33, 103], dtype=torch.int32, device=dev)
+    qkv = torch.randn(110, (H + 2 * Hk) * D, generator=torch.Generator().manual_seed(1)).to(dev)
+    d = torch.randn(110, H * D, generator=torch.Generator().manual_seed(2)).to(dev)
+    a, t = qkv.clone().requires_grad_(True), table.clone().requires_grad_(True)
+    y = R.relpos_self_attention(a, H, t, lut, kv_heads=Hk, cu_seqlens=cu, longest=70)
+    y.backward(d)
+    assert not y[103:].any() and not a.grad[103:].any() and bool(torch.isfinite(a.grad).all())
+    b, t2 = qkv.clone().requires_grad_(True), table.clone().requires_grad_(True)
+    parts = [R.relpos_self_attention(b[None, s:e], H, t2, lut, kv_heads=Hk) for s, e in ((0, 33), (33, 103))]
+    torch.cat([p[0] for p in parts]).backward(d[:103])
+    assert torch.equal(a.grad[:103], b.grad[:103]) and rel(t.grad, t2.grad) < 2e-5
+    # dense bias feeding composed attention equals the fused one
+    t3 = table.clone().requires_grad_(True)
+    s = torch.einsum("bihd,bjhd->bhij", q, k.repeat_interleave(2, 2)) * 64 ** -0.5 + R.relpos_bias(t3, lut, 70, 90)
+    o = torch.einsum("bhij,bjhd->bihd", torch.softmax(s, -1), v.repeat_interleave(2, 2))
+    o.backward(dout)
+    assert rel(o, out) < 2e-5 and rel(t3.grad, want[3]) < 2e-5
+
+
+def test_layers_together_and_a_training_step(dev):
+    """two layers that share one table, bf16 module under the framework's own optimiser kernel: forward and every gradient against the same layers composed
+    in 64 bits; padded and packed inputs give the same tokens"""
+    from spokennlp_amd import relpos as R
+    ops = _ops()
+    torch.manual_seed(0)
+    Hs, heads, L, lens = 256, 4, 150, [150, 97, 1]
+    l0 = R.RelPosSelfAttention(Hs, heads, kv_heads=2).to(dev)
+    l1 = R.RelPosSelfAttention(Hs, heads, kv_heads=2, table=l0.table).to(dev)
+    assert l1.table is l0.table and len(list(torch.nn.ModuleList([l0, l1]).parameters())) == 9
+    x = torch.randn(3, L, Hs, device=dev)
+    mask = torch.arange(L, device=dev)[None] < torch.tensor(lens, device=dev)[:, None]
+    w = torch.randn(3, L, Hs, device=dev) * mask[..., None]
+
+    def run(xx, **kw):
+        h = xx + l0(xx, **kw)
+        return h + l1(h, **kw)
+    y = run(x, key_mask=mask)
+    (y * w).sum().backward()
+    grads = {n: p.grad.clone() for n, p in torch.nn.ModuleList([l0, l1]).named_parameters()}
+    # packed
+    cu = torch.tensor([0, 150, 247, 248], dtype=torch.int32, device=dev)
+    yp = run(x[mask], cu_seqlens=cu, longest=150)
+    assert rel(yp, y[mask]) < 2e-6
+    # 64 bits
+    P = {n: p.detach().to(F64).requires_grad_(True) for n, p in torch.nn.ModuleList([l0, l1]).named_parameters()}
+
+    def layer(h, i):
+        qkv = h @ P[f"{i}.qkv.weight"].t() + P[f"{i}.qkv.bias"]
+        q, k, v = (t.unflatten(-1, (-1, 64)) for t in qkv.split([256, 128, 128], -1))
+        r = torch.arange(L, device=dev)[None] - torch.arange(L, device=dev)[:, None]
+        b = P["0.table"][l0.bucket_map.long()[r.clamp(-128, 128) + 128]].permute(2, 0, 1)
+        s = torch.einsum("bihd,bjhd->bhij", q, k.repeat_interleave(2, 2)) / 8 + b
+        p = torch.softmax(s.masked_fill(~mask[:, None, None], -math.inf), -1)
+        return torch.einsum("bhij,bjhd->bihd", p, v.repeat_interleave(2, 2)).flatten(-2) @ P[f"{i}.out.weight"].t() + P[f"{i}.out.bias"]
+    h = x.to(F64)
+    h = h + layer(h, 0)
+    h = h + layer(h, 1)
+    assert rel(y * mask[..., None], h.detach() * mask[..., None]) < 2e-5
+    (h * w.to(F64)).sum().backward()
+    for n, g in grads.items():
+        assert rel(g, P[n].grad) < 5e-5, n                   # two layers of fp32 products, each within 2e-5
+    # one optimiser step of the shared table and its gradient through amdseg_adamw
+    p, m, v2 = l0.table.detach().clone().flatten(), torch.zeros(128, device=dev), torch.zeros(128, device=dev)
+    ops.adamw(p, grads["0.table"].flatten().contiguous(), m, v2, None, 1e-2, 0.9, 0.999, 1e-8, 0.0, 1)
+    assert bool(((p - l0.table.detach().flatten()).abs() <= 1.0001e-2).all()) and bool((p != l0.table.detach().flatten()).any())
+
+
+def test_backward_captured_beside_a_living_eager_graph(dev):
+    """a training step captured into a graph while an eager graph of the same leaves is alive (its buffers held): both finish, with the same gradients"""
+    from spokennlp_amd import relpos as R
+    q, k, v, table, lut, dout = make(dev, torch.bfloat16, 2, 130, 130, 4, 2, 64)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v, table)]
+    eager = R.relpos_attention(*leaves, lut)
+    copies = [x.detach().clone().requires_grad_(True) for x in leaves]
+
+    def step():
+        o = R.relpos_attention(*copies, lut)
+        return torch.autograd.grad(o, copies, dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    eager.backward(dout)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y.grad) for x, y in zip(got, leaves))

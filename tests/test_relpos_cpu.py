@@ -106,3 +106,18 @@ def test_python_surface_refuses():
         ops.relpos_bias_fwd(torch.zeros(8, 4), torch.zeros(17, dtype=torch.int32), 4, 4)
     with pytest.raises(ValueError):
         ops.relpos_bias_bwd(torch.zeros(1, 4, 4, 4), torch.zeros(17, dtype=torch.int32), 8)
+
+
+def test_module_shapes_and_refusals():
+    from spokennlp_amd import relpos as R
+    m = R.RelPosSelfAttention(256, 4, kv_heads=2, buckets=16, max_distance=64)
+    assert m.qkv.weight.shape == (512, 256) and m.table.shape == (16, 4) and m.bucket_map.tolist() == ops.relpos_bucket_list(16, 64, True)
+    assert "bucket_map" not in m.state_dict()
+    with pytest.raises(ValueError):
+        R.RelPosSelfAttention(256, 4, kv_heads=3)
+    with pytest.raises(ValueError):
+        R.RelPosSelfAttention(256, 4, table=torch.nn.Parameter(torch.zeros(8, 4)))
+    with pytest.raises(ValueError, match="columns"):
+        R.relpos_self_attention(torch.zeros(1, 4, 500), 4, m.table, m.bucket_map)
+    with pytest.raises(ValueError, match="one GPU"):
+        m(torch.zeros(1, 4, 256))
