@@ -10,6 +10,7 @@
 #pragma once
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include "common.h"
 #include "tile64.h"
 
@@ -102,6 +103,11 @@ template <int DT> struct RpTile<bf16_t, DT> {
         const uint4 u = make_uint4(rp_pack2(s[0][0], s[0][1]), rp_pack2(s[0][2], s[0][3]), rp_pack2(s[1][0], s[1][1]), rp_pack2(s[1][2], s[1][3]));
         return __builtin_bit_cast(frag, u);
     }
+    // x - what pf() kept of x
+    static __device__ __forceinline__ void less(f32x4* x, frag f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] -= bf2f((bf16_t)f[e]);
+    }
     // the columns kb * 32 + g * 8 .. + 7 of one row of a global tensor, zero beyond D
     static __device__ __forceinline__ frag gfrag(const bf16_t* row, int kb, int g, int D, bool ok) {
         frag f = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -140,6 +146,7 @@ template <int DT> struct RpTile<float, DT> {
         return c;
     }
     static __device__ __forceinline__ frag pf(const f32x4* s) { return s[0]; }
+    static __device__ __forceinline__ void less(f32x4* x, frag) { x[0] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
     static __device__ __forceinline__ frag gfrag(const float* row, int kb, int g, int D, bool ok) {
         frag f = {0.f, 0.f, 0.f, 0.f};
         if (ok && kb * 16 + g * 4 < D) f = *reinterpret_cast<const frag*>(row + kb * 16 + g * 4);

@@ -8,8 +8,11 @@
 // delta.  sum_j ds_ij = 0, so a bucket that holds most of a row's probability has for its gradient what is left of a cancellation; delta taken from the
 // bf16 `out` is off by up to 2^-8 of it, the same way for every element of the row (1 % of dtable measured, 40 queries against 3 .. 1500 keys).  What the
 // ds of a row sum to instead of 0 IS that error (sum_j p_ij = 1): rp_dq_kernel sums them in fp32 on its way and hands the mended delta on.  Its own dq
-// feels the error only where a row's probability sits on a few keys (by 1 / sqrt of their number): row blocks of at most RP_TWICE_KEYS keys walk them
-// twice, the first time for the sum alone (dq of 33-token sequences: 2.5e-3 -> 2.3e-3 of its norm; longer ones 2.4e-3 either way).
+// feels the error only where a row's probability sits on a few keys (by 1 / sqrt of their number), beside the rounding of ds to bf16 for the product with k.
+// Row blocks of at most RP_FINE keys, and sequences of at most RP_FINE / 2 rows (too few values for roundings to average out), have ds as two bf16 parts there:
+// dq within 1.8e-3 of its norm instead of 2.5e-3, one more product of the three, on blocks whose time is latency.  (A copy of the whole walk, FINE, in a
+// kernel of its own instance, MIXED: as a branch inside the chunk it cost D = 128 its registers, 4 x 2048 200 -> 467 us, beside the walk 239 us; as a second
+// launch it took 30 us more of a causal 3 x 1023 at D = 128, this way 11.)
 //
 // dtable.  In the accumulator layout lane (g, i16) holds ds of query 4 g + r (register r) and key i16, so -rel = const + 4 g + r - i16.  Moving register r
 // by r lanes inside its 16 (a DPP operand modifier of the add itself) puts equal rel into equal lanes: the 16 x 16 tiles of one block diagonal add
@@ -19,7 +22,7 @@
 #include "relpos.h"
 #include "relpos_launch.h"
 
-#define RP_TWICE_KEYS 128
+#define RP_FINE 128
 
 template <int CTRL>
 __device__ __forceinline__ float rp_dpp(float v) {
@@ -58,7 +61,17 @@ __device__ __forceinline__ float rp_join4(float x0, float x1, float x2, float x3
     return a + b;
 }
 
-template <typename T, int DT, int QT>
+// keys that the 128-row block of row q0 may see, in whole chunks (the same for either QT: a row's bits must not depend on the grid)
+__device__ __forceinline__ bool rp_fine(const RpArgs& a, const RpSeq& sq, int q0) {
+    int c = (sq.kn + 63) / 64;
+    if (a.causal) {
+        const int last = min(q0 / 128 * 128 + 128, sq.qn) - 1 + sq.off;
+        c = last < 0 ? 0 : min(c, last / 64 + 1);
+    }
+    return c * 64 <= RP_FINE || sq.qn <= RP_FINE / 2;
+}
+
+template <typename T, int DT, int QT_, bool MIXED>
 __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
@@ -75,8 +88,9 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     int rb, h, b;
     rp_place(blockIdx.x, a.nrb, a.B, a.heads, a.kv_heads, rb, h, b);
     const RpSeq sq = rp_seq(a, b);
-    constexpr int BQ = 64 * QT;
-    if (rb * BQ >= sq.qn) return;
+    constexpr int BQ_ = 64 * QT_;
+    constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums, and so is ds)
+    if (rb * BQ_ >= sq.qn) return;
     RpTable table;
     table.start(a, 1, tid);
     RpStage<T, DT> rk, rv;
@@ -93,18 +107,17 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     const float c2 = a.scale * RP_LOG2E;
     const int mid = a.span + RP_PAD, span = a.span;
     const bool causal = a.causal;
-    constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums)
     const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
     bool first = true;
 
-    for (; rb * BQ < sq.qn; rb += a.nrb) {
-        const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
-        int c_end = (sq.kn + 63) / 64, c_128 = c_end;
+    auto block = [&](auto qt_, auto fine_, const int q0) __attribute__((always_inline)) {
+        constexpr int QT = decltype(qt_)::value, BQ = 64 * QT;
+        constexpr bool FINE = decltype(fine_)::value;
+        const int qw = q0 + w * 16 * QT;
+        int c_end = (sq.kn + 63) / 64;
         if (causal) {
             const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
-            const int last128 = min(q0 / 128 * 128 + 128, sq.qn) - 1 + sq.off;  // (the rule must not depend on QT)
-            c_128 = last128 < 0 ? 0 : min(c_128, last128 / 64 + 1);
         }
         typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
         float nl[QT], rsum[QT];                             // -lse in the exponent's units; sum of a row's ds (each of its four lanes: a quarter of the keys)
@@ -116,96 +129,100 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) dq[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
-        const int pass0 = MEND && c_128 * 64 <= RP_TWICE_KEYS ? 0 : 1;
-        for (int pass = pass0; pass < 2; ++pass) {
-            auto fetch = [&](int at, int buf, uint64_t bits) {
-                rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
-                rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
-            };
-            uint64_t bits;
-            int c = keys.seek(0, c_end, bits), buf = 0;
-            if (!first) __syncthreads();                    // (nobody is left in the buffers)
-            if (NB == 2 && c < c_end) fetch(c, 0, bits);    // on its way before anything else is waited for
-            if (pass == pass0) {
-                typename Ti::frag fo[QT][Ti::KB];
-                float lse[QT];                              // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
+        auto fetch = [&](int at, int buf, uint64_t bits) {
+            rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
+            rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        };
+        uint64_t bits;
+        int c = keys.seek(0, c_end, bits), buf = 0;
+        if (!first) __syncthreads();                    // (nobody is left in the buffers)
+        if (NB == 2 && c < c_end) fetch(c, 0, bits);    // on its way before anything else is waited for
+        typename Ti::frag fo[QT][Ti::KB];
+        float lse[QT];                              // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
 #pragma unroll
-                for (int ct = 0; ct < QT; ++ct) {
-                    const int q = qw + ct * 16 + i16;
-                    const bool ok = q < sq.qn;
-                    const int64_t qt = (int64_t)(sq.q0 + q);
+        for (int ct = 0; ct < QT; ++ct) {
+            const int q = qw + ct * 16 + i16;
+            const bool ok = q < sq.qn;
+            const int64_t qt = (int64_t)(sq.q0 + q);
 #pragma unroll
-                    for (int kk = 0; kk < Ti::KB; ++kk) {
-                        fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
-                        fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
-                        fo[ct][kk] = Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok);
-                    }
-                    lse[ct] = ok ? a.lse[rp_row(a, sq, b, h, q)] : INFINITY;
-                }
-                if (first) table.finish(a, tab, h);
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct) {
-                    float acc = 0.f;
-#pragma unroll
-                    for (int kk = 0; kk < Ti::KB; ++kk) acc += Ti::dot(fdo[ct][kk], fo[ct][kk]);
-                    acc += __shfl_xor(acc, 16, 64);
-                    acc += __shfl_xor(acc, 32, 64);
-                    nd[ct] = (f32x4){-acc, -acc, -acc, -acc};
-                    nl[ct] = lse[ct] == -INFINITY ? -INFINITY : -lse[ct] * RP_LOG2E;
-                }
+            for (int kk = 0; kk < Ti::KB; ++kk) {
+                fq[ct][kk] = Ti::gfrag((const T*)a.q + b * a.sq.sb + qt * a.sq.st + h * a.sq.sh, kk, g, a.D, ok);
+                fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
+                fo[ct][kk] = Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok);
             }
-            first = false;
-            auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
-                const char* tV = tK + Ti::BYTES;
-                const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
-                float al[QT];
+            lse[ct] = ok ? a.lse[rp_row(a, sq, b, h, q)] : INFINITY;
+        }
+        if (first) table.finish(a, tab, h);
 #pragma unroll
-                for (int ct = 0; ct < QT; ++ct) al[ct] = nl[ct] + fc;
-                const float* bt = tab + (rel0 + mid + 4 * g - i16);
+        for (int ct = 0; ct < QT; ++ct) {
+            float acc = 0.f;
 #pragma unroll
-                for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
-                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], z[Ti::RPS + QT - 1];
-                    rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
+            for (int kk = 0; kk < Ti::KB; ++kk) acc += Ti::dot(fdo[ct][kk], fo[ct][kk]);
+            acc += __shfl_xor(acc, 16, 64);
+            acc += __shfl_xor(acc, 32, 64);
+            nd[ct] = (f32x4){-acc, -acc, -acc, -acc};
+            nl[ct] = lse[ct] == -INFINITY ? -INFINITY : -lse[ct] * RP_LOG2E;
+        }
+        first = false;
+        auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
+            const char* tV = tK + Ti::BYTES;
+            const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
+            float al[QT];
 #pragma unroll
-                    for (int kk = 0; kk < Ti::KB; ++kk)
+            for (int ct = 0; ct < QT; ++ct) al[ct] = nl[ct] + fc;
+            const float* bt = tab + (rel0 + mid + 4 * g - i16);
 #pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j) {
-                            const int f = kp * Ti::RPS + j;
-                            const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
+            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], z[Ti::RPS + QT - 1];
+                rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
 #pragma unroll
-                            for (int ct = 0; ct < QT; ++ct) {
-                                const f32x4 start = z[j - ct + QT - 1];
-                                s[ct][j] = Ti::mma(fk, fq[ct][kk], kk == 0 ? start : s[ct][j]);
-                                dp[ct][j] = Ti::mma(fv, fdo[ct][kk], kk == 0 ? nd[ct] : dp[ct][j]);
-                            }
-                        }
-                    if (edge) {
+                for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j) {
-                            const int f = kp * Ti::RPS + j;
-                            const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const int f = kp * Ti::RPS + j;
+                        const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                                for (int ct = 0; ct < QT; ++ct)
-                                    s[ct][j][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][j][r] : -INFINITY;
+                        for (int ct = 0; ct < QT; ++ct) {
+                            const f32x4 start = z[j - ct + QT - 1];
+                            s[ct][j] = Ti::mma(fk, fq[ct][kk], kk == 0 ? start : s[ct][j]);
+                            dp[ct][j] = Ti::mma(fv, fdo[ct][kk], kk == 0 ? nd[ct] : dp[ct][j]);
                         }
                     }
-                    typename Ti::frag fds[QT];
+                if (edge) {
 #pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) {
-                        float sum = 0.f;
+                    for (int j = 0; j < Ti::RPS; ++j) {
+                        const int f = kp * Ti::RPS + j;
+                        const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
 #pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j)
+                        for (int r = 0; r < 4; ++r)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                dp[ct][j][r] *= __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, al[ct]));
-                                if (MEND) sum += dp[ct][j][r];
-                            }
-                        rsum[ct] += sum;
-                        fds[ct] = Ti::pf(dp[ct]);
+                            for (int ct = 0; ct < QT; ++ct)
+                                s[ct][j][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][j][r] : -INFINITY;
                     }
-                    if (pass == 0) continue;
+                }
+                typename Ti::frag fds[QT];
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            dp[ct][j][r] *= __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, al[ct]));
+                            if (MEND) sum += dp[ct][j][r];
+                        }
+                    rsum[ct] += sum;
+                    fds[ct] = Ti::pf(dp[ct]);
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
+                }
+                if constexpr (FINE) {                       // what the rounding of ds left behind, as a second part
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) { Ti::less(dp[ct], fds[ct]); fds[ct] = Ti::pf(dp[ct]); }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
                         const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
@@ -213,31 +230,29 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                         for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
                     }
                 }
-            };
-            while (c < c_end) {
-                if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
-                rp_landed();                                // this chunk is there, nobody reads the buffer of the one before it any more
-                const char* tK = smem + buf * 2 * Ti::BYTES;
-                const int rel0 = c * 64 - (qw + sq.off);
-                const uint64_t now = bits;
-                c = keys.seek(c + 1, c_end, bits);
-                buf ^= NB - 1;
-                if (NB == 2 && c < c_end) fetch(c, buf, bits);
-                if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
-                const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
-                chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
             }
-            if (!MEND) break;
+        };
+        while (c < c_end) {
+            if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
+            rp_landed();                                // this chunk is there, nobody reads the buffer of the one before it any more
+            const char* tK = smem + buf * 2 * Ti::BYTES;
+            const int rel0 = c * 64 - (qw + sq.off);
+            const uint64_t now = bits;
+            c = keys.seek(c + 1, c_end, bits);
+            buf ^= NB - 1;
+            if (NB == 2 && c < c_end) fetch(c, buf, bits);
+            if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
+            const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+            chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
+        }
+        if (MEND)
 #pragma unroll
             for (int ct = 0; ct < QT; ++ct) {
                 float rho = rsum[ct];
                 rho += __shfl_xor(rho, 16, 64);
                 rho += __shfl_xor(rho, 32, 64);
-                const float x = nd[ct][0] - rho;
-                nd[ct] = (f32x4){x, x, x, x};
-                rsum[ct] = 0.f;
+                nd[ct][0] -= rho;
             }
-        }
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
@@ -248,6 +263,15 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             for (int d = 0; d < DT; ++d)
                 if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, dq[ct][d] * a.scale);
         }
+    };
+    for (; rb * BQ_ < sq.qn; rb += a.nrb) {
+        constexpr int FQ = DT <= 4 ? QT_ : 1;               // (D > 64: 16 columns a wave, the second part needs the registers)
+        if constexpr (MIXED)
+            if (rp_fine(a, sq, rb * BQ_)) {
+                for (int q0 = rb * BQ_; q0 < min((rb + 1) * BQ_, sq.qn); q0 += 64 * FQ) block(std::integral_constant<int, FQ>(), std::true_type(), q0);
+                continue;
+            }
+        block(std::integral_constant<int, QT_>(), std::false_type(), rb * BQ_);
     }
 }
 
@@ -601,6 +625,13 @@ int amdseg_relpos_sums_impl(const float* part, float* sums, int64_t wgs, const i
     return amdseg_launch_status();
 }
 
+template <typename T, int DT, int QT, bool MIXED>
+static int rp_dq_one(const RpArgs& a, int64_t n, int lds, hipStream_t s) {
+    const int rc = rp_allow_lds((const void*)rp_dq_kernel<T, DT, QT, MIXED>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((rp_dq_kernel<T, DT, QT, MIXED>), dim3((unsigned)n), dim3(256), lds, s, a);
+    return 0;
+}
 template <typename T, int DT>
 static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStream_t s) {
     const int ND = 2 * (a.span + RP_PAD) + 1;
@@ -611,14 +642,15 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
     if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
-    int rc;
-    if (n == 0) {
-    } else if (sizeof(T) == 4 || qt == 1) {
-        if ((rc = rp_allow_lds((const void*)rp_dq_kernel<T, DT, 1>, lds))) return rc;
-        hipLaunchKernelGGL((rp_dq_kernel<T, DT, 1>), dim3((unsigned)n), dim3(256), lds, s, a);
-    } else if constexpr (sizeof(T) == 2) {
-        if ((rc = rp_allow_lds((const void*)rp_dq_kernel<T, DT, 2>, lds))) return rc;
-        hipLaunchKernelGGL((rp_dq_kernel<T, DT, 2>), dim3((unsigned)n), dim3(256), lds, s, a);
+    int rc = 0;
+    if (n > 0) {
+        if (sizeof(T) == 4) rc = rp_dq_one<T, DT, 1, false>(a, n, lds, s);
+        else if constexpr (sizeof(T) == 2) {                // can any row block be FINE?  Packed and ragged lengths are on the device
+            const bool mixed = a.causal || a.cu_q || a.k_lens || a.Lk <= RP_FINE || a.Lq <= RP_FINE / 2;
+            if (mixed) rc = qt == 1 ? rp_dq_one<T, DT, 1, true>(a, n, lds, s) : rp_dq_one<T, DT, 2, true>(a, n, lds, s);
+            else rc = qt == 1 ? rp_dq_one<T, DT, 1, false>(a, n, lds, s) : rp_dq_one<T, DT, 2, false>(a, n, lds, s);
+        }
+        if (rc) return rc;
     }
     if ((rc = amdseg_launch_status())) return rc;
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
