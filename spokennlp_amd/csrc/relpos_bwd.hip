@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         return;
     }
     int rb, h, b;
-    rp_place(blockIdx.x, a.nrb, a.B, a.heads, a.kv_heads, rb, h, b);
+    rp_place(blockIdx.x, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ_ = 64 * QT_;
     constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums, and so is ds)
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
         return;
     }
     int rb, hk, b;
-    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads, a.kv_heads, rb, hk, b);
+    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads, a.kv_heads, false, rb, hk, b);
     const RpSeq sq = rp_seq(a, b);
     constexpr int BK = 64 * QT;
     const int G = a.heads / a.kv_heads;

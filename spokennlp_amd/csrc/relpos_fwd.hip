@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     }
     id -= split * nmain;
     int rb, h, b;
-    rp_place(id, a.nrb, a.B, a.heads, a.kv_heads, rb, h, b);
+    rp_place(id, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
     if (rb * BQ >= sq.qn) return;
