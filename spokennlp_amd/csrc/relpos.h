@@ -35,6 +35,8 @@ struct RpArgs {
     int nsplit, split_keys;     // forward: splits over the keys, keys of one (a multiple of 64)
     float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
     float* stat;                // backward: what the dK / dV kernel needs of a row: -lse in the exponent's units [rows], -sum_j p_ij dp_ij [rows]
+    int parts;                  // backward: workgroups that share a kv head's query heads in the dK / dV kernel
+    float* part_kv;             // backward, parts > 1: [dk, dv][parts][rows of k][kv_heads][D]
     float* part_d;              // backward: [heads][B * nrb][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
 };
 

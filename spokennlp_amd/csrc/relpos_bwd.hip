@@ -285,22 +285,22 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     float* tab = rows + NB * 128;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int nmain = a.B * a.kv_heads * a.nrb;
+    const int parts = a.parts, nmain = a.B * a.kv_heads * parts * a.nrb;
     if ((int)blockIdx.x >= nmain) {
         const int lead = rp_clamp(a.cu_k[0], 0, a.Tk), end = rp_clamp(a.cu_k[a.B], lead, a.Tk);
         rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
         rp_zero_rows((T*)a.dv, a.sdv, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
         return;
     }
-    int rb, hk, b;
-    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads, a.kv_heads, false, rb, hk, b);
+    int rb, hp, b;
+    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads * parts, a.kv_heads, false, rb, hp, b);
+    const int hk = hp / parts, G = a.heads / a.kv_heads / parts, h0 = hp * G;       // this workgroup's query heads: h0 .. h0 + G - 1
     const RpSeq sq = rp_seq(a, b);
     constexpr int BK = 64 * QT;
-    const int G = a.heads / a.kv_heads;
     const float c2 = a.scale * RP_LOG2E;
     const bool causal = a.causal;
     const int rows_k = a.cu_k ? sq.kn : a.Lk;               // padded: rows past k_lens are gradients of zero, and written
-    float* part = a.part_d ? a.part_d + ((int64_t)hk * G * a.B * a.nrb + (int64_t)b * a.nrb + rb) * ND : nullptr;     // of the group's first head
+    float* part = a.part_d ? a.part_d + ((int64_t)h0 * a.B * a.nrb + (int64_t)b * a.nrb + rb) * ND : nullptr;     // of the first head
     const int64_t part_h = (int64_t)a.B * a.nrb * ND;
     if (part && rb * BK >= rows_k)
         for (int gi = 0; gi < G; ++gi)
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             }
         };
         auto head = [&](int gi) {                           // a head's first chunk, on its way before anything else is waited for
-            const int h = hk * G + gi;
+            const int h = h0 + gi;
             qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
             ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
             stat_h = a.stat + rp_row(a, sq, b, h, 0);
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
         for (int gi = 0; gi < G; ++gi) {
             if (gi) { __syncthreads(); head(gi); }          // (nobody is left in the buffers, the table, the bins)
-            table.finish(a, tab, hk * G + gi);
+            table.finish(a, tab, h0 + gi);
             if (part)
                 for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
             int buf = 0;
@@ -535,17 +535,45 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
         for (int ct = 0; ct < QT; ++ct) {
             const int key = kw + ct * 16 + i16;
             if (key >= rows_k) continue;
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            if (parts > 1) {
+                const int64_t rows_all = (int64_t)a.B * a.Lk, row = (int64_t)b * a.Lk + key;
+                float* kp_ = a.part_kv + (((hp - hk * parts) * rows_all + row) * a.kv_heads + hk) * a.D;
+                float* vp_ = kp_ + parts * rows_all * a.kv_heads * a.D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (d * 16 + g * 4 < a.D) {
+                        *reinterpret_cast<f32x4*>(kp_ + d * 16 + g * 4) = seen[ct] ? dk[ct][d] * a.scale : z;
+                        *reinterpret_cast<f32x4*>(vp_ + d * 16 + g * 4) = seen[ct] ? dv[ct][d] : z;
+                    }
+                continue;
+            }
             T* kp_ = (T*)a.dk + b * a.sdk.sb + (int64_t)(sq.k0 + key) * a.sdk.st + hk * a.sdk.sh;
             T* vp_ = (T*)a.dv + b * a.sdv.sb + (int64_t)(sq.k0 + key) * a.sdv.st + hk * a.sdv.sh;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 if (d * 16 + g * 4 < a.D) {
-                    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
                     Ti::st4(kp_ + d * 16 + g * 4, seen[ct] ? dk[ct][d] * a.scale : z);
                     Ti::st4(vp_ + d * 16 + g * 4, seen[ct] ? dv[ct][d] : z);
                 }
         }
     }
+}
+
+// dk, dv = the sums of the `parts` workgroups of a kv head, in their order.  Bound by its bytes (4 parts of 3 x 1023 x 4 x 128: 50 MB read).
+template <typename T>
+__global__ __launch_bounds__(256) void rp_join_kv_kernel(RpArgs a) {
+    const int64_t one = (int64_t)a.B * a.Lk * a.kv_heads * a.D, x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (x >= one) return;
+    const int width = a.kv_heads * a.D, which = blockIdx.y;
+    const int64_t row = x / width;
+    const int hk = (int)(x % width) / a.D, d = (int)(x % width) % a.D;
+    const float* p = a.part_kv + which * a.parts * one + x;
+    f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    for (int i = 1; i < a.parts; ++i) s += *reinterpret_cast<const f32x4*>(p + i * one);
+    const RpTensor& st = which ? a.sdv : a.sdk;
+    const int64_t b = row / a.Lk, r = row % a.Lk;
+    RpTile<T, 2>::st4((T*)(which ? a.dv : a.dk) + b * st.sb + r * st.st + hk * st.sh + d, s);
 }
 
 // dtable from the workgroups' sums, in a fixed order: one workgroup per (bucket, head) lists the places of rel that belong to its bucket, then adds those of
@@ -654,7 +682,8 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     }
     if ((rc = amdseg_launch_status())) return rc;
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
-    const int64_t m = (int64_t)a.B * a.kv_heads * a.nrb + tail;
+    a.parts = rp_dkv_parts(a, kt);
+    const int64_t m = (int64_t)a.B * a.kv_heads * a.parts * a.nrb + tail;
     if (m > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
@@ -665,7 +694,13 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
         if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 2>, lds2))) return rc;
         hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 2>), dim3((unsigned)m), dim3(256), lds2, s, a);
     }
-    if ((rc = amdseg_launch_status()) || !a.part_d) return rc;
+    if ((rc = amdseg_launch_status())) return rc;
+    if (a.parts > 1) {
+        const int64_t vecs = (int64_t)a.B * a.Lk * a.kv_heads * (a.D / 4);          // (< 512 workgroups of 64 kt keys: below 2^24)
+        hipLaunchKernelGGL(rp_join_kv_kernel<T>, dim3((unsigned)((vecs + 255) / 256), 2), dim3(256), 0, s, a);
+        if ((rc = amdseg_launch_status())) return rc;
+    }
+    if (!a.part_d) return 0;
     return amdseg_relpos_sums_impl(a.part_d, sums, (int64_t)a.B * a.nrb, a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
 }
 template <typename T>

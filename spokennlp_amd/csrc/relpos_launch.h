@@ -18,15 +18,28 @@ static inline int rp_allow_lds(const void* kernel, int bytes) {
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return e == hipSuccess ? 0 : (int)e;
 }
-// 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products; 32 x 512 forward 54 us against 64, dK / dV 108 against 146) unless that
-// leaves CUs without a workgroup, and in fp32 (registers).  D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a
+// 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products; 32 x 512 forward 54 us against 64, dK / dV 108 against 146) unless one
+// gives the CUs a second workgroup that they would not have: grids of up to 256 (2048 rows of 16 heads: dK / dV 73 us against 77), forward and dQ at D <= 64 up
+// to 384 (2 x 2048 rows of 12 heads: forward 59 against 66, dQ 64 against 71; dK / dV 122 against 98; at 432 two win: 22 against 22.5, 27 against 31).  fp32: one (registers).  D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a
 // SIMD (16 x 512: 113 us against 104 with one tile), and a forward grid of three rounds or more runs better on three waves a SIMD of one tile (4 x 2048:
 // 177 against 165).
-static inline int rp_qt(int64_t wgs_of_two, int dtype) { return dtype == 1 ? 1 : wgs_of_two < 256 ? 1 : 2; }
+static inline int rp_qt(int64_t wgs_of_two, int most_of_one, int dtype) { return dtype == 1 ? 1 : wgs_of_two <= most_of_one ? 1 : 2; }
 static inline int64_t rp_wgs_of_two(const RpArgs& a) { return (int64_t)((a.Lq + 127) / 128) * a.B * a.heads; }
-static inline int rp_dq_qt(const RpArgs& a, int dtype) { return rp_qt(rp_wgs_of_two(a), dtype); }
+static inline int rp_dq_qt(const RpArgs& a, int dtype) { return rp_qt(rp_wgs_of_two(a), a.D > 64 ? 256 : 384, dtype); }
 static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return a.D > 64 && rp_wgs_of_two(a) >= 768 ? 1 : rp_dq_qt(a, dtype); }
-static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, dtype); }
+static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, 256, dtype); }
+// dK / dV of shared kv heads: a workgroup walks the rows of all G query heads; where that leaves less than two workgroups a CU, `parts` of them take G / parts
+// heads each and rp_join_kv_kernel adds their fp32 sums (a walk of less than RP_PART_STEPS chunks is not worth its launch).  Not for packed sequences: `longest` is
+// a hint there and must not change bits.
+#define RP_PART_STEPS 16
+static inline int rp_dkv_parts(const RpArgs& a, int kt) {
+    const int G = a.heads / a.kv_heads;
+    const int64_t n = (int64_t)((a.Lk + 64 * kt - 1) / (64 * kt)) * a.B * a.kv_heads;
+    if (G == 1 || n == 0 || a.cu_q || (int64_t)((a.Lq + 63) / 64) * G < RP_PART_STEPS) return 1;
+    int p = 1;
+    while (p < G && (G % p || n * p < 512)) ++p;
+    return p;
+}
 // the rows of a kv head's query heads fit the 16 columns of one tile
 static inline bool rp_few(const RpArgs& a) {
     return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;

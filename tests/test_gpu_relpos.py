@@ -247,6 +247,33 @@ def test_packed(dev, dtype, causal):
         assert bool((x[end:] == 7.0).all()) and not bool((x[:end] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1030, 1030, 2, 1, 64), (2, 515, 190, 6, 2, 64), (2, 300, 333, 15, 3, 40), (3, 513, 513, 16, 4, 128), (1, 200, 70, 6, 1, 96)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_long_walks_of_shared_heads_in_parts(dev, dtype, shape, ragged):
+    """dk and dv of a kv head with many query heads and rows, where few workgroups hold keys: the heads are dealt over several workgroups"""
+    print("CASE", dtype, shape, ragged, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, table, lut, dout = make(dev, dtype, *shape)
+    lens = torch.tensor([Lk - 61 * (b + 1) if b < 2 else 0 for b in range(B)], dtype=torch.int32, device=dev) if ragged else None
+    mask = None
+    if ragged:
+        mask = torch.rand(B, Lk, generator=torch.Generator().manual_seed(4)).to(dev) < 0.7
+        k, v = (torch.where((mask & (torch.arange(Lk, device=dev) < lens[:, None]))[..., None, None], x, math.nan) for x in (k, v))
+        want_k = torch.nan_to_num(k)                         # (the oracle sees zeros in hidden rows, the kernels NaN)
+        out, lse = _ops().relpos_attn_fwd(q, k, v, table, lut, key_mask=mask, k_lens=lens)
+        got = _ops().relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, key_mask=mask, k_lens=lens)
+        a = check(dev, q, want_k, torch.nan_to_num(v), table, lut, dout, key_mask=mask, k_lens=lens)
+        for x, y in zip((out, lse) + got, a):
+            assert torch.equal(x, y)
+        return
+    a = check(dev, q, k, v, table, lut, dout, causal=Lq == Lk)
+    dk = torch.full((B, Hk, Lk, D + 8), 7.0, dtype=dtype, device=dev)[..., :D].permute(0, 2, 1, 3)
+    dv = torch.full((B, Lk, Hk, 2, D), 7.0, dtype=dtype, device=dev)
+    _ops().relpos_attn_bwd(q, k, v, table, lut, a[0], dout, a[1], causal=Lq == Lk, dq=torch.empty_like(q), dk=dk, dv=dv[:, :, :, 1])
+    assert torch.equal(dk, a[3]) and torch.equal(dv[:, :, :, 1], a[4]) and bool((dv[:, :, :, 0] == 7).all())
+
+
 def test_packed_rows_in_front(dev):
     """offsets that do not start at 0: the rows in front belong to no sequence either"""
     ops = _ops()
