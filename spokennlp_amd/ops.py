@@ -556,15 +556,16 @@ def _rp_table(c, table, bucket_map, heads):
     c.span, c.table_dtype, c.buckets = n // 2, _dt(table), table.shape[0]
 
 
-def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end):
+def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, more_key, more):
     """-> (RelposCfg, shape of lse, workspace bytes forward, backward).  What follows from shapes, strides, types and options alone is worked out once per
-    such combination and copied (a call on a few rows is otherwise longer on the host than on the GPU); pointers and devices are looked at every time."""
-    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, table.shape, table.dtype, bucket_map.shape, scale, max_q, max_k,
-           bool(causal), bool(align_end), cu_q is None or cu_q.shape, cu_k is None or cu_k.shape, k_lens is None,
-           None if key_mask is None else (key_mask.shape, key_mask.stride(), key_mask.dtype))
+    such combination and copied (a call on a few rows is otherwise longer on the host than on the GPU); pointers and devices are looked at every time.
+    `more(c, shape of lse)` fills in the other tensors' strides, `more_key` is all that it looks at."""
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, table.shape, table.stride(), table.dtype, bucket_map.shape,
+           bucket_map.stride(), bucket_map.dtype, scale, max_q, max_k, bool(causal), bool(align_end), cu_q is None or cu_q.shape, cu_k is None or cu_k.shape,
+           k_lens is None, None if key_mask is None else (key_mask.shape, key_mask.stride(), key_mask.dtype), more_key)
     known = _rp_known.get(key)
     if known is None:
-        known = _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
+        known = _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, more)
         if len(_rp_known) >= 256:
             _rp_known.clear()
         _rp_known[key] = known
@@ -572,12 +573,11 @@ def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max
     dev = q.device
     if dev.type != "cuda" or k.device != dev or v.device != dev:
         raise ValueError("q, k, v must be on one GPU")
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        if t.data_ptr() & 15:
-            raise ValueError(f"{n}: rows must start on 16 bytes")
-    if table.device != dev or bucket_map.device != dev or not table.is_contiguous():
-        raise ValueError(f"table (contiguous) and bucket_map must be on {dev}")
-    c.table, c.map = table.data_ptr(), _rp_int(bucket_map, "bucket_map", bucket_map.numel(), dev)
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        raise ValueError("q, k, v: rows must start on 16 bytes")
+    if table.device != dev or bucket_map.device != dev:
+        raise ValueError(f"table and bucket_map must be on {dev}")
+    c.table, c.map = table.data_ptr(), bucket_map.data_ptr()
     if cu_q is not None:
         c.cu_q, c.cu_k = _rp_int(cu_q, "cu_q", c.B + 1, dev), _rp_int(cu_k, "cu_k", c.B + 1, dev)
     if k_lens is not None:
@@ -592,7 +592,7 @@ def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max
 _rp_known = {}
 
 
-def _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end):
+def _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, more):
     """the checks and the part of RelposCfg that depend on no pointer"""
     packed = cu_q is not None
     if packed != (cu_k is not None):
@@ -638,24 +638,27 @@ def _rp_plan(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, ma
             raise ValueError("key_mask: the last dimension must be contiguous")
         c.mask_stride = 0 if packed or key_mask.shape[0] == 1 else key_mask.stride(0)
     _rp_table(c, table, bucket_map, heads)
+    _rp_int(bucket_map, "bucket_map", 2 * c.span + 1, bucket_map.device)
     c.scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-6 < c.scale < 1e6:
         raise ValueError(f"scale = {scale}: a positive number")
     c.causal, c.align_end = int(bool(causal)), int(bool(align_end))
+    lse_shape = (heads, c.Tq) if packed else (c.B, heads, c.Lq)
+    more(c, lse_shape)
     # the library sizes its workspaces from shapes; the two pointers it asks for (and whether there is a mask or offsets at all) stand in
     probe = L.RelposCfg.from_buffer_copy(c)
     probe.map = probe.table = 256
     if packed:
         probe.cu_q = probe.cu_k = 256
     lib = L.load()
-    return (bytes(c), (heads, c.Tq) if packed else (c.B, heads, c.Lq), lib.amdseg_relpos_attn_ws_bytes(C.byref(probe), 0),
+    return (bytes(c), lse_shape, lib.amdseg_relpos_attn_ws_bytes(C.byref(probe), 0),
             lib.amdseg_relpos_attn_ws_bytes(C.byref(probe), 1))
 
 
 def _rp_out(t, like, name, es):
-    """a caller's output tensor: shape, dtype, device, and no two elements in one place"""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
+    """a caller's output tensor: shape, dtype, and no two elements in one place"""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype}")
     at = 1
     for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if s < at:
@@ -670,22 +673,14 @@ def _rp_dense(shape):
     return (st[0] * shape[1] if len(shape) == 4 else 0, *st)
 
 
-class _rp_on:
-    """the GPU of a call's tensors as the current one (nothing to do where it is), and its current stream's handle"""
+def _rp_here(dev):
+    """is a call's GPU the current one?  (If not, the call enters again under torch.cuda.device.)"""
+    return torch._C._cuda_getDevice() == dev.index
 
-    def __init__(self, dev):
-        self.dev = dev
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _rp_s(dev):
+    """handle of the current stream of a GPU, without the Stream object (1 us less per call)"""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None, causal=False,
@@ -698,17 +693,24 @@ def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_len
     Query i stands at position i, or (align_end) so that the last query stands at the last key.  A row that sees no key: zero, lse -inf.
     Returns (out, lse); lse fp32 [B, heads, Lq] / [heads, tokens], None unless need_lse.  `out`: rows outside every packed sequence are left as they were
     (a fresh tensor has zeros there)."""
-    c, lse_shape, ws_bytes, _ = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
-    with _rp_on(q.device) as stream:
-        if out is None:
-            out = q.new_empty(q.shape)
-            c.zero_tail = 1
-            c.out_stride[:] = _rp_dense(q.shape)
-        else:
-            c.out_stride[:] = _rp_out(out, q, "out", q.element_size())
-        lse = table.new_empty(lse_shape, dtype=torch.float32) if need_lse else None
-        ws = table.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-        L.check(L.load().amdseg_relpos_attn_fwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(ws), ws_bytes, stream), "amdseg_relpos_attn_fwd")
+    def more(c, _):
+        c.zero_tail = int(out is None)
+        c.out_stride[:] = _rp_dense(q.shape) if out is None else _rp_out(out, q, "out", q.element_size())
+
+    c, lse_shape, ws_bytes, _ = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end,
+                                        None if out is None else (out.shape, out.stride(), out.dtype), more)
+    dev = q.device
+    if not _rp_here(dev):
+        with torch.cuda.device(dev):
+            return relpos_attn_fwd(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, need_lse, out)
+    if out is None:
+        out = q.new_empty(q.shape)
+    elif out.device != dev or out.data_ptr() & 15:
+        raise ValueError(f"out must be on {dev}, its rows on 16 bytes")
+    lse = table.new_empty(lse_shape, dtype=torch.float32) if need_lse else None
+    ws = table.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    L.check(L.load().amdseg_relpos_attn_fwd(C.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _p(lse), _p(ws), ws_bytes, _rp_s(dev)),
+            "amdseg_relpos_attn_fwd")
     return out, lse
 
 
@@ -717,30 +719,40 @@ def relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale=None, key_
     """gradients of relpos_attn_fwd from its `out` and `lse` (amdseg_relpos_attn_bwd): (dq, dk, dv, dtable), the last in the table's dtype or None.
     dq / dk / dv may be given (column blocks of one buffer): rows outside every packed sequence are left as they were in all three or, if none is given,
     zero.  Sums are taken in a fixed order: the same call gives the same bits."""
-    c, lse_shape, _, ws_bytes = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end)
-    dev, es = q.device, q.element_size()
     if (dq is None) != (dk is None) or (dq is None) != (dv is None):
         raise ValueError("dq, dk, dv: give all three or none")
-    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype or out.device != dev or dout.device != dev:
-        raise ValueError(f"out and dout must be {tuple(q.shape)} {q.dtype} on {dev}")
-    if lse.shape != lse_shape or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
-        raise ValueError(f"lse must be the contiguous fp32 {lse_shape} of relpos_attn_fwd")
-    with _rp_on(dev) as stream:
+
+    def more(c, lse_shape):
+        es = q.element_size()
+        if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype:
+            raise ValueError(f"out and dout must be {tuple(q.shape)} {q.dtype}")
+        if lse.shape != lse_shape or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise ValueError(f"lse must be the contiguous fp32 {lse_shape} of relpos_attn_fwd")
         c.out_stride[:] = _rp_strides(out, "out", es)
         c.dout_stride[:] = _rp_strides(dout, "dout", es)
-        if dq is None:
-            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-            c.zero_tail = 1
-            c.dq_stride[:] = _rp_dense(q.shape)
-            c.dk_stride[:] = c.dv_stride[:] = _rp_dense(k.shape)
-        else:
-            c.dq_stride[:] = _rp_out(dq, q, "dq", es)
-            c.dk_stride[:] = _rp_out(dk, k, "dk", es)
-            c.dv_stride[:] = _rp_out(dv, v, "dv", es)
-        dtable = torch.empty_like(table) if need_dtable else None
-        ws = table.new_empty(ws_bytes, dtype=torch.uint8)
-        L.check(L.load().amdseg_relpos_attn_bwd(C.byref(c), _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(dtable), _p(ws),
-                                                ws_bytes, stream), "amdseg_relpos_attn_bwd")
+        c.zero_tail = int(dq is None)
+        for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            getattr(c, name + "_stride")[:] = _rp_dense(like.shape) if t is None else _rp_out(t, like, name, es)
+
+    c, lse_shape, _, ws_bytes = _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end,
+                                        (out.shape, out.stride(), out.dtype, dout.shape, dout.stride(), dout.dtype, lse.shape, lse.stride(), lse.dtype,
+                                         dq is None or (dq.shape, dq.stride(), dq.dtype, dk.shape, dk.stride(), dk.dtype, dv.shape, dv.stride(), dv.dtype)), more)
+    dev = q.device
+    if not _rp_here(dev):
+        with torch.cuda.device(dev):
+            return relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, need_dtable,
+                                   dq, dk, dv)
+    if dq is None:
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    if out.device != dev or dout.device != dev or lse.device != dev or dq.device != dev or dk.device != dev or dv.device != dev:
+        raise ValueError(f"out, dout, lse (and dq, dk, dv) must be on {dev}")
+    at = out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    if (at[0] | at[1] | at[3] | at[4] | at[5]) & 15:
+        raise ValueError("out, dout (and dq, dk, dv): rows must start on 16 bytes")
+    dtable = table.new_empty(table.shape) if need_dtable else None
+    ws = table.new_empty(ws_bytes, dtype=torch.uint8)
+    L.check(L.load().amdseg_relpos_attn_bwd(C.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), *at, _p(dtable), ws.data_ptr(), ws_bytes, _rp_s(dev)),
+            "amdseg_relpos_attn_bwd")
     return dq, dk, dv, dtable
 
 
@@ -750,14 +762,16 @@ def relpos_bias_fwd(table, bucket_map, Lq, Lk, q_offset=0, out_dtype=torch.float
     if table.dim() != 2 or Lq < 0 or Lk < 0:
         raise ValueError(f"table [buckets, heads], Lq and Lk >= 0, not {tuple(table.shape)}, {Lq}, {Lk}")
     c, dev, heads = L.RelposCfg(), table.device, table.shape[1]
+    if dev.type == "cuda" and not _rp_here(dev):
+        with torch.cuda.device(dev):
+            return relpos_bias_fwd(table, bucket_map, Lq, Lk, q_offset, out_dtype)
     if dev.type != "cuda":
         raise ValueError("table must be on a GPU")
     _rp_table(c, table, bucket_map, heads)
     m = _rp_int(bucket_map, "bucket_map", bucket_map.numel(), dev)
-    with _rp_on(dev) as stream:
-        out = table.new_empty((heads, Lq, Lk), dtype=out_dtype)
-        L.check(L.load().amdseg_relpos_bias_fwd(_p(table), c.table_dtype, m, c.span, c.buckets, heads, Lq, Lk, q_offset, _p(out), _dt(out), stream),
-                "amdseg_relpos_bias_fwd")
+    out = table.new_empty((heads, Lq, Lk), dtype=out_dtype)
+    L.check(L.load().amdseg_relpos_bias_fwd(_p(table), c.table_dtype, m, c.span, c.buckets, heads, Lq, Lk, q_offset, _p(out), _dt(out), _rp_s(dev)),
+            "amdseg_relpos_bias_fwd")
     return out
 
 
@@ -776,11 +790,13 @@ def relpos_bias_bwd(dbias, bucket_map, buckets, q_offset=0):
     if dbias.data_ptr() & 15:
         raise ValueError("dbias must start on 16 bytes")
     m = _rp_int(bucket_map, "bucket_map", n, dev)
-    with _rp_on(dev) as stream:
-        dtable = dbias.new_empty((buckets, heads), dtype=torch.float32)
-        lib = L.load()
-        ws_bytes = lib.amdseg_relpos_bias_ws_bytes(B, heads, Lq, n // 2)
-        ws = dbias.new_empty(ws_bytes, dtype=torch.uint8)
-        L.check(lib.amdseg_relpos_bias_bwd(_p(dbias), _dt(dbias), m, n // 2, buckets, B, heads, Lq, Lk, q_offset, _p(dtable), _p(ws), ws_bytes, stream),
-                "amdseg_relpos_bias_bwd")
+    if not _rp_here(dev):
+        with torch.cuda.device(dev):
+            return relpos_bias_bwd(dbias, bucket_map, buckets, q_offset)
+    dtable = dbias.new_empty((buckets, heads), dtype=torch.float32)
+    lib = L.load()
+    ws_bytes = lib.amdseg_relpos_bias_ws_bytes(B, heads, Lq, n // 2)
+    ws = dbias.new_empty(ws_bytes, dtype=torch.uint8)
+    L.check(lib.amdseg_relpos_bias_bwd(_p(dbias), _dt(dbias), m, n // 2, buckets, B, heads, Lq, Lk, q_offset, _p(dtable), _p(ws), ws_bytes, _rp_s(dev)),
+            "amdseg_relpos_bias_bwd")
     return dtable
