@@ -673,6 +673,10 @@ def _rp_dense(shape):
     return (st[0] * shape[1] if len(shape) == 4 else 0, *st)
 
 
+def _rp_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rp_here(dev):
     """is a call's GPU the current one?  (If not, the call enters again under torch.cuda.device.)"""
     return torch._C._cuda_getDevice() == dev.index
@@ -704,7 +708,7 @@ def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_len
         with torch.cuda.device(dev):
             return relpos_attn_fwd(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, need_lse, out)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = _rp_like(q)
     elif out.device != dev or out.data_ptr() & 15:
         raise ValueError(f"out must be on {dev}, its rows on 16 bytes")
     lse = table.new_empty(lse_shape, dtype=torch.float32) if need_lse else None
@@ -743,13 +747,13 @@ def relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale=None, key_
             return relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, scale, key_mask, k_lens, cu_q, cu_k, max_q, max_k, causal, align_end, need_dtable,
                                    dq, dk, dv)
     if dq is None:
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        dq, dk, dv = _rp_like(q), _rp_like(k), _rp_like(v)
     if out.device != dev or dout.device != dev or lse.device != dev or dq.device != dev or dk.device != dev or dv.device != dev:
         raise ValueError(f"out, dout, lse (and dq, dk, dv) must be on {dev}")
     at = out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     if (at[0] | at[1] | at[3] | at[4] | at[5]) & 15:
         raise ValueError("out, dout (and dq, dk, dv): rows must start on 16 bytes")
-    dtable = table.new_empty(table.shape) if need_dtable else None
+    dtable = _rp_like(table) if need_dtable else None
     ws = table.new_empty(ws_bytes, dtype=torch.uint8)
     L.check(L.load().amdseg_relpos_attn_bwd(C.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), *at, _p(dtable), ws.data_ptr(), ws_bytes, _rp_s(dev)),
             "amdseg_relpos_attn_bwd")
