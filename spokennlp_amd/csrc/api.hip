@@ -703,19 +703,20 @@ static int relpos_args(const struct amdseg_relpos_cfg* c, RpArgs& a) {
 }
 static size_t relpos_up(size_t n) { return (n + 255) / 256 * 256; }
 static size_t relpos_rows(const RpArgs& a) { return a.cu_q ? (size_t)a.heads * a.Tq : (size_t)a.B * a.heads * a.Lq; }
-static size_t relpos_bwd_ws(const RpArgs& a, int dtype, size_t* sums_at, size_t* part_at, size_t* kv_at) {
+static size_t relpos_bwd_ws(const RpArgs& a, int dtype, size_t* sums_at, size_t* part_at, size_t* kv_at, size_t* q_at) {
     const size_t nd = 2 * ((size_t)a.span + RP_PAD) + 1, bk = 64 * rp_dkv_qt(a, dtype), nrb = (a.Lk + bk - 1) / bk;
     *sums_at = relpos_up(8 * relpos_rows(a));
     *part_at = *sums_at + relpos_up(4 * nd * a.heads);
-    *kv_at = *part_at + relpos_up(4 * nd * a.heads * a.B * nrb);
-    const size_t parts = rp_dkv_parts(a, rp_dkv_qt(a, dtype)), rows_k = (size_t)a.B * a.Lk;
-    return *kv_at + (parts > 1 ? 8 * parts * rows_k * a.kv_heads * a.D : 0);
+    const size_t qs = rp_qsplit(a), parts = qs * rp_dkv_parts(a, rp_dkv_qt(a, dtype), (int)qs), ks = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
+    *kv_at = *part_at + relpos_up(4 * nd * a.heads * a.B * nrb * qs);
+    *q_at = *kv_at + (parts > 1 ? relpos_up(8 * parts * a.B * a.Lk * a.kv_heads * a.D) : 0);
+    return *q_at + (ks > 1 ? 4 * ks * relpos_rows(a) * (a.D + 1) : 0);
 }
 size_t amdseg_relpos_attn_ws_bytes(const struct amdseg_relpos_cfg* c, int backward) {
     RpArgs a;
     if (relpos_args(c, a)) return 0;
-    size_t x, y, z;
-    if (backward) return relpos_bwd_ws(a, c->dtype, &x, &y, &z);
+    size_t x, y, z, u;
+    if (backward) return relpos_bwd_ws(a, c->dtype, &x, &y, &z, &u);
     const size_t n = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
     return n > 1 ? n * relpos_rows(a) * (a.D + 2) * 4 : 0;
 }
@@ -747,12 +748,15 @@ int amdseg_relpos_attn_bwd(const struct amdseg_relpos_cfg* c, const void* q, con
     if (!relpos_rows_ok(q, c->q_stride, es, noq) || !relpos_rows_ok(k, c->k_stride, es, nok) || !relpos_rows_ok(v, c->v_stride, es, nok) ||
         !relpos_rows_ok(out, c->out_stride, es, noq) || !relpos_rows_ok(dout, c->dout_stride, es, noq) || !relpos_rows_ok(dq, c->dq_stride, es, noq) ||
         !relpos_rows_ok(dk, c->dk_stride, es, nok) || !relpos_rows_ok(dv, c->dv_stride, es, nok) || (!noq && !lse)) return AMDSEG_ERR_ARG;
-    size_t sums_at, part_at, kv_at;
-    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < relpos_bwd_ws(a, c->dtype, &sums_at, &part_at, &kv_at)) return AMDSEG_ERR_ARG;
+    size_t sums_at, part_at, kv_at, q_at;
+    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < relpos_bwd_ws(a, c->dtype, &sums_at, &part_at, &kv_at, &q_at)) return AMDSEG_ERR_ARG;
     a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.lse = (float*)lse; a.dq = dq; a.dk = dk; a.dv = dv;
     a.stat = (float*)ws;
     a.part_d = dtable ? (float*)((char*)ws + part_at) : nullptr;
     a.part_kv = (float*)((char*)ws + kv_at);
+    a.part_q = (float*)((char*)ws + q_at);
+    a.nsplit = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
+    a.split_keys = rp_split_keys(a.Lq);
     return amdseg_relpos_bwd_impl(a, c->dtype, dtable, (float*)((char*)ws + sums_at), S(stream));
 }
 static bool relpos_bias_ok(int dtype, const int32_t* map, int span, int buckets, int B, int heads, int Lq, int Lk, int q_offset) {

@@ -32,12 +32,13 @@ struct RpArgs {
     float scale;
     int nrb;                    // row blocks of a sequence (grid); a workgroup steps by it, so a wrong `longest` hint costs time, never rows
     int mask_words;             // 8-byte words of the key mask in LDS
-    int nsplit, split_keys;     // forward: splits over the keys, keys of one (a multiple of 64)
+    int nsplit, split_keys;     // forward and dQ: splits over the keys, keys of one (a multiple of 64)
     float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
     float* stat;                // backward: what the dK / dV kernel needs of a row: -lse in the exponent's units [rows], -sum_j p_ij dp_ij [rows]
-    int parts;                  // backward: workgroups that share a kv head's query heads in the dK / dV kernel
-    float* part_kv;             // backward, parts > 1: [dk, dv][parts][rows of k][kv_heads][D]
-    float* part_d;              // backward: [heads][B * nrb][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
+    float* part_q;              // backward, nsplit > 1: [nsplit][rows][D] sums of dq, then [nsplit][rows] sums of ds
+    int parts, qsplit;          // backward: workgroups that share a kv head's query heads, and its query rows, in the dK / dV kernel
+    float* part_kv;             // backward, parts * qsplit > 1: [dk, dv][parts * qsplit][rows of k][kv_heads][D]
+    float* part_d;              // backward: [heads][B * nrb * qsplit][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
 };
 
 // one sequence: where its rows start and how many there are.  The values of cu_q / cu_k / k_lens come from device memory that the host has not seen:

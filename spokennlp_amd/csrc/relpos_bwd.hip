@@ -80,13 +80,14 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.heads * a.nrb;
-    if ((int)blockIdx.x >= nmain) {
+    const int split = nmain ? blockIdx.x / nmain : a.nsplit;
+    if (split >= a.nsplit) {
         const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq);
-        rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain, RP_TAIL_WGS, tid);
+        rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain * a.nsplit, RP_TAIL_WGS, tid);
         return;
     }
     int rb, h, b;
-    rp_place(blockIdx.x, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
+    rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ_ = 64 * QT_;
     constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums, and so is ds)
@@ -119,6 +120,8 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
         }
+        int c_from = 0;
+        if (a.nsplit > 1) { c_from = split * (a.split_keys / 64); c_end = min(c_end, c_from + a.split_keys / 64); }
         typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
         float nl[QT], rsum[QT];                             // -lse in the exponent's units; sum of a row's ds (each of its four lanes: a quarter of the keys)
         f32x4 nd[QT];                                       // -delta, as what the product dout . v starts from
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
         };
         uint64_t bits;
-        int c = keys.seek(0, c_end, bits), buf = 0;
+        int c = keys.seek(c_from, c_end, bits), buf = 0;
         if (!first) __syncthreads();                    // (nobody is left in the buffers)
         if (NB == 2 && c < c_end) fetch(c, 0, bits);    // on its way before anything else is waited for
         typename Ti::frag fo[QT][Ti::KB];
@@ -251,13 +254,25 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                 float rho = rsum[ct];
                 rho += __shfl_xor(rho, 16, 64);
                 rho += __shfl_xor(rho, 32, 64);
-                nd[ct][0] -= rho;
+                rsum[ct] = rho;
             }
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
             if (q >= sq.qn) continue;
-            if (g == 0) { a.stat[rp_row(a, sq, b, h, q)] = nl[ct]; a.stat[rows + rp_row(a, sq, b, h, q)] = nd[ct][0]; }
+            const int64_t row = rp_row(a, sq, b, h, q);
+            if (a.nsplit > 1) {                             // rp_join_q_kernel adds them up
+                float* op = a.part_q + (split * rows + row) * a.D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(op + d * 16 + g * 4) = dq[ct][d] * a.scale;
+                if (g == 0) {
+                    a.part_q[a.nsplit * rows * a.D + split * rows + row] = rsum[ct];
+                    if (split == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = nd[ct][0]; }
+                }
+                continue;
+            }
+            if (g == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = nd[ct][0] - rsum[ct]; }
             T* op = (T*)a.dq + b * a.sdq.sb + (int64_t)(sq.q0 + q) * a.sdq.st + h * a.sdq.sh;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -285,23 +300,23 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     float* tab = rows + NB * 128;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int parts = a.parts, nmain = a.B * a.kv_heads * parts * a.nrb;
-    if ((int)blockIdx.x >= nmain) {
+    const int parts = a.parts, qsplit = a.qsplit, nmain = a.B * a.kv_heads * parts * a.nrb, split = nmain ? blockIdx.x / nmain : qsplit;
+    if (split >= qsplit) {
         const int lead = rp_clamp(a.cu_k[0], 0, a.Tk), end = rp_clamp(a.cu_k[a.B], lead, a.Tk);
-        rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
-        rp_zero_rows((T*)a.dv, a.sdv, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain, RP_TAIL_WGS, tid);
+        rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain * qsplit, RP_TAIL_WGS, tid);
+        rp_zero_rows((T*)a.dv, a.sdv, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain * qsplit, RP_TAIL_WGS, tid);
         return;
     }
     int rb, hp, b;
-    rp_place(blockIdx.x, a.nrb, a.B, a.kv_heads * parts, a.kv_heads, false, rb, hp, b);
+    rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.kv_heads * parts, a.kv_heads, false, rb, hp, b);
     const int hk = hp / parts, G = a.heads / a.kv_heads / parts, h0 = hp * G;       // this workgroup's query heads: h0 .. h0 + G - 1
     const RpSeq sq = rp_seq(a, b);
     constexpr int BK = 64 * QT;
     const float c2 = a.scale * RP_LOG2E;
     const bool causal = a.causal;
     const int rows_k = a.cu_k ? sq.kn : a.Lk;               // padded: rows past k_lens are gradients of zero, and written
-    float* part = a.part_d ? a.part_d + ((int64_t)h0 * a.B * a.nrb + (int64_t)b * a.nrb + rb) * ND : nullptr;     // of the first head
-    const int64_t part_h = (int64_t)a.B * a.nrb * ND;
+    float* part = a.part_d ? a.part_d + (((int64_t)h0 * a.B * a.nrb + (int64_t)b * a.nrb + rb) * qsplit + split) * ND : nullptr;     // of the first head
+    const int64_t part_h = (int64_t)a.B * a.nrb * qsplit * ND;
     if (part && rb * BK >= rows_k)
         for (int gi = 0; gi < G; ++gi)
             for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
@@ -323,6 +338,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
         const int k0 = rb * BK, kw = k0 + w * 16 * QT;
         int c_first = 0, n_ch = (sq.qn + 63) / 64;
         if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
+        if (qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
         const T *qb, *ob;
         const float* stat_h;
         auto fetch = [&](int c, int buf) {
@@ -536,10 +552,10 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             const int key = kw + ct * 16 + i16;
             if (key >= rows_k) continue;
             const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            if (parts > 1) {
+            if (parts * qsplit > 1) {
                 const int64_t rows_all = (int64_t)a.B * a.Lk, row = (int64_t)b * a.Lk + key;
-                float* kp_ = a.part_kv + (((hp - hk * parts) * rows_all + row) * a.kv_heads + hk) * a.D;
-                float* vp_ = kp_ + parts * rows_all * a.kv_heads * a.D;
+                float* kp_ = a.part_kv + ((((hp - hk * parts) * qsplit + split) * rows_all + row) * a.kv_heads + hk) * a.D;
+                float* vp_ = kp_ + parts * qsplit * rows_all * a.kv_heads * a.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
                     if (d * 16 + g * 4 < a.D) {
@@ -560,7 +576,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     }
 }
 
-// dk, dv = the sums of the `parts` workgroups of a kv head, in their order.  Bound by its bytes (4 parts of 3 x 1023 x 4 x 128: 50 MB read).
+// dk, dv = the sums of the parts * qsplit workgroups of a kv head, in their order.  Bound by its bytes (4 parts of 3 x 1023 x 4 x 128: 50 MB read).
 template <typename T>
 __global__ __launch_bounds__(256) void rp_join_kv_kernel(RpArgs a) {
     const int64_t one = (int64_t)a.B * a.Lk * a.kv_heads * a.D, x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -568,12 +584,30 @@ __global__ __launch_bounds__(256) void rp_join_kv_kernel(RpArgs a) {
     const int width = a.kv_heads * a.D, which = blockIdx.y;
     const int64_t row = x / width;
     const int hk = (int)(x % width) / a.D, d = (int)(x % width) % a.D;
-    const float* p = a.part_kv + which * a.parts * one + x;
+    const float* p = a.part_kv + which * a.parts * a.qsplit * one + x;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
-    for (int i = 1; i < a.parts; ++i) s += *reinterpret_cast<const f32x4*>(p + i * one);
+    for (int i = 1; i < a.parts * a.qsplit; ++i) s += *reinterpret_cast<const f32x4*>(p + i * one);
     const RpTensor& st = which ? a.sdv : a.sdk;
     const int64_t b = row / a.Lk, r = row % a.Lk;
     RpTile<T, 2>::st4((T*)(which ? a.dv : a.dk) + b * st.sb + r * st.st + hk * st.sh + d, s);
+}
+
+// dq and the mended delta of the splits over the keys, in their order (padded form)
+template <typename T>
+__global__ __launch_bounds__(256) void rp_join_q_kernel(RpArgs a) {
+    const int64_t rows = (int64_t)a.B * a.heads * a.Lq, x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (x >= rows * a.D) return;
+    const int64_t row = x / a.D;
+    const int d = (int)(x % a.D);
+    f32x4 s = *reinterpret_cast<const f32x4*>(a.part_q + x);
+    for (int i = 1; i < a.nsplit; ++i) s += *reinterpret_cast<const f32x4*>(a.part_q + i * rows * a.D + x);
+    const int64_t bh = row / a.Lq, q = row % a.Lq;
+    RpTile<T, 2>::st4((T*)a.dq + bh / a.heads * a.sdq.sb + q * a.sdq.st + bh % a.heads * a.sdq.sh + d, s);
+    if (d == 0 && sizeof(T) == 2) {
+        float rho = 0.f;
+        for (int i = 0; i < a.nsplit; ++i) rho += a.part_q[a.nsplit * rows * a.D + i * rows + row];
+        a.stat[rows + row] -= rho;
+    }
 }
 
 // dtable from the workgroups' sums, in a fixed order: one workgroup per (bucket, head) lists the places of rel that belong to its bucket, then adds those of
@@ -667,7 +701,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     a.mask_words = rp_mask_bytes(a) / 8;
     const int qt = rp_dq_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
     a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
-    const int64_t n = (int64_t)a.B * a.nrb * a.heads + tail;
+    const int64_t n = (int64_t)a.B * a.nrb * a.heads * a.nsplit + tail;
     if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
     int rc = 0;
@@ -682,8 +716,15 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     }
     if ((rc = amdseg_launch_status())) return rc;
     a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
-    a.parts = rp_dkv_parts(a, kt);
-    const int64_t m = (int64_t)a.B * a.kv_heads * a.parts * a.nrb + tail;
+    if (a.nsplit > 1 && n > 0) {
+        const int64_t vecs = (int64_t)a.B * a.heads * a.Lq * (a.D / 4);
+        if ((vecs + 255) / 256 > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
+        hipLaunchKernelGGL(rp_join_q_kernel<T>, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, a);
+        if ((rc = amdseg_launch_status())) return rc;
+    }
+    a.qsplit = rp_qsplit(a);
+    a.parts = rp_dkv_parts(a, kt, a.qsplit);
+    const int64_t m = (int64_t)a.B * a.kv_heads * a.parts * a.qsplit * a.nrb + tail;
     if (m > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
@@ -695,13 +736,14 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
         hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 2>), dim3((unsigned)m), dim3(256), lds2, s, a);
     }
     if ((rc = amdseg_launch_status())) return rc;
-    if (a.parts > 1) {
-        const int64_t vecs = (int64_t)a.B * a.Lk * a.kv_heads * (a.D / 4);          // (< 512 workgroups of 64 kt keys: below 2^24)
+    if (a.parts * a.qsplit > 1 && m > 0) {
+        const int64_t vecs = (int64_t)a.B * a.Lk * a.kv_heads * (a.D / 4);
+        if ((vecs + 255) / 256 > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
         hipLaunchKernelGGL(rp_join_kv_kernel<T>, dim3((unsigned)((vecs + 255) / 256), 2), dim3(256), 0, s, a);
         if ((rc = amdseg_launch_status())) return rc;
     }
     if (!a.part_d) return 0;
-    return amdseg_relpos_sums_impl(a.part_d, sums, (int64_t)a.B * a.nrb, a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
+    return amdseg_relpos_sums_impl(a.part_d, sums, (int64_t)a.B * a.nrb * a.qsplit, a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
 }
 template <typename T>
 static int rp_bwd_d(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {

@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     int id = blockIdx.x;
     const int nmain = a.B * a.heads * a.nrb;
-    const int split = id / nmain;
+    const int split = nmain ? id / nmain : a.nsplit;
     if (split >= a.nsplit) {                                // the buffer rows outside every sequence
         const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq), which = id - nmain * a.nsplit;
         rp_zero_rows((T*)a.out, a.so, a.heads, a.D, lead, end, a.Tq, which, RP_TAIL_WGS, tid);

@@ -32,14 +32,17 @@ static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : 
 // heads each and rp_join_kv_kernel adds their fp32 sums (a walk of less than RP_PART_STEPS chunks is not worth its launch).  Not for packed sequences: `longest` is
 // a hint there and must not change bits.
 #define RP_PART_STEPS 16
-static inline int rp_dkv_parts(const RpArgs& a, int kt) {
+static inline int rp_dkv_parts(const RpArgs& a, int kt, int qsplit) {
     const int G = a.heads / a.kv_heads;
-    const int64_t n = (int64_t)((a.Lk + 64 * kt - 1) / (64 * kt)) * a.B * a.kv_heads;
-    if (G == 1 || n == 0 || a.cu_q || (int64_t)((a.Lq + 63) / 64) * G < RP_PART_STEPS) return 1;
+    const int64_t n = (int64_t)((a.Lk + 64 * kt - 1) / (64 * kt)) * a.B * a.kv_heads * qsplit;
+    if (G == 1 || n == 0 || a.cu_q || (int64_t)((a.Lq + 63) / 64) * G / qsplit < RP_PART_STEPS) return 1;
     int p = 1;
     while (p < G && (G % p || n * p < 512)) ++p;
     return p;
 }
+// and its mirror for dK / dV: few keys against many query rows, whose walk is cut every RP_SPLIT_ROWS
+#define RP_SPLIT_ROWS 1024
+static inline int rp_qsplit(const RpArgs& a) { return !a.cu_q && a.Lk <= 128 && a.Lq > RP_SPLIT_ROWS ? (a.Lq + RP_SPLIT_ROWS - 1) / RP_SPLIT_ROWS : 1; }
 // the rows of a kv head's query heads fit the 16 columns of one tile
 static inline bool rp_few(const RpArgs& a) {
     return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;

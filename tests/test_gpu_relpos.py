@@ -274,6 +274,43 @@ def test_long_walks_of_shared_heads_in_parts(dev, dtype, shape, ragged):
     assert torch.equal(dk, a[3]) and torch.equal(dv[:, :, :, 1], a[4]) and bool((dv[:, :, :, 0] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(2, 86, 2100, 2, 2, 40), (1, 9, 1300, 8, 4, 64), (3, 128, 1025, 2, 1, 128), (2, 1100, 5, 2, 2, 64), (1, 2500, 128, 4, 2, 64),
+                                   (1, 3100, 127, 6, 1, 32), (2, 1025, 64, 2, 2, 96)])
+@pytest.mark.parametrize("how", ["plain", "causal", "ragged"])
+def test_backward_of_long_against_short(dev, dtype, shape, how):
+    """few query rows against many keys, few keys against many query rows: the long side's walk is cut into pieces whose sums are joined"""
+    print("CASE", dtype, shape, how, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, table, lut, dout = make(dev, dtype, *shape)
+    opt = {}
+    if how == "causal":
+        opt = dict(causal=True, align_end=Lq < Lk)
+    elif how == "ragged":
+        opt = dict(k_lens=torch.tensor([max(1, Lk // 3) if b else Lk for b in range(B)], dtype=torch.int32, device=dev),
+                   key_mask=torch.rand(B, Lk, generator=torch.Generator().manual_seed(4)).to(dev) < 0.7)
+    a = check(dev, q, k, v, table, lut, dout, **opt)
+    alone = [x[:1] if torch.is_tensor(x) else x for x in (q, k, v)]
+    one = {n: x[:1] if torch.is_tensor(x) else x for n, x in opt.items()}
+    got = _ops().relpos_attn_bwd(*alone, table, lut, a[0][:1], dout[:1], a[1][:1].contiguous(), **one)
+    if H == Hk:                                             # (the heads of a group are dealt over workgroups by the grid's size)
+        for x, y in zip(got[:3], a[2:5]):
+            assert torch.equal(x, y[:1])
+
+
+def test_packed_without_a_sequence(dev):
+    """offsets of no sequence at all: fresh outputs are zero, given ones stay as they were"""
+    ops = _ops()
+    q, k, v, table, lut, dout = (x[0] if x.dim() == 4 else x for x in make(dev, torch.bfloat16, 1, 90, 90, 4, 2, 64))
+    cu = torch.zeros(1, dtype=torch.int32, device=dev)
+    out, lse = ops.relpos_attn_fwd(q, k, v, table, lut, cu_q=cu, cu_k=cu)
+    dq, dk, dv, dt = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, cu_q=cu, cu_k=cu)
+    assert not out.any() and bool((lse == -math.inf).all()) and not dq.any() and not dk.any() and not dv.any() and not dt.any()
+    mine = [torch.full_like(x, 7.0) for x in (q, k, v)]
+    ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, cu_q=cu, cu_k=cu, dq=mine[0], dk=mine[1], dv=mine[2])
+    assert all(bool((x == 7).all()) for x in mine)
+
+
 def test_packed_rows_in_front(dev):
     """offsets that do not start at 0: the rows in front belong to no sequence either"""
     ops = _ops()
