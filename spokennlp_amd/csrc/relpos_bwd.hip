@@ -71,6 +71,7 @@ __device__ __forceinline__ bool rp_fine(const RpArgs& a, const RpSeq& sq, int q0
     return c * 64 <= RP_FINE || sq.qn <= RP_FINE / 2;
 }
 
+// MIXED: row blocks may be FINE, or the keys are split (an instance of its own: what only these need costs the plain one 5 % at 4 x 4096 by its registers)
 template <typename T, int DT, int QT_, bool MIXED>
 __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
@@ -80,10 +81,10 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     const int nmain = a.B * a.heads * a.nrb;
-    const int split = nmain ? blockIdx.x / nmain : a.nsplit;
-    if (split >= a.nsplit) {
+    const int nsplit = MIXED ? a.nsplit : 1, split = nmain ? (int)blockIdx.x / nmain : nsplit;
+    if (split >= nsplit) {
         const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq);
-        rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain * a.nsplit, RP_TAIL_WGS, tid);
+        rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain * nsplit, RP_TAIL_WGS, tid);
         return;
     }
     int rb, h, b;
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
         }
         int c_from = 0;
-        if (a.nsplit > 1) { c_from = split * (a.split_keys / 64); c_end = min(c_end, c_from + a.split_keys / 64); }
+        if (MIXED && nsplit > 1) { c_from = split * (a.split_keys / 64); c_end = min(c_end, c_from + a.split_keys / 64); }
         typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
         float nl[QT], rsum[QT];                             // -lse in the exponent's units; sum of a row's ds (each of its four lanes: a quarter of the keys)
         f32x4 nd[QT];                                       // -delta, as what the product dout . v starts from
@@ -261,13 +262,13 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             const int q = qw + ct * 16 + i16;
             if (q >= sq.qn) continue;
             const int64_t row = rp_row(a, sq, b, h, q);
-            if (a.nsplit > 1) {                             // rp_join_q_kernel adds them up
+            if (MIXED && nsplit > 1) {                      // rp_join_q_kernel adds them up
                 float* op = a.part_q + (split * rows + row) * a.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
                     if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(op + d * 16 + g * 4) = dq[ct][d] * a.scale;
                 if (g == 0) {
-                    a.part_q[a.nsplit * rows * a.D + split * rows + row] = rsum[ct];
+                    a.part_q[nsplit * rows * a.D + split * rows + row] = rsum[ct];
                     if (split == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = nd[ct][0]; }
                 }
                 continue;
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     };
     for (; rb * BQ_ < sq.qn; rb += a.nrb) {
         constexpr int FQ = DT <= 4 ? QT_ : 1;               // (D > 64: 16 columns a wave, the second part needs the registers)
-        if constexpr (MIXED)
+        if constexpr (MIXED && MEND)
             if (rp_fine(a, sq, rb * BQ_)) {
                 for (int q0 = rb * BQ_; q0 < min((rb + 1) * BQ_, sq.qn); q0 += 64 * FQ) block(std::integral_constant<int, FQ>(), std::true_type(), q0);
                 continue;
@@ -290,7 +291,8 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     }
 }
 
-template <typename T, int DT, int QT>
+// CUT: the query heads of a group, or the query rows, are dealt over several workgroups (an instance of its own, as above)
+template <typename T, int DT, int QT, bool CUT>
 __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv_kernel(RpArgs a) {
     typedef RpTile<T, DT> Ti;
     constexpr int NB = rp_nb<T, DT>;
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     float* tab = rows + NB * 128;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int parts = a.parts, qsplit = a.qsplit, nmain = a.B * a.kv_heads * parts * a.nrb, split = nmain ? blockIdx.x / nmain : qsplit;
+    const int parts = CUT ? a.parts : 1, qsplit = CUT ? a.qsplit : 1, nmain = a.B * a.kv_heads * parts * a.nrb, split = nmain ? (int)blockIdx.x / nmain : qsplit;
     if (split >= qsplit) {
         const int lead = rp_clamp(a.cu_k[0], 0, a.Tk), end = rp_clamp(a.cu_k[a.B], lead, a.Tk);
         rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain * qsplit, RP_TAIL_WGS, tid);
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
         const int k0 = rb * BK, kw = k0 + w * 16 * QT;
         int c_first = 0, n_ch = (sq.qn + 63) / 64;
         if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
-        if (qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
+        if (CUT && qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
         const T *qb, *ob;
         const float* stat_h;
         auto fetch = [&](int c, int buf) {
@@ -552,7 +554,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
             const int key = kw + ct * 16 + i16;
             if (key >= rows_k) continue;
             const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            if (parts * qsplit > 1) {
+            if (CUT) {
                 const int64_t rows_all = (int64_t)a.B * a.Lk, row = (int64_t)b * a.Lk + key;
                 float* kp_ = a.part_kv + ((((hp - hk * parts) * qsplit + split) * rows_all + row) * a.kv_heads + hk) * a.D;
                 float* vp_ = kp_ + parts * qsplit * rows_all * a.kv_heads * a.D;
@@ -694,6 +696,15 @@ static int rp_dq_one(const RpArgs& a, int64_t n, int lds, hipStream_t s) {
     hipLaunchKernelGGL((rp_dq_kernel<T, DT, QT, MIXED>), dim3((unsigned)n), dim3(256), lds, s, a);
     return 0;
 }
+template <typename T, int DT, int QT>
+static int rp_dkv_one(const RpArgs& a, int64_t n, int lds, hipStream_t s) {
+    const bool cut = a.parts * a.qsplit > 1;
+    const int rc = rp_allow_lds(cut ? (const void*)rp_dkv_kernel<T, DT, QT, true> : (const void*)rp_dkv_kernel<T, DT, QT, false>, lds);
+    if (rc) return rc;
+    if (cut) hipLaunchKernelGGL((rp_dkv_kernel<T, DT, QT, true>), dim3((unsigned)n), dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((rp_dkv_kernel<T, DT, QT, false>), dim3((unsigned)n), dim3(256), lds, s, a);
+    return 0;
+}
 template <typename T, int DT>
 static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStream_t s) {
     const int ND = 2 * (a.span + RP_PAD) + 1;
@@ -706,9 +717,9 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
     int rc = 0;
     if (n > 0) {
-        if (sizeof(T) == 4) rc = rp_dq_one<T, DT, 1, false>(a, n, lds, s);
+        if (sizeof(T) == 4) rc = a.nsplit > 1 ? rp_dq_one<T, DT, 1, true>(a, n, lds, s) : rp_dq_one<T, DT, 1, false>(a, n, lds, s);
         else if constexpr (sizeof(T) == 2) {                // can any row block be FINE?  Packed and ragged lengths are on the device
-            const bool mixed = a.causal || a.cu_q || a.k_lens || a.Lk <= RP_FINE || a.Lq <= RP_FINE / 2;
+            const bool mixed = a.causal || a.cu_q || a.k_lens || a.Lk <= RP_FINE || a.Lq <= RP_FINE / 2 || a.nsplit > 1;
             if (mixed) rc = qt == 1 ? rp_dq_one<T, DT, 1, true>(a, n, lds, s) : rp_dq_one<T, DT, 2, true>(a, n, lds, s);
             else rc = qt == 1 ? rp_dq_one<T, DT, 1, false>(a, n, lds, s) : rp_dq_one<T, DT, 2, false>(a, n, lds, s);
         }
@@ -729,13 +740,11 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
     } else if (sizeof(T) == 4 || DT > 4 || kt == 1) {
-        if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 1>, lds2))) return rc;
-        hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 1>), dim3((unsigned)m), dim3(256), lds2, s, a);
+        rc = rp_dkv_one<T, DT, 1>(a, m, lds2, s);
     } else if constexpr (sizeof(T) == 2 && DT <= 4) {
-        if ((rc = rp_allow_lds((const void*)rp_dkv_kernel<T, DT, 2>, lds2))) return rc;
-        hipLaunchKernelGGL((rp_dkv_kernel<T, DT, 2>), dim3((unsigned)m), dim3(256), lds2, s, a);
+        rc = rp_dkv_one<T, DT, 2>(a, m, lds2, s);
     }
-    if ((rc = amdseg_launch_status())) return rc;
+    if (rc || (rc = amdseg_launch_status())) return rc;
     if (a.parts * a.qsplit > 1 && m > 0) {
         const int64_t vecs = (int64_t)a.B * a.Lk * a.kv_heads * (a.D / 4);
         if ((vecs + 255) / 256 > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
