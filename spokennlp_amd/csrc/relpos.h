@@ -225,11 +225,11 @@ __device__ __forceinline__ void rp_cleared() { asm volatile("s_waitcnt lgkmcnt(0
 __device__ __forceinline__ void rp_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); __syncthreads(); }
 
 // the bias values of the score tiles whose block diagonal (row tile - column tile) is k0, k0 + 1, ...: lane (g, i16), register r = rel 16 k + 4 g + r - i16
-// (or zeros, where the whole tile is beyond the span)
+// (or `far`, where the whole tile is beyond the span)
 template <int N>
-__device__ __forceinline__ void rp_bias_or_zero(bool near, const float* bt, int k0, f32x4 (&z)[N]) {
+__device__ __forceinline__ void rp_bias(bool near, const float* bt, int k0, float far, f32x4 (&z)[N]) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < N; ++k) z[k] = (f32x4){far, far, far, far};
     if (near)
 #pragma unroll
         for (int k = 0; k < N; ++k)

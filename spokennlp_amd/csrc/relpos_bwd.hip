@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
 #pragma unroll
             for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
                 f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], z[Ti::RPS + QT - 1];
-                rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
+                rp_bias(near, bt, kp * Ti::RPS + 1 - QT, 0.f, z);
 #pragma unroll
                 for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
@@ -416,20 +416,16 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                 const char* tO = tQ + Ti::BYTES;
                 const float* rowd = rowl + 64;
                 const float* bt = tab + (rel0 + mid + 4 * g - i16);
-                const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
+                const float far = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0];
 #pragma unroll
                 for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
                     f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS], dr[Ti::RPS], z[Ti::RPS + QT - 1];
-                    rp_bias_or_zero(near, bt, kp * Ti::RPS + 1 - QT, z);
+                    rp_bias(near, bt, kp * Ti::RPS + 1 - QT, far, z);
 #pragma unroll
                     for (int j = 0; j < Ti::RPS; ++j) {
                         const int f = kp * Ti::RPS + j;
                         lr[j] = *reinterpret_cast<const f32x4*>(rowl + f * 16 + g * 4);
                         dr[j] = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
-                        if (!near) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) lr[j][r] += fc;
-                        }
                     }
 #pragma unroll
                     for (int kk = 0; kk < Ti::KB; ++kk)

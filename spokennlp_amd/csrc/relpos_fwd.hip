@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
         auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
             const char* tV = tK + Ti::BYTES;
             f32x4 s[QT][4], z[3 + QT];
-            rp_bias_or_zero(near, tab + (rel0 + mid + 4 * g - i16), 1 - QT, z);
+            rp_bias(near, tab + (rel0 + mid + 4 * g - i16), 1 - QT, 0.f, z);
 #pragma unroll
             for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
