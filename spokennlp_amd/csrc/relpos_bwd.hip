@@ -452,6 +452,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                             }
                     }
                     typename Ti::frag fp[QT], fds[QT];
+                    typename Ti::frag fo = Ti::colf(tO, kp, 0, l), fq = Ti::colf(tQ, kp, 0, l);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int ct = 0; ct < QT; ++ct) {
 #pragma unroll
@@ -494,11 +496,12 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                     }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        const typename Ti::frag fo = Ti::colf(tO, kp, d, l), fq = Ti::colf(tQ, kp, d, l);
+                        const typename Ti::frag co = fo, cq = fq;
+                        if (d + 1 < DT) { fo = Ti::colf(tO, kp, d + 1, l); fq = Ti::colf(tQ, kp, d + 1, l); }
 #pragma unroll
                         for (int ct = 0; ct < QT; ++ct) {
-                            dv[ct][d] = Ti::mma(fo, fp[ct], dv[ct][d]);
-                            dk[ct][d] = Ti::mma(fq, fds[ct], dk[ct][d]);
+                            dv[ct][d] = Ti::mma(co, fp[ct], dv[ct][d]);
+                            dk[ct][d] = Ti::mma(cq, fds[ct], dk[ct][d]);
                         }
                     }
                 }
