@@ -91,6 +91,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ_ = 64 * QT_;
+    constexpr bool AHEAD = sizeof(T) == 2;
     constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums, and so is ds)
     if (rb * BQ_ >= sq.qn) return;
     RpTable table;
@@ -204,7 +205,8 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                                 s[ct][j][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][j][r] : -INFINITY;
                     }
                 }
-                typename Ti::frag fds[QT];
+                typename Ti::frag fds[QT], ahead;           // K fragments are read one step ahead, the first under the exponentials (fp32 has no registers for it)
+                if constexpr (AHEAD) { ahead = Ti::colf(tK, kp, 0, l); __builtin_amdgcn_sched_barrier(0); }
 #pragma unroll
                 for (int ct = 0; ct < QT; ++ct) {
                     float sum = 0.f;
@@ -220,7 +222,8 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                 }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const typename Ti::frag fk = Ti::colf(tK, kp, d, l);
+                    const typename Ti::frag fk = AHEAD ? ahead : Ti::colf(tK, kp, d, l);
+                    if (AHEAD && d + 1 < DT) ahead = Ti::colf(tK, kp, d + 1, l);
 #pragma unroll
                     for (int ct = 0; ct < QT; ++ct) dq[ct][d] = Ti::mma(fk, fds[ct], dq[ct][d]);
                 }
@@ -452,8 +455,9 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                             }
                     }
                     typename Ti::frag fp[QT], fds[QT];
-                    typename Ti::frag fo = Ti::colf(tO, kp, 0, l), fq = Ti::colf(tQ, kp, 0, l);
-                    __builtin_amdgcn_sched_barrier(0);
+                    constexpr bool AHEAD = sizeof(T) == 2;  // column fragments one step ahead, as in rp_dq_kernel
+                    typename Ti::frag fo, fq;
+                    if constexpr (AHEAD) { fo = Ti::colf(tO, kp, 0, l); fq = Ti::colf(tQ, kp, 0, l); __builtin_amdgcn_sched_barrier(0); }
 #pragma unroll
                     for (int ct = 0; ct < QT; ++ct) {
 #pragma unroll
@@ -496,8 +500,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                     }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        const typename Ti::frag co = fo, cq = fq;
-                        if (d + 1 < DT) { fo = Ti::colf(tO, kp, d + 1, l); fq = Ti::colf(tQ, kp, d + 1, l); }
+                        const typename Ti::frag co = AHEAD ? fo : Ti::colf(tO, kp, d, l), cq = AHEAD ? fq : Ti::colf(tQ, kp, d, l);
+                        if (AHEAD && d + 1 < DT) { fo = Ti::colf(tO, kp, d + 1, l); fq = Ti::colf(tQ, kp, d + 1, l); }
 #pragma unroll
                         for (int ct = 0; ct < QT; ++ct) {
                             dv[ct][d] = Ti::mma(co, fp[ct], dv[ct][d]);

@@ -111,6 +111,8 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                 }
             }
             const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
+            typename Ti::frag ahead = Ti::colf(tV, 0, 0, l);        // V fragments are read one step ahead: the first under the exponentials
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ct = 0; ct < QT; ++ct) {
                 float mx = s[ct][0][0];
@@ -150,7 +152,9 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                 for (int ct = 0; ct < QT; ++ct) fp[ct] = Ti::pf(&s[ct][kp * Ti::RPS]);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const typename Ti::frag fv = Ti::colf(tV, kp, d, l);
+                    const typename Ti::frag fv = ahead;
+                    if (d + 1 < DT) ahead = Ti::colf(tV, kp, d + 1, l);
+                    else if (kp + 1 < 64 / Ti::KSTEP) ahead = Ti::colf(tV, kp + 1, 0, l);
 #pragma unroll
                     for (int ct = 0; ct < QT; ++ct) o[ct][d] = Ti::mma(fv, fp[ct], o[ct][d]);
                 }
