@@ -7,7 +7,8 @@
 //
 // delta.  sum_j ds_ij = 0, so a bucket that holds most of a row's probability has for its gradient what is left of a cancellation; delta taken from the
 // bf16 `out` is off by up to 2^-8 of it, the same way for every element of the row (1 % of dtable measured, 40 queries against 3 .. 1500 keys).  What the
-// ds of a row sum to instead of 0 IS that error (sum_j p_ij = 1): rp_dq_kernel sums them in fp32 on its way and hands the mended delta on.  Its own dq
+// ds of a row sum to instead of 0 IS that error (sum_j p_ij = 1): rp_dq_kernel sums them in fp32 on its way and hands the mended delta on
+// (fp32 alike, where p's own rounding is what it mends: dtable 7.3e-7 -> 6.4e-7 of its norm, 6 x 1180 at D = 128).  Its own dq
 // feels the error only where a row's probability sits on a few keys (by 1 / sqrt of their number), beside the rounding of ds to bf16 for the product with k.
 // Row blocks of at most RP_FINE keys, and sequences of at most RP_FINE / 2 rows (too few values for roundings to average out), have ds as two bf16 parts there:
 // dq within 1.8e-3 of its norm instead of 2.5e-3, one more product of the three, on blocks whose time is latency.  (A copy of the whole walk, FINE, in a
@@ -92,7 +93,6 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     const RpSeq sq = rp_seq(a, b);
     constexpr int BQ_ = 64 * QT_;
     constexpr bool AHEAD = sizeof(T) == 2;
-    constexpr bool MEND = sizeof(T) == 2;                   // (fp32: delta is as exact as the sums, and so is ds)
     if (rb * BQ_ >= sq.qn) return;
     RpTable table;
     table.start(a, 1, tid);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             dp[ct][j][r] *= __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, al[ct]));
-                            if (MEND) sum += dp[ct][j][r];
+                            sum += dp[ct][j][r];
                         }
                     rsum[ct] += sum;
                     fds[ct] = Ti::pf(dp[ct]);
@@ -252,14 +252,11 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
             chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
         }
-        if (MEND)
 #pragma unroll
-            for (int ct = 0; ct < QT; ++ct) {
-                float rho = rsum[ct];
-                rho += __shfl_xor(rho, 16, 64);
-                rho += __shfl_xor(rho, 32, 64);
-                rsum[ct] = rho;
-            }
+        for (int ct = 0; ct < QT; ++ct) {
+            rsum[ct] += __shfl_xor(rsum[ct], 16, 64);
+            rsum[ct] += __shfl_xor(rsum[ct], 32, 64);
+        }
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
@@ -285,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     };
     for (; rb * BQ_ < sq.qn; rb += a.nrb) {
         constexpr int FQ = DT <= 4 ? QT_ : 1;               // (D > 64: 16 columns a wave, the second part needs the registers)
-        if constexpr (MIXED && MEND)
+        if constexpr (MIXED && sizeof(T) == 2)
             if (rp_fine(a, sq, rb * BQ_)) {
                 for (int q0 = rb * BQ_; q0 < min((rb + 1) * BQ_, sq.qn); q0 += 64 * FQ) block(std::integral_constant<int, FQ>(), std::true_type(), q0);
                 continue;
@@ -608,7 +605,7 @@ __global__ __launch_bounds__(256) void rp_join_q_kernel(RpArgs a) {
     for (int i = 1; i < a.nsplit; ++i) s += *reinterpret_cast<const f32x4*>(a.part_q + i * rows * a.D + x);
     const int64_t bh = row / a.Lq, q = row % a.Lq;
     RpTile<T, 2>::st4((T*)a.dq + bh / a.heads * a.sdq.sb + q * a.sdq.st + bh % a.heads * a.sdq.sh + d, s);
-    if (d == 0 && sizeof(T) == 2) {
+    if (d == 0) {
         float rho = 0.f;
         for (int i = 0; i < a.nsplit; ++i) rho += a.part_q[a.nsplit * rows * a.D + i * rows + row];
         a.stat[rows + row] -= rho;
