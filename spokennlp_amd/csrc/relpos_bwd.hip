@@ -188,11 +188,15 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                         const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g), fv = Ti::rowf(tV, f * 16 + i16, kk, g);
 #pragma unroll
                         for (int ct = 0; ct < QT; ++ct) {
-                            const f32x4 start = z[j - ct + QT - 1];
-                            s[ct][j] = Ti::mma(fk, fq[ct][kk], kk == 0 ? start : s[ct][j]);
+                            s[ct][j] = Ti::mma(fk, fq[ct][kk], kk == 0 ? rp_start<T>(z[j - ct + QT - 1]) : s[ct][j]);
                             dp[ct][j] = Ti::mma(fv, fdo[ct][kk], kk == 0 ? nd[ct] : dp[ct][j]);
                         }
                     }
+                if (sizeof(T) == 4)
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) s[ct][j] += z[j - ct + QT - 1];
                 if (edge) {
 #pragma unroll
                     for (int j = 0; j < Ti::RPS; ++j) {
@@ -435,11 +439,15 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
                             const typename Ti::frag fq = Ti::rowf(tQ, f * 16 + i16, kk, g), fo = Ti::rowf(tO, f * 16 + i16, kk, g);
 #pragma unroll
                             for (int ct = 0; ct < QT; ++ct) {
-                                const f32x4 start = z[j - ct + QT - 1];
-                                s[ct][j] = Ti::mma(fq, fk[ct][kk], kk == 0 ? start : s[ct][j]);
+                                s[ct][j] = Ti::mma(fq, fk[ct][kk], kk == 0 ? rp_start<T>(z[j - ct + QT - 1]) : s[ct][j]);
                                 dp[ct][j] = Ti::mma(fo, fv[ct][kk], kk == 0 ? dr[j] : dp[ct][j]);
                             }
                         }
+                    if (sizeof(T) == 4)
+#pragma unroll
+                        for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct) s[ct][j] += z[j - ct + QT - 1];
                     if (edge) {                             // a hidden key's column, rel > 0 with `causal`, a row behind the sequence: p = 0
 #pragma unroll
                         for (int j = 0; j < Ti::RPS; ++j)

@@ -96,9 +96,14 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
                     const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g);
 #pragma unroll
                     for (int ct = 0; ct < QT; ++ct) {
-                        s[ct][f] = Ti::mma(fk, fq[ct][kk], kk == 0 ? z[f - ct + QT - 1] : s[ct][f]);
+                        s[ct][f] = Ti::mma(fk, fq[ct][kk], kk == 0 ? rp_start<T>(z[f - ct + QT - 1]) : s[ct][f]);
                     }
                 }
+            if (sizeof(T) == 4)
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) s[ct][f] += z[f - ct + QT - 1];
             if (edge) {
 #pragma unroll
                 for (int f = 0; f < 4; ++f) {
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
         }
         const int rel0 = c * 64 + 4 * g - pos;
         const bool near = c * 64 + 63 - sq.off > -a.span && c * 64 - (sq.off + a.Lq - 1) < a.span;
-        f32x4 s[4];
+        f32x4 s[4], z[4];
         if (near) {
             const float inv = 1.0f / a.scale;
             int bk[4][4];
@@ -274,14 +279,17 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[f][r] = rp_table(a, bk[f][r], h) * inv;
+                for (int r = 0; r < 4; ++r) z[f][r] = rp_table(a, bk[f][r], h) * inv;
         } else
 #pragma unroll
-            for (int f = 0; f < 4; ++f) s[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int f = 0; f < 4; ++f) z[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
-            for (int f = 0; f < 4; ++f) s[f] = Ti::mma(fk[f][kk], fq[kk], s[f]);
+            for (int f = 0; f < 4; ++f) s[f] = Ti::mma(fk[f][kk], fq[kk], kk == 0 ? rp_start<T>(z[f]) : s[f]);
+        if (sizeof(T) == 4)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) s[f] += z[f];
         const float fc = near ? 0.f : c * 64 > sq.off ? farR : farL;
         if (now != ~0ull || causal)
 #pragma unroll
