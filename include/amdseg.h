@@ -423,6 +423,8 @@ int amdseg_heads_bwd_rows(const float* gout, const float* x, int M, int H, float
  * fp32 tensors in exact fp32); table_dtype independent; softmax, lse and every sum fp32.
  * lse: [B, heads, Lq] or, packed, [heads, Tq]; may be NULL in forward.  Backward: dq, dk, dv (strides of their own), dtable [buckets, heads] in
  * table_dtype (NULL: not computed); sums are taken in a fixed order (bit-reproducible), gradients of shared kv heads include all their query heads.
+ * A sequence's out, lse and dq do not depend on the batch around it; dk and dv neither, unless kv heads are shared (how many workgroups share a group's heads
+ * follows the grid).  Outputs and ws must overlap neither each other nor an input.
  * ws: amdseg_relpos_attn_ws_bytes(cfg, backward) bytes of scratch on 16 bytes (0 bytes: NULL allowed). */
 struct amdseg_relpos_cfg {
     int32_t dtype, table_dtype, B, Lq, Lk, Tq, Tk, heads, kv_heads, D, span, buckets, causal, align_end, zero_tail;

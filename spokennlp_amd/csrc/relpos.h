@@ -6,7 +6,7 @@
 // The bias depends on (i, j) through rel alone, so it is no [Lq, Lk] operand but a vector of 2 span + 1 floats per head.  A workgroup writes it into LDS
 // once, extended by RP_PAD copies of the end values on both sides: a 64-row tile that touches |rel| < span then indexes without clamping, and a tile
 // wholly beyond one end (almost all of a long sequence) starts from a constant and costs nothing.  It is kept divided by `scale`: MFMA accumulators START from
-// it and scale * log2 e multiplies the finished score inside the exponent's fma.
+// it (fp32: it is added behind the products, rp_start) and scale * log2 e multiplies the finished score inside the exponent's fma.
 #pragma once
 #include <math.h>
 #include <algorithm>

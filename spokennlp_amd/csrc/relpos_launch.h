@@ -20,8 +20,8 @@ static inline int rp_allow_lds(const void* kernel, int bytes) {
 }
 // 16-row tiles a wave carries as columns: two (every LDS fragment feeds two products; 32 x 512 forward 54 us against 64, dK / dV 108 against 146) unless one
 // gives the CUs a second workgroup that they would not have: grids of up to 256 (2048 rows of 16 heads: dK / dV 73 us against 77), forward and dQ at D <= 64 up
-// to 384 (2 x 2048 rows of 12 heads: forward 59 against 66, dQ 64 against 71; dK / dV 122 against 98; at 432 two win: 22 against 22.5, 27 against 31).  fp32: one (registers).  D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a
-// SIMD (16 x 512: 113 us against 104 with one tile), and a forward grid of three rounds or more runs better on three waves a SIMD of one tile (4 x 2048:
+// to 384 (2 x 2048 rows of 12 heads: forward 59 against 66, dQ 64 against 71; dK / dV 122 against 98; at 432 two win: 22 against 22.5, 27 against 31).  fp32: one (registers).
+// D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a SIMD (16 x 512: 113 us against 104 with one tile), and a forward grid of three rounds or more runs better on three waves a SIMD of one tile (4 x 2048:
 // 177 against 165).
 static inline int rp_qt(int64_t wgs_of_two, int most_of_one, int dtype) { return dtype == 1 ? 1 : wgs_of_two <= most_of_one ? 1 : 2; }
 static inline int64_t rp_wgs_of_two(const RpArgs& a) { return (int64_t)((a.Lq + 127) / 128) * a.B * a.heads; }
@@ -29,7 +29,8 @@ static inline int rp_dq_qt(const RpArgs& a, int dtype) { return rp_qt(rp_wgs_of_
 static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return a.D > 64 && rp_wgs_of_two(a) >= 768 ? 1 : rp_dq_qt(a, dtype); }
 static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, 256, dtype); }
 // dK / dV of shared kv heads: a workgroup walks the rows of all G query heads; where that leaves less than two workgroups a CU, `parts` of them take G / parts
-// heads each and rp_join_kv_kernel adds their fp32 sums (a walk of less than RP_PART_STEPS chunks is not worth its launch).  Not for packed sequences: `longest` is
+// heads each and rp_join_kv_kernel adds their fp32 sums (3 x 1023 causal, 16 / 4 heads, D = 128: 150 -> 75 us with the join;
+// at RP_PART_STEPS chunks a walk, 4 x 256 rows of 16 / 4 heads, 37 -> 23, below that there is little to share out).  Not for packed sequences: `longest` is
 // a hint there and must not change bits.
 #define RP_PART_STEPS 16
 static inline int rp_dkv_parts(const RpArgs& a, int kt, int qsplit) {
@@ -40,7 +41,7 @@ static inline int rp_dkv_parts(const RpArgs& a, int kt, int qsplit) {
     while (p < G && (G % p || n * p < 512)) ++p;
     return p;
 }
-// and its mirror for dK / dV: few keys against many query rows, whose walk is cut every RP_SPLIT_ROWS
+// dK / dV of few keys against many query rows: the walk is cut every RP_SPLIT_ROWS (forward + backward, 11 x 3949 rows x 5 keys: 148 -> 79 us).  Shapes alone decide.
 #define RP_SPLIT_ROWS 1024
 static inline int rp_qsplit(const RpArgs& a) { return !a.cu_q && a.Lk <= 128 && a.Lq > RP_SPLIT_ROWS ? (a.Lq + RP_SPLIT_ROWS - 1) / RP_SPLIT_ROWS : 1; }
 // the rows of a kv head's query heads fit the 16 columns of one tile
@@ -48,7 +49,8 @@ static inline bool rp_few(const RpArgs& a) {
     return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;
 }
 // splits over the keys: few query rows against many keys (single tokens, a handful of rows against a cache), joined by rp_join_kernel.  A number of keys that
-// the shapes alone decide: a sequence's sums do not depend on the batch around it.  (3 x 47 rows of 4 heads against 4545 keys, fp32: 449 -> 148 us.)
+// the shapes alone decide: a sequence's sums do not depend on the batch around it.  (3 x 47 rows of 4 heads against 4545 keys, fp32: 449 -> 148 us; dQ is split
+// alike, joined by rp_join_q_kernel: forward + backward of 4 x 86 rows x 6756 keys 192 -> 102 us.)
 static inline int rp_split_keys(int Lq) { return Lq <= 16 ? 512 : 1024; }
 static inline int rp_nsplit(int Lq, int Lk, bool packed) {
     return !packed && Lq <= 128 && Lk > rp_split_keys(Lq) ? (Lk + rp_split_keys(Lq) - 1) / rp_split_keys(Lq) : 1;

@@ -561,7 +561,8 @@ def _rp_cfg(q, k, v, table, bucket_map, scale, key_mask, k_lens, cu_q, cu_k, max
     such combination and copied (a call on a few rows is otherwise longer on the host than on the GPU); pointers and devices are looked at every time.
     `more(c, shape of lse)` fills in the other tensors' strides, `more_key` is all that it looks at."""
     key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, table.shape, table.stride(), table.dtype, bucket_map.shape,
-           bucket_map.stride(), bucket_map.dtype, scale, max_q, max_k, bool(causal), bool(align_end), cu_q is None or cu_q.shape, cu_k is None or cu_k.shape,
+           bucket_map.stride(), bucket_map.dtype, scale if scale is None else float(scale), max_q if max_q is None else int(max_q),
+           max_k if max_k is None else int(max_k), bool(causal), bool(align_end), cu_q is None or cu_q.shape, cu_k is None or cu_k.shape,
            k_lens is None, None if key_mask is None else (key_mask.shape, key_mask.stride(), key_mask.dtype), more_key)
     known = _rp_known.get(key)
     if known is None:

@@ -93,7 +93,7 @@ class _RelposBias(torch.autograd.Function):
 def relpos_attention(q, k, v, table, bucket_map, *, scale=None, key_mask=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None, causal=False,
                      align_end=False):
     """differentiable ops.relpos_attn_fwd: out with q's shape; gradients for q, k, v and the table"""
-    how = dict(scale=scale, key_mask=key_mask, k_lens=k_lens, cu_q=cu_q, cu_k=cu_k, max_q=max_q, max_k=max_k, causal=causal, align_end=align_end)
+    how = dict(scale=None if scale is None else float(scale), key_mask=key_mask, k_lens=k_lens, cu_q=cu_q, cu_k=cu_k, max_q=max_q, max_k=max_k, causal=causal, align_end=align_end)
     return _RelposAttention.apply(q, k, v, table, bucket_map, how)
 
 
@@ -103,7 +103,7 @@ def relpos_self_attention(qkv, heads, table, bucket_map, *, kv_heads=None, scale
     kv_heads = kv_heads or heads
     if qkv.shape[-1] % (heads + 2 * kv_heads):
         raise ValueError(f"a projection of {qkv.shape[-1]} columns does not hold {heads} + 2 * {kv_heads} heads")
-    how = dict(scale=scale, key_mask=key_mask, cu_q=cu_seqlens, cu_k=cu_seqlens, max_q=longest, max_k=longest, causal=causal)
+    how = dict(scale=None if scale is None else float(scale), key_mask=key_mask, cu_q=cu_seqlens, cu_k=cu_seqlens, max_q=longest, max_k=longest, causal=causal)
     return _RelposSelfAttention.apply(qkv, table, bucket_map, heads, kv_heads, how).flatten(-2)
 
 

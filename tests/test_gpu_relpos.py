@@ -311,6 +311,33 @@ def test_packed_without_a_sequence(dev):
     assert all(bool((x == 7).all()) for x in mine)
 
 
+def test_options_are_taken_by_value(dev):
+    """a scale given as a 0-dim tensor that changes between two calls, gradients into given views where the walk is split"""
+    ops = _ops()
+    q, k, v, table, lut, dout = make(dev, torch.float32, 1, 70, 2100, 2, 2, 64)
+    scale = torch.tensor(0.125)
+    one = ops.relpos_attn_fwd(q, k, v, table, lut, scale=scale)[0]
+    scale.mul_(2)
+    two = ops.relpos_attn_fwd(q, k, v, table, lut, scale=scale)[0]
+    assert torch.equal(one, ops.relpos_attn_fwd(q, k, v, table, lut, scale=0.125)[0])
+    assert torch.equal(two, ops.relpos_attn_fwd(q, k, v, table, lut, scale=0.25)[0]) and not torch.equal(one, two)
+    from spokennlp_amd import relpos
+    grads = []
+    for s in (scale, 0.25):                                 # (the tensor changes between the forward pass and the backward one)
+        leaf = q.detach().clone().requires_grad_()
+        y = relpos.relpos_attention(leaf, k, v, table, lut, scale=s)
+        scale.fill_(0.5)
+        y.backward(dout)
+        grads.append(leaf.grad)
+    assert torch.equal(*grads)
+    out, lse = ops.relpos_attn_fwd(q, k, v, table, lut)
+    want = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse)
+    dq = torch.full((1, 2, 70, 72), 7.0, device=dev)[..., :64].permute(0, 2, 1, 3)
+    got = ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, dq=dq, dk=torch.empty_like(k), dv=torch.empty_like(v))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
 def test_packed_rows_in_front(dev):
     """offsets that do not start at 0: the rows in front belong to no sequence either"""
     ops = _ops()
