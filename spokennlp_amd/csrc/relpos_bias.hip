@@ -6,6 +6,7 @@
 
 // Write-bound.  A workgroup keeps its head's 2 span + 1 values in LDS (one float of gap per 8, so that lanes 8 elements apart hit different banks)
 // and writes rows in 16-byte units; a row that does not start on 16 bytes has its first and last unit element by element.
+// 12 x 1537 x 2049 fp32: 151 MB in 27 us, 5.7 TB/s; 12 x 512 x 512 bf16: 5.5 us.
 template <typename T>
 __global__ __launch_bounds__(256) void rp_bias_kernel(RpArgs a, int off, int rows_per_wg) {
     extern __shared__ float val[];
@@ -39,6 +40,7 @@ __global__ __launch_bounds__(256) void rp_bias_kernel(RpArgs a, int off, int row
 //    equal rel stay in the same one of its 15 registers; 16 bytes a load, 64 lanes side by side.  At the end the lanes lay their registers into LDS, the lower 8
 //    first, then the upper 7, which belong to the next lane's places: one writer each, no order of arrival anywhere.
 //  * The two far sides are one sum each: 16 lanes a row, 16-byte loads, four under way.
+// 2 x 12 x 1537 x 2049 fp32 (rows that start on 4 bytes): 302 MB in 84 us, 3.6 TB/s, joins 9 us; 8 x 12 x 512 x 512 bf16 16 us, joins 9.
 typedef uint32_t rp_u4 __attribute__((ext_vector_type(4), aligned(2)));      // 16 bytes from any element: rows start where they start
 template <typename T> __device__ __forceinline__ void rp_ld8(const T* p, float (&v)[8]);
 template <> __device__ __forceinline__ void rp_ld8<bf16_t>(const bf16_t* p, float (&v)[8]) {

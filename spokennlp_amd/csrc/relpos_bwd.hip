@@ -4,6 +4,8 @@
 // Two kernels, neither with an atomic on a gradient: rp_dq_kernel owns query rows and walks the keys (dq, delta), rp_dkv_kernel owns keys and walks the
 // query rows of every head of its group (dk, dv, the sums for dtable).  Seven products instead of the five of the formulas; results do not depend on
 // any order of arrival.
+// Bound by vector issue beside the products (0.55 .. 0.6 and 0.36 of the cycles; two waves a SIMD, which overlap them only in part), no LDS conflicts.  12 heads,
+// D = 64, bf16: 32 x 512 dQ 74 us, dK / dV 105 us (table sums 5 + 5); 4 x 4096 409 .. 426 and 545 us, 750 TFLOP/s of the executed products together.
 //
 // delta.  sum_j ds_ij = 0, so a bucket that holds most of a row's probability has for its gradient what is left of a cancellation; delta taken from the
 // bf16 `out` is off by up to 2^-8 of it, the same way for every element of the row (1 % of dtable measured, 40 queries against 3 .. 1500 keys).  What the
@@ -602,7 +604,7 @@ __global__ __launch_bounds__(256) void rp_join_kv_kernel(RpArgs a) {
     RpTile<T, 2>::st4((T*)(which ? a.dv : a.dk) + b * st.sb + r * st.st + hk * st.sh + d, s);
 }
 
-// dq and the mended delta of the splits over the keys, in their order (padded form)
+// dq and the mended delta of the splits over the keys, in their order (padded form).  A launch's latency: few rows, a handful of splits
 template <typename T>
 __global__ __launch_bounds__(256) void rp_join_q_kernel(RpArgs a) {
     const int64_t rows = (int64_t)a.B * a.heads * a.Lq, x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
