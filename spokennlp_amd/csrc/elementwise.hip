@@ -450,9 +450,11 @@ __device__ __forceinline__ uint4 lnb_ld16(__amdgpu_buffer_rsrc_t r, uint32_t vof
     const lnb_v4i v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0);
     return make_uint4((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w);
 }
+// (the row's offset goes into the lane offset: with a scalar one the compiler takes the data registers of a 16-byte store as free in the next instruction,
+// and the hardware still reads them -- a vector instruction that rewrote the first one there had its value stored in 1 of 700 chunks)
 __device__ __forceinline__ void lnb_st16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, const uint4& q) {
     const lnb_v4i v = {(int)q.x, (int)q.y, (int)q.z, (int)q.w};
-    __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)voff, (int)soff, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(v, r, (int)(voff + soff), 0, 0);
 }
 __global__ LNP_BOUNDS void ln_bwd_pair768_kernel(const bf16_t* __restrict__ dy, const bf16_t* __restrict__ z,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
