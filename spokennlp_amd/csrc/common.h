@@ -64,11 +64,14 @@ __device__ __forceinline__ bf16_t f2bf(float f) {
     u += 0x7fffu + ((u >> 16) & 1u);
     return (bf16_t)(u >> 16);
 }
-// two fp32 -> packed bf16x2 with the gfx950 hardware conversion (round-to-nearest-even); one VALU op instead of ~14
+// two fp32 -> packed bf16x2 with the gfx950 hardware conversion (round-to-nearest-even); one VALU op instead of ~14.  The compiler's own conversion, not
+// inline asm: an asm statement that reads the result of a transcendental or matrix instruction right behind it gets no wait states from the compiler --
+// v_exp_f32 straight into an asm v_cvt_pk gave now and then the value of before
+typedef __bf16 amdseg_bf2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2bf(float lo, float hi) {
-    uint32_t r;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
-    return r;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, amdseg_bf2));
 }
 
 // generic load/store of an activation element type T in {float, bf16_t}

@@ -88,15 +88,6 @@ __device__ __forceinline__ void rp_place(int id, int nrb, int B, int heads, int 
 // RpTile<T, DT>: [64 rows][DT * 16 columns] in LDS.  A row fragment is the operand whose contraction runs along the columns (K of S^T = K Q^T), a
 // column fragment the one whose contraction runs along the rows (V^T of O^T = V^T P^T).  PF(): accumulator registers of the score tiles as the other
 // operand of that product -- the row order inside a contraction step is the accumulators' own, so the probabilities never move between lanes.
-// two fp32 -> bf16 x 2 (round to nearest even).  The compiler's conversion, not inline asm: an asm statement that reads the result of a transcendental (or
-// matrix) instruction right behind it gets no wait states from the compiler -- v_exp_f32 straight into an asm v_cvt_pk gave now and then the value of before
-typedef __bf16 rp_bf2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t rp_pack2(float x, float y) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const f2 v = {x, y};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, rp_bf2));
-}
-
 template <typename T, int DT> struct RpTile;
 template <int DT> struct RpTile<bf16_t, DT> {
     typedef bf16x8 frag;
@@ -111,7 +102,7 @@ template <int DT> struct RpTile<bf16_t, DT> {
     }
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ frag pf(const f32x4* s) {
-        const uint4 u = make_uint4(rp_pack2(s[0][0], s[0][1]), rp_pack2(s[0][2], s[0][3]), rp_pack2(s[1][0], s[1][1]), rp_pack2(s[1][2], s[1][3]));
+        const uint4 u = make_uint4(pack2bf(s[0][0], s[0][1]), pack2bf(s[0][2], s[0][3]), pack2bf(s[1][0], s[1][1]), pack2bf(s[1][2], s[1][3]));
         return __builtin_bit_cast(frag, u);
     }
     // x - what pf() kept of x
@@ -131,7 +122,7 @@ template <int DT> struct RpTile<bf16_t, DT> {
         for (int e = 0; e < 8; ++e) s += bf2f((bf16_t)a[e]) * bf2f((bf16_t)b[e]);
         return s;
     }
-    static __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(rp_pack2(v[0], v[1]), rp_pack2(v[2], v[3])); }
+    static __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
 };
 template <int DT> struct RpTile<float, DT> {
     typedef f32x4 frag;
