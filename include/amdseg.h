@@ -414,6 +414,9 @@ int amdseg_heads_bwd_rows(const float* gout, const float* x, int M, int H, float
  *   p_ij = softmax over the visible keys;  out_i = sum_j p_ij v_j;  lse_i = log sum_j exp(s_ij)
  * Key j is visible from query i iff j < keys of the sequence, key_mask (optional, 0 = hidden) allows it and, with `causal`, rel <= 0.  A row without a
  * visible key: out = 0, lse = -inf, no gradient.  K / V rows of hidden keys are never used, whatever they hold.
+ * Finite table entries may have any size: t beyond +-2^14 enters the scores as +-(2^14 + 128 log2(|t| / 2^14)) -- of two such buckets the larger still takes the
+ * row, and a row that sees only one has the softmax of scale q . k over it; lse is that of these scores, gradients are those of the formula.  An entry of -inf
+ * hides its bucket's keys.
  * Padded form (cu_q == cu_k == NULL): B sequences of Lq query and Lk key rows; k_lens (optional, int32 [B]) = keys held of each (a cache).
  * Packed form: sequence b = rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. of k (int32 [B + 1], device); Tq, Tk = rows of the buffers, Lq, Lk = the longest
  * sequence (a launch hint: too small a value costs time, not rows).  Rows outside every sequence: written as zeros (lse -inf) with zero_tail, else left alone.

@@ -281,6 +281,15 @@ __device__ __forceinline__ float rp_table(const RpArgs& a, int bk, int h) {
     const int64_t at = (int64_t)rp_clamp(bk, 0, a.buckets - 1) * a.heads + h;
     return a.table_bf16 ? bf2f(((const bf16_t*)a.table)[at]) : ((const float*)a.table)[at];
 }
+// A finite entry of any size as a score.  Beyond +-RP_HUGE it is brought in by a logarithm, which keeps the order of entries: twice as large is RP_DOUBLING more,
+// and e^-128 is 0.  Taken as they stand the largest would overflow over the scale or times log2 e, and a row that sees nothing else would have no
+// digits left: q . k vanishes beside 1e9, and exp2(s - lse) in backward is off by the rounding of lse (2^-24 of it; 2^-10 at most here).  Infinities stay.
+#define RP_HUGE 16384.f
+#define RP_DOUBLING 128.f
+__device__ __forceinline__ float rp_entry(const RpArgs& a, int bk, int h) {
+    const float t = rp_table(a, bk, h), x = fabsf(t);
+    return x > RP_HUGE && x < INFINITY ? copysignf(RP_HUGE + RP_DOUBLING * __builtin_amdgcn_logf(x * (1.f / RP_HUGE)), t) : t;
+}
 struct RpTable {
     int bk[2], n, mid, sign, tid;
     __device__ __forceinline__ int map(const RpArgs& a, int x) const { return a.map[rp_clamp(sign * (x - mid), -a.span, a.span) + a.span]; }
@@ -293,11 +302,11 @@ struct RpTable {
         const float inv = 1.0f / a.scale;
         float v[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) v[u] = rp_table(a, bk[u], h);
+        for (int u = 0; u < 2; ++u) v[u] = rp_entry(a, bk[u], h);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
             if (tid + 256 * u < n) tab[tid + 256 * u] = v[u] * inv;
-        for (int x = tid + 512; x < n; x += 256) tab[x] = rp_table(a, map(a, x), h) * inv;
+        for (int x = tid + 512; x < n; x += 256) tab[x] = rp_entry(a, map(a, x), h) * inv;
     }
 };
 // zero rows [0, lead) and [end, T) of a packed tensor: `which` of `nwg` workgroups

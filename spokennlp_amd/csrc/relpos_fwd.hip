@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
 #pragma unroll
         for (int kk = 0; kk < Ti::KB; ++kk) fq[kk] = Ti::gfrag(qrow, kk, g, a.D, col_ok);
     }
-    const float c2 = a.scale * RP_LOG2E, farL = rp_table(a, a.map[0], h) * RP_LOG2E, farR = rp_table(a, a.map[2 * a.span], h) * RP_LOG2E;
+    const float c2 = a.scale * RP_LOG2E, farL = rp_entry(a, a.map[0], h) * RP_LOG2E, farR = rp_entry(a, a.map[2 * a.span], h) * RP_LOG2E;
     if (keys.m || sq.kn % 64 || a.D != DT * 16) {
 #pragma unroll
         for (int n = 0; n < Ti::BYTES / 1024; ++n) *reinterpret_cast<uint4*>(tV + n * 1024 + l * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[f][r] = rp_table(a, bk[f][r], h) * inv;
+                for (int r = 0; r < 4; ++r) z[f][r] = rp_entry(a, bk[f][r], h) * inv;
         } else
 #pragma unroll
             for (int f = 0; f < 4; ++f) z[f] = (f32x4){0.f, 0.f, 0.f, 0.f};

@@ -1,0 +1,94 @@
+"""Attention under a learned relative position bias where calls are at the edge of what the documentation allows, on a real MI355X.  The oracle and the
+tolerances are those of test_gpu_relpos.py unless a test says otherwise."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_relpos import F64, TOL, _ops, check, make, rel
+
+pytestmark = pytest.mark.gpu
+
+
+def passes(q, k, v, table, lut, dout, **how):
+    """forward and backward: out, lse, dq, dk, dv, dtable"""
+    ops = _ops()
+    out, lse = ops.relpos_attn_fwd(q, k, v, table, lut, **how)
+    return (out, lse) + ops.relpos_attn_bwd(q, k, v, table, lut, out, dout, lse, **how)
+
+
+# ---- finite table entries of any size
+# What |s| ~ 2^15 costs: the entry over the scale, the sums of the products on top of it, lse and its product with log2 e are rounded to 24 bits there, half a step
+# of [2^14, 2^15) is 2^-10, at most eight of them (four products of 32 at D <= 128, or one addition in fp32, and four others) reach the exponent: e^(8 * 2^-10) - 1
+FAR_TOL = 8 * 2.0 ** -10
+
+
+def one_key(out, v):
+    """a row with all of its probability on one key: e v / e with e near 1 rounded where it is summed, 1 / e and two products: four roundings of the row's v in fp32;
+    in bf16 e is rounded too, but the sum 1 / e is taken of is not: one of 2^-8 more (and the output's own)"""
+    tol = 4 * 2.0 ** -24 if out.dtype == torch.float32 else 2 * 2.0 ** -8
+    return bool(((out.to(F64) - v.to(F64)).abs() <= tol * v.to(F64).abs()).all())
+
+
+def ref_shifted(q, k, v, table, lut, seen, causal, dout):
+    """ref_attention with each row's largest visible entry taken off first: the same softmax, and 64 bits then hold the products beside entries of any size"""
+    span = lut.numel() // 2
+    q, k, v, table = (x.detach().to(F64).requires_grad_() for x in (q, k, v, table))
+    r = torch.arange(k.shape[0], device=q.device)[None] - torch.arange(q.shape[0], device=q.device)[:, None]
+    b = table[lut.long()[r.clamp(-span, span) + span]].permute(2, 0, 1)
+    vis = seen[None] & (r <= 0) if causal else seen[None].expand_as(r)
+    top = b.detach().masked_fill(~vis[None], -math.inf).amax(-1, keepdim=True)
+    top = torch.where(torch.isfinite(top), top, torch.zeros_like(top))
+    s = torch.einsum("ihd,jhd->hij", q, k) * q.shape[-1] ** -0.5 + (b - top)
+    blind = ~vis.any(1)
+    p = torch.softmax(s.masked_fill(~vis[None], -math.inf).masked_fill(blind[None, :, None], 0.0), -1) * (~blind)[None, :, None]
+    out = torch.einsum("hij,jhd->ihd", p, v)
+    return [out.detach()] + list(torch.autograd.grad(out, (q, k, v, table), dout.to(F64)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("entry", ["lowest", "lowest_bf16", -1e30, -1e9, -1e4, 1e4, 1e9, "highest_bf16", "highest"])
+@pytest.mark.parametrize("where", ["near", "far"])
+def test_finite_table_entries_of_any_size(dev, dtype, entry, where):
+    """a bucket at the types' lowest (highest) value: it loses against (wins over) every other one, and a row that sees nothing else has the softmax over it, with
+    its gradients.  near: the bucket of distance 0, under a causal mask (row 0 sees nothing else); far: the last bucket to the left, most rows see
+    nothing else"""
+    print("CASE", dtype, entry, where, flush=True)
+    x = {"lowest": torch.finfo(torch.float32).min, "lowest_bf16": torch.finfo(torch.bfloat16).min, "highest": torch.finfo(torch.float32).max,
+         "highest_bf16": torch.finfo(torch.bfloat16).max}.get(entry, entry)
+    causal = where == "near"
+    q, k, v, table, lut, dout = make(dev, dtype, 1, 200, 200, 2, 2, 64, buckets=8, max_distance=48, bidirectional=not causal)
+    table = table.float()
+    seen = torch.ones(200, dtype=torch.bool, device=dev)
+    if causal:
+        table[0] = x
+        if x > 0:
+            table[3] = x                                     # (two buckets that win: both are seen by most rows)
+    else:
+        table[int(lut[0])] = x
+        seen[30:] = False
+    got = passes(q, k, v, table, lut, dout, causal=causal, key_mask=seen[None])
+    assert all(bool(torch.isfinite(y).all()) for y in got)
+    want = ref_shifted(q[0], k[0], v[0], table, lut, seen, causal, dout[0])
+    err = dict(out=rel(got[0][0], want[0]), dq=rel(got[2][0], want[1]), dk=rel(got[3][0], want[2]), dv=rel(got[4][0], want[3]))
+    # dtable: a row whose probability is all in one bucket gives it sum_j ds_ij = 0 in exact arithmetic; relative to the summands' size (test_any_map)
+    mass = 2 * 200 * float(dout.float().norm(dim=-1).max()) * float(v.float().norm(dim=-1).max())
+    err["dtable"] = float((got[5].to(F64) - want[4]).abs().max()) / mass
+    print(err, flush=True)
+    assert max(err.values()) < TOL[dtype] + FAR_TOL, err
+    if causal and x < 0:
+        assert one_key(got[0][0, 0], v[0, 0])
+    # a module's dense bias has the entry itself
+    assert torch.equal(_ops().relpos_bias_fwd(table, lut, 3, 3)[0, 2, 2], table[int(lut[48]), 0])
+
+
+def test_finite_table_entries_keep_their_order(dev):
+    """of buckets at unlike huge values the largest takes the row"""
+    q, k, v, _, _, _ = make(dev, torch.float32, 1, 40, 40, 1, 1, 64)
+    lut = torch.tensor([0] * 39 + [1] + [2] * 39, dtype=torch.int32, device=dev)          # left, itself, right
+    levels = [torch.finfo(torch.float32).min, -1e38, -4e37, -1e30, -1e9, -2e5, -1e5, -1e4, 0.0, 1e4, 3e4, 1e9, 1e30, 4e37, 1e38, torch.finfo(torch.float32).max]
+    for lo, hi in zip(levels, levels[1:]):
+        table = torch.tensor([[lo], [hi], [lo]], dtype=torch.float32, device=dev)
+        out, lse = _ops().relpos_attn_fwd(q, k, v, table, lut)
+        assert one_key(out, v), (lo, hi)
+        assert bool(torch.isfinite(lse).all())
