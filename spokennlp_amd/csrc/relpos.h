@@ -57,6 +57,8 @@ __device__ __forceinline__ RpSeq rp_seq(const RpArgs& a, int b) {
     s.off = a.align_end ? s.kn - s.qn : 0;
     return s;
 }
+// the first `n` keys of a sequence are all that its query rows before `rows` may see
+__device__ __forceinline__ int rp_seen(const RpArgs& a, const RpSeq& s, int rows) { return a.causal ? rp_clamp(min(rows, s.qn) + s.off, 0, s.kn) : s.kn; }
 // index of (sequence b, head h, row i) in lse / delta
 __device__ __forceinline__ int64_t rp_row(const RpArgs& a, const RpSeq& s, int b, int h, int i) {
     return a.cu_q ? (int64_t)h * a.Tq + s.q0 + i : ((int64_t)b * a.heads + h) * a.Lq + i;
@@ -170,8 +172,8 @@ template <typename T, int DT> constexpr int rp_nb = DT * sizeof(T) >= 32 ? 1 : 2
 
 // 64 rows of a tensor global -> LDS by the DMA path, 1 KiB a wave and instruction, no register in between.  The swizzle sits on the global side (lane l
 // fetches what its fixed LDS slot holds).  Rows whose bit is clear and columns from D on are not fetched: their places keep what they held -- the zeros of
-// rp_clear_lds or a visible row of an earlier chunk -- so what stands in hidden rows (infinities, NaN) reaches no product, and a probability of exactly 0 meets
-// a finite number.
+// rp_clear_own or a visible row of an earlier chunk -- so what stands in hidden rows (infinities, NaN) reaches no product, and a probability of exactly 0 meets
+// a finite number.  (A key that `causal` hides from a part of a workgroup's rows is fetched.)
 template <typename T, int DT> struct RpStage {
     typedef RpTile<T, DT> Ti;
     static constexpr int N = Ti::BYTES / 4096;              // pieces of a wave
@@ -237,7 +239,7 @@ __device__ __forceinline__ uint64_t rp_low_bits(int n) { return n >= 64 ? ~0ull 
 
 // visible keys of a 64-key chunk as a wave-uniform word.  A key mask is turned into words in LDS by the workgroup before its first chunk (the chunk loop
 // then has no load of its own whose wait would drain the chunks under way); only chunks beyond RP_MASK_WORDS (or a packed batch's hint) are looked up as
-// they come.
+// they come.  `kn`: the keys that may be seen at all, of the sequence or (upto) of the rows at hand.
 #define RP_MASK_WORDS 1024
 struct RpKeys {
     const uint8_t* m; const uint64_t* words; int kn, lane, nw;
@@ -245,6 +247,7 @@ struct RpKeys {
         m = a.key_mask ? a.key_mask + (a.cu_k ? (int64_t)s.k0 : (int64_t)b * a.mask_sb) : nullptr;
         words = lds; kn = s.kn; lane = lane_; nw = a.mask_words;
     }
+    __device__ __forceinline__ int upto(int n) { kn = n; return (n + 63) / 64; }       // -> chunks that hold them
     __device__ __forceinline__ uint64_t look(int c) const { const int key = c * 64 + lane; return __ballot(key < kn && m[key] != 0); }
     __device__ __forceinline__ void build(uint64_t* lds, int w) const {       // (only with a mask; a barrier follows)
         const int n = min((kn + 63) / 64, nw);
@@ -260,10 +263,12 @@ struct RpKeys {
         }
     }
     __device__ __forceinline__ uint64_t bits(int c) const {
-        if (!m) return rp_low_bits(kn - c * 64);
+        const uint64_t low = rp_low_bits(kn - c * 64);
+        if (!m) return low;
         if (c >= nw) return look(c);
         const uint64_t x = words[c];
-        return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)), lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
+        return low & (((uint64_t)hi << 32) | lo);
     }
     // the next chunk from c on that holds a visible key
     __device__ __forceinline__ int seek(int c, int c_end, uint64_t& w) const {

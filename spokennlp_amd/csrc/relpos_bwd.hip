@@ -66,12 +66,7 @@ __device__ __forceinline__ float rp_join4(float x0, float x1, float x2, float x3
 
 // keys that the 128-row block of row q0 may see, in whole chunks (the same for either QT: a row's bits must not depend on the grid)
 __device__ __forceinline__ bool rp_fine(const RpArgs& a, const RpSeq& sq, int q0) {
-    int c = (sq.kn + 63) / 64;
-    if (a.causal) {
-        const int last = min(q0 / 128 * 128 + 128, sq.qn) - 1 + sq.off;
-        c = last < 0 ? 0 : min(c, last / 64 + 1);
-    }
-    return c * 64 <= RP_FINE || sq.qn <= RP_FINE / 2;
+    return (rp_seen(a, sq, q0 / 128 * 128 + 128) + 63) / 64 * 64 <= RP_FINE || sq.qn <= RP_FINE / 2;
 }
 
 // MIXED: row blocks may be FINE, or the keys are split (an instance of its own: what only these need costs the plain one 5 % at 4 x 4096 by its registers)
@@ -102,7 +97,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
     RpKeys keys;
     keys.init(a, sq, b, l, words);
-    if (keys.m || sq.kn % 64 || a.D != DT * 16)             // (something of a chunk is not fetched)
+    if (keys.m || a.causal || sq.kn % 64 || a.D != DT * 16) // (something of a chunk is not fetched)
         for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
     rp_cleared();
     if (keys.m) { keys.build(words, w); __syncthreads(); }
@@ -119,12 +114,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         constexpr int QT = decltype(qt_)::value, BQ = 64 * QT;
         constexpr bool FINE = decltype(fine_)::value;
         const int qw = q0 + w * 16 * QT;
-        int c_end = (sq.kn + 63) / 64;
-        if (causal) {
-            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;
-            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
-        }
-        int c_from = 0;
+        int c_from = 0, c_end = keys.upto(rp_seen(a, sq, q0 + BQ));
         if (MIXED && nsplit > 1) { c_from = split * (a.split_keys / 64); c_end = min(c_end, c_from + a.split_keys / 64); }
         typename Ti::frag fq[QT][Ti::KB], fdo[QT][Ti::KB];
         float nl[QT], rsum[QT];                             // -lse in the exponent's units; sum of a row's ds (each of its four lanes: a quarter of the keys)
@@ -373,7 +363,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int key = kw + ct * 16 + i16;
-            const bool in = key < sq.kn;
+            const bool in = key < rp_seen(a, sq, sq.qn);
             const int64_t kt = (int64_t)(sq.k0 + key);
             seen[ct] = in && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
 #pragma unroll

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     rk.init(a.sk.st, a.D, w, l); rv.init(a.sv.st, a.D, w, l);
     RpKeys keys;
     keys.init(a, sq, b, l, words);
-    if (keys.m || sq.kn % 64 || a.D != DT * 16)             // (something of a chunk is not fetched)
+    if (keys.m || a.causal || sq.kn % 64 || a.D != DT * 16) // (something of a chunk is not fetched)
         for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
     rp_cleared();
     if (keys.m) { keys.build(words, w); __syncthreads(); }
@@ -56,11 +56,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
 
     for (; rb * BQ < sq.qn; rb += a.nrb) {
         const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
-        int c = 0, c_end = (sq.kn + 63) / 64;
-        if (causal) {
-            const int last = min(q0 + BQ, sq.qn) - 1 + sq.off;                  // the last key any row of the block sees
-            c_end = last < 0 ? 0 : min(c_end, last / 64 + 1);
-        }
+        int c = 0, c_end = keys.upto(rp_seen(a, sq, q0 + BQ));
         if (a.nsplit > 1) { c = split * (a.split_keys / 64); c_end = min(c_end, c + a.split_keys / 64); }
         auto fetch = [&](int at, int buf, uint64_t bits) {
             rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
@@ -230,8 +226,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
     keys.init(a, sq, b, l, nullptr);
     keys.nw = 0;                                            // (the mask as it comes: a wave sees two or three chunks of it)
     const bool causal = a.causal;
-    int c_end = (sq.kn + 63) / 64;
-    if (causal) c_end = sq.kn <= 0 || a.Lq - 1 + sq.off < 0 ? 0 : min(c_end, (a.Lq - 1 + sq.off) / 64 + 1);
+    int c_end = keys.upto(rp_seen(a, sq, a.Lq));
     const int c0 = split * (a.split_keys / 64);
     c_end = a.nsplit > 1 ? min(c_end, c0 + a.split_keys / 64) : c_end;
     typename Ti::frag fq[Ti::KB];
@@ -241,7 +236,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
         for (int kk = 0; kk < Ti::KB; ++kk) fq[kk] = Ti::gfrag(qrow, kk, g, a.D, col_ok);
     }
     const float c2 = a.scale * RP_LOG2E, farL = rp_entry(a, a.map[0], h) * RP_LOG2E, farR = rp_entry(a, a.map[2 * a.span], h) * RP_LOG2E;
-    if (keys.m || sq.kn % 64 || a.D != DT * 16) {
+    if (keys.m || keys.kn % 64 || a.D != DT * 16) {
 #pragma unroll
         for (int n = 0; n < Ti::BYTES / 1024; ++n) *reinterpret_cast<uint4*>(tV + n * 1024 + l * 16) = make_uint4(0u, 0u, 0u, 0u);
         rp_cleared();

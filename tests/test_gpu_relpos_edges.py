@@ -92,3 +92,46 @@ def test_finite_table_entries_keep_their_order(dev):
         out, lse = _ops().relpos_attn_fwd(q, k, v, table, lut)
         assert one_key(out, v), (lo, hi)
         assert bool(torch.isfinite(lse).all())
+
+
+# ---- keys that no row sees
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(2, 100, 333, 4, 2, 64), (1, 1, 700, 8, 2, 128), (2, 3, 2100, 4, 2, 64), (2, 90, 2100, 2, 2, 40), (1, 300, 420, 2, 2, 128),
+                                   (1, 128, 129, 12, 12, 64), (1, 1, 2, 1, 1, 8)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_keys_behind_the_last_query_are_not_used(dev, dtype, shape, bad):
+    """a causal pass over the first Lq places of longer K / V buffers whose rest was never written: the same bits as with finite rows there, their gradients zero"""
+    print("CASE", dtype, shape, bad, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, table, lut, dout = make(dev, dtype, *shape, bidirectional=False)
+    clean = check(dev, q, k, v, table, lut, dout, causal=True) if Lq > 1 else passes(q, k, v, table, lut, dout, causal=True)
+    kb, vb = k.clone(), v.clone()
+    kb[:, Lq:], vb[:, Lq:] = bad, bad
+    for x, y in zip(passes(q, kb, vb, table, lut, dout, causal=True), clean):
+        assert torch.equal(x, y)
+    assert not clean[3][:, Lq:].any() and not clean[4][:, Lq:].any()
+    # the same with a key mask, and packed with more keys than queries
+    m = torch.rand(B, Lk, generator=torch.Generator().manual_seed(3)).to(dev) < 0.8
+    m[:, 0] = True
+    a, b = passes(q, k, v, table, lut, dout, causal=True, key_mask=m), passes(q, kb, vb, table, lut, dout, causal=True, key_mask=m)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    cq = torch.arange(B + 1, dtype=torch.int32, device=dev) * Lq
+    ck = torch.arange(B + 1, dtype=torch.int32, device=dev) * Lk
+    flat = [x.flatten(0, 1) for x in (q, k, v, dout)], [x.flatten(0, 1) for x in (q, kb, vb, dout)]
+    a, b = (passes(*x[:3], table, lut, x[3], causal=True, cu_q=cq, cu_k=ck) for x in flat)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 300, 310, 2, 2, 64), (1, 640, 670, 48, 48, 64), (2, 300, 399, 4, 2, 128)])
+def test_rows_of_a_block_take_nothing_from_keys_behind_it(dev, dtype, shape):
+    """causal with the last query at the last key: NaN in keys behind what a block of 128 rows sees leaves those rows as they were"""
+    print("CASE", dtype, shape, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, table, lut, dout = make(dev, dtype, *shape, bidirectional=False)
+    a = passes(q, k, v, table, lut, dout, causal=True, align_end=True)
+    kb, vb = k.clone(), v.clone()
+    kb[:, 128 + Lk - Lq:], vb[:, 128 + Lk - Lq:] = math.nan, math.nan
+    b = passes(q, kb, vb, table, lut, dout, causal=True, align_end=True)
+    for x, y in zip((a[0][:, :128], a[1][:, :, :128], a[2][:, :128]), (b[0][:, :128], b[1][:, :, :128], b[2][:, :128])):
+        assert torch.equal(x, y)
