@@ -413,7 +413,7 @@ int amdseg_heads_bwd_rows(const float* gout, const float* x, int M, int H, float
  *   s_ij = scale q_i . k_j + table[map[clamp(rel, -span, span) + span], head],   rel = j - (i + off),   off = 0 or (align_end) keys - queries of the sequence
  *   p_ij = softmax over the visible keys;  out_i = sum_j p_ij v_j;  lse_i = log sum_j exp(s_ij)
  * Key j is visible from query i iff j < keys of the sequence, key_mask (optional, 0 = hidden) allows it and, with `causal`, rel <= 0.  A row without a
- * visible key: out = 0, lse = -inf, no gradient.  K / V rows of keys that no query row of the sequence sees (behind its
+ * visible key: out = 0, lse = -inf, no gradient, whatever q and dout hold there.  K / V rows of keys that no query row of the sequence sees (behind its
  * keys, masked, under `causal` behind its last query) are never used, whatever they hold.  A key that `causal` hides from earlier rows only is data of the
  * later ones and has to be finite: an infinity or NaN in it may reach the rows of up to 128 before it.
  * Finite table entries may have any size: t beyond +-2^14 enters the scores as +-(2^14 + 128 log2(|t| / 2^14)) -- of two such buckets the larger still takes the

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
         if (!first) __syncthreads();                    // (nobody is left in the buffers)
         if (NB == 2 && c < c_end) fetch(c, 0, bits);    // on its way before anything else is waited for
         typename Ti::frag fo[QT][Ti::KB];
-        float lse[QT];                              // a row outside, or one that saw no key (lse = -inf): p = exp(s - inf) = 0
+        float lse[QT];                              // a row outside, or one that saw no key: -inf, and nl = -inf gives p = 0
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
             const int q = qw + ct * 16 + i16;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                 fdo[ct][kk] = Ti::gfrag((const T*)a.dout + b * a.sdo.sb + qt * a.sdo.st + h * a.sdo.sh, kk, g, a.D, ok);
                 fo[ct][kk] = Ti::gfrag((const T*)a.o + b * a.so.sb + qt * a.so.st + h * a.so.sh, kk, g, a.D, ok);
             }
-            lse[ct] = ok ? a.lse[rp_row(a, sq, b, h, q)] : INFINITY;
+            lse[ct] = ok ? a.lse[rp_row(a, sq, b, h, q)] : -INFINITY;
         }
         if (first) table.finish(a, tab, h);
 #pragma unroll
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             acc += __shfl_xor(acc, 16, 64);
             acc += __shfl_xor(acc, 32, 64);
             nd[ct] = (f32x4){-acc, -acc, -acc, -acc};
-            nl[ct] = lse[ct] == -INFINITY ? -INFINITY : -lse[ct] * RP_LOG2E;
+            nl[ct] = lse[ct] == -INFINITY ? -INFINITY : lse[ct] == INFINITY ? NAN : -lse[ct] * RP_LOG2E;
         }
         first = false;
         auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
@@ -258,22 +258,25 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
             const int q = qw + ct * 16 + i16;
             if (q >= sq.qn) continue;
             const int64_t row = rp_row(a, sq, b, h, q);
+            const bool blind = nl[ct] == -INFINITY;         // no key: no gradient, whatever dout holds there
+            const float ndq = blind ? 0.f : nd[ct][0], rs = blind ? 0.f : rsum[ct];
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
             if (MIXED && nsplit > 1) {                      // rp_join_q_kernel adds them up
                 float* op = a.part_q + (split * rows + row) * a.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
-                    if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(op + d * 16 + g * 4) = dq[ct][d] * a.scale;
+                    if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(op + d * 16 + g * 4) = blind ? zero : dq[ct][d] * a.scale;
                 if (g == 0) {
-                    a.part_q[nsplit * rows * a.D + split * rows + row] = rsum[ct];
-                    if (split == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = nd[ct][0]; }
+                    a.part_q[nsplit * rows * a.D + split * rows + row] = rs;
+                    if (split == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = ndq; }
                 }
                 continue;
             }
-            if (g == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = nd[ct][0] - rsum[ct]; }
+            if (g == 0) { a.stat[row] = nl[ct]; a.stat[rows + row] = ndq - rs; }
             T* op = (T*)a.dq + b * a.sdq.sb + (int64_t)(sq.q0 + q) * a.sdq.st + h * a.sdq.sh;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, dq[ct][d] * a.scale);
+                if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, blind ? zero : dq[ct][d] * a.scale);
         }
     };
     for (; rb * BQ_ < sq.qn; rb += a.nrb) {
@@ -323,7 +326,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     table.start(a, -1, tid);
     RpStage<T, DT> rq, ro;
     rq.init(a.sq.st, a.D, w, l); ro.init(a.sdo.st, a.D, w, l);
-    if (sq.qn % 64 || a.D != DT * 16) {                     // (something of a chunk is not fetched)
+    if (a.causal || sq.qn % 64 || a.D != DT * 16) {         // (something of a chunk is not fetched)
         for (int t = 0; t < 2 * NB; ++t) rp_clear_own<T, DT>(smem + t * Ti::BYTES, w, l);
         if (w == 0)
             for (int x = l; x < NB * 128; x += 64) rows[x] = 0.f;
@@ -334,13 +337,23 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
 
     for (; rb * BK < rows_k; rb += a.nrb) {
         const int k0 = rb * BK, kw = k0 + w * 16 * QT;
-        int c_first = 0, n_ch = (sq.qn + 63) / 64;
-        if (causal) c_first = max(0, k0 - sq.off) / 64;     // query rows before k0 - off see none of these keys
+        int c_first = 0, n_ch = (sq.qn + 63) / 64, r_first = 0;
+        if (causal) {                                       // query rows before r_first see none of these keys, and nothing of them is used
+            int kf = k0;
+            if (a.key_mask) {
+                const uint8_t* m = a.key_mask + (a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb);
+                uint64_t vis = 0;
+                for (; kf < min(k0 + BK, sq.kn) && !(vis = __ballot(kf + l < sq.kn && m[kf + l] != 0)); kf += 64) {}
+                kf += vis ? __builtin_ctzll(vis) : 0;
+            }
+            r_first = max(0, kf - sq.off);
+            c_first = r_first / 64;
+        }
         if (CUT && qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
         const T *qb, *ob;
         const float* stat_h;
         auto fetch = [&](int c, int buf) {
-            const uint64_t ok = rp_low_bits(sq.qn - c * 64);
+            const uint64_t ok = rp_low_bits(sq.qn - c * 64) & ~rp_low_bits(r_first - c * 64);
             rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + buf * 2 * Ti::BYTES, w, l);
             ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
             if (w == 0 && ((ok >> l) & 1)) {                // 64 rows' stat: 4 bytes a lane

@@ -135,3 +135,34 @@ def test_rows_of_a_block_take_nothing_from_keys_behind_it(dev, dtype, shape):
     b = passes(q, kb, vb, table, lut, dout, causal=True, align_end=True)
     for x, y in zip((a[0][:, :128], a[1][:, :, :128], a[2][:, :128]), (b[0][:, :128], b[1][:, :, :128], b[2][:, :128])):
         assert torch.equal(x, y)
+
+
+# ---- rows that see no key
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(3, 300, 300, 4, 2, 64), (2, 200, 90, 2, 2, 128), (2, 1500, 100, 4, 2, 64), (3, 40, 2100, 4, 4, 32), (3, 9, 700, 2, 2, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_the_gradient_of_a_row_without_a_key_is_not_used(dev, dtype, shape, bad):
+    """causal with the first keys hidden, and more queries than keys ending together: rows without a key have q and dout of any value and give no gradient"""
+    print("CASE", dtype, shape, bad, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    q, k, v, table, lut, dout = make(dev, dtype, *shape, bidirectional=False)
+    m = torch.ones(B, Lk, dtype=torch.bool, device=dev)
+    first = [0, 37, 70, 5][:B] if Lk > 90 else [0, 21]
+    for b, n in enumerate(first):
+        m[b, :n] = False
+    if B == 3:
+        m[2] = False                                         # (a sequence of no keys at all)
+    how = dict(causal=True, align_end=True, key_mask=m)
+    a = passes(q, k, v, table, lut, dout, **how)
+    empty = (a[1] == -math.inf).all(1)                       # [B, Lq]
+    assert empty.any() and not empty.all()
+    qb, db = q.clone(), dout.clone()
+    qb[empty], db[empty] = bad, bad
+    b = passes(qb, k, v, table, lut, db, **how)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    assert not b[2][empty].any()
+    cq, ck = (torch.arange(B + 1, dtype=torch.int32, device=dev) * n for n in (Lq, Lk))
+    how = dict(causal=True, align_end=True, key_mask=m.flatten(), cu_q=cq, cu_k=ck)
+    a, b = (passes(x.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), table, lut, y.flatten(0, 1), **how) for x, y in ((q, dout), (qb, db)))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
