@@ -14,7 +14,7 @@
 #include "common.h"
 #include "tile64.h"
 
-#define RP_PAD 112              // 63 (tile rows) + 32 (columns of a wave) + 15 lanes of the gradient's diagonal registers
+#define RP_PAD 112              // 63 (tile rows) + 32 (columns of a wave, or of rp_near's group) + 15 lanes of the gradient's diagonal registers
 #define RP_MAX_SPAN 1024
 #define RP_MAX_WGS ((1 << 24) - 1)   // a grid has less than 2^32 threads
 #define RP_LOG2E 1.4426950408889634f
@@ -216,6 +216,16 @@ __device__ __forceinline__ void rp_clear_own(char* tile, int w, int l) {
 }
 __device__ __forceinline__ void rp_cleared() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void rp_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); __syncthreads(); }
+
+// has a wave's chunk some |rel| < span (its scores start from the table) or none (from 0, the constant joins in the exponent)?  The two round differently, so in
+// bf16 the 32 rows around the wave's decide, whether it has 16 of them or all: a row's bits do not follow the tiles that a grid chooses.
+// `rel0` = rel of the chunk's first key and the wave's first query, which is row `qw`; RP_PAD covers the reach of the group's other half
+template <typename T>
+__device__ __forceinline__ bool rp_near(int rel0, int qw, int span) {
+    constexpr int G = sizeof(T) == 2 ? 32 : 16;
+    const int first = rel0 + (qw & (G - 1));                // ... and the group's first query
+    return first + 63 > -span && first - (G - 1) < span;
+}
 
 // the bias values of the score tiles whose block diagonal (row tile - column tile) is k0, k0 + 1, ...: lane (g, i16), register r = rel 16 k + 4 g + r - i16
 // (or `far`, where the whole tile is beyond the span)

@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
             buf ^= NB - 1;
             if (NB == 2 && c < c_end) fetch(c, buf, bits);
             if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
-            const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+            const bool near = rp_near<T>(rel0, qw, span);
             chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
         }
 #pragma unroll

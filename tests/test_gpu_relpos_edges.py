@@ -166,3 +166,29 @@ def test_the_gradient_of_a_row_without_a_key_is_not_used(dev, dtype, shape, bad)
     how = dict(causal=True, align_end=True, key_mask=m.flatten(), cu_q=cq, cu_k=ck)
     a, b = (passes(x.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), table, lut, y.flatten(0, 1), **how) for x, y in ((q, dout), (qb, db)))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---- the same bits in any batch
+@pytest.mark.parametrize("span", [9, 48, 128, 200])
+@pytest.mark.parametrize("extra", [0, 10, 33])
+@pytest.mark.parametrize("D", [64, 40, 96])
+def test_bits_do_not_follow_the_batch(dev, span, extra, D):
+    """a sequence alone (16 query rows a wave) and among 24 (32 rows a wave), whole and packed with hints of any size; spans and offsets that are no multiple of
+    a tile"""
+    print("CASE", span, extra, D, flush=True)
+    L = 400
+    q, k, v, table, lut, dout = make(dev, torch.bfloat16, 24, L, L + extra, 12, 12, D, buckets=8, max_distance=span)
+    for causal in (False, True):
+        how = dict(causal=causal, align_end=True)
+        a = passes(q, k, v, table, lut, dout, **how)
+        for b in (0, 5):
+            one = passes(q[b:b + 1], k[b:b + 1], v[b:b + 1], table, lut, dout[b:b + 1], **how)
+            for n in range(5):
+                assert torch.equal(one[n][0], a[n][b]), (causal, n)
+    cq, ck = (torch.arange(25, dtype=torch.int32, device=dev) * n for n in (L, L + extra))
+    flat = [x.flatten(0, 1) for x in (q, k, v)]
+    for hint in (None, L + extra, 1):
+        p = passes(*flat, table, lut, dout.flatten(0, 1), cu_q=cq, cu_k=ck, max_q=hint, max_k=hint, **how)
+        assert torch.equal(p[0], a[0].flatten(0, 1)) and torch.equal(p[1], a[1].transpose(0, 1).flatten(1)), hint
+        for n in (2, 3, 4):
+            assert torch.equal(p[n], a[n].flatten(0, 1)), (hint, n)
