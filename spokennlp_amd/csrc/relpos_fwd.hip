@@ -216,7 +216,8 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float ml[4][16][2];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int split = blockIdx.x, b = blockIdx.y / a.kv_heads, hk = blockIdx.y % a.kv_heads;
+    const int split = blockIdx.x, pair = blockIdx.z * gridDim.y + blockIdx.y, b = pair / a.kv_heads, hk = pair % a.kv_heads;
+    if (b >= a.B) return;
     const int G = a.heads / a.kv_heads;
     const RpSeq sq = rp_seq(a, b);
     char* tV = smem + w * Ti::BYTES;
@@ -416,7 +417,9 @@ static int rp_few_launch(const RpArgs& a, hipStream_t s) {
     const int lds = 4 * RpTile<T, DT>::BYTES;
     const int rc = rp_allow_lds((const void*)rp_few_kernel<T, DT>, lds);
     if (rc) return rc;
-    hipLaunchKernelGGL((rp_few_kernel<T, DT>), dim3(a.nsplit, a.B * a.kv_heads), dim3(256), lds, s, a);
+    const int64_t pairs = (int64_t)a.B * a.kv_heads, y = std::min<int64_t>(pairs, 65535), z = (pairs + 65534) / 65535;
+    if (z > 4096) return AMDSEG_ERR_SHAPE;                  // (pair numbers stay below 2^28)
+    hipLaunchKernelGGL((rp_few_kernel<T, DT>), dim3(a.nsplit, (unsigned)y, (unsigned)z), dim3(256), lds, s, a);
     return amdseg_launch_status();
 }
 template <typename T>

@@ -44,9 +44,9 @@ static inline int rp_dkv_parts(const RpArgs& a, int kt, int qsplit) {
 // dK / dV of few keys against many query rows: the walk is cut every RP_SPLIT_ROWS (forward + backward, 11 x 3949 rows x 5 keys: 148 -> 79 us).  Shapes alone decide.
 #define RP_SPLIT_ROWS 1024
 static inline int rp_qsplit(const RpArgs& a) { return !a.cu_q && a.Lk <= 128 && a.Lq > RP_SPLIT_ROWS ? (a.Lq + RP_SPLIT_ROWS - 1) / RP_SPLIT_ROWS : 1; }
-// the rows of a kv head's query heads fit the 16 columns of one tile
+// the rows of a kv head's query heads fit the 16 columns of one tile (shapes of a sequence alone: its bits must not follow the batch)
 static inline bool rp_few(const RpArgs& a) {
-    return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16 && (int64_t)a.B * a.kv_heads <= 65535;
+    return !a.cu_q && (int64_t)(a.heads / a.kv_heads) * a.Lq <= 16;
 }
 // splits over the keys: few query rows against many keys (single tokens, a handful of rows against a cache), joined by rp_join_kernel.  A number of keys that
 // the shapes alone decide: a sequence's sums do not depend on the batch around it.  (3 x 47 rows of 4 heads against 4545 keys, fp32: 449 -> 148 us; dQ is split

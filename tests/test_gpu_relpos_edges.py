@@ -192,3 +192,13 @@ def test_bits_do_not_follow_the_batch(dev, span, extra, D):
         assert torch.equal(p[0], a[0].flatten(0, 1)) and torch.equal(p[1], a[1].transpose(0, 1).flatten(1)), hint
         for n in (2, 3, 4):
             assert torch.equal(p[n], a[n].flatten(0, 1)), (hint, n)
+
+
+def test_bits_of_single_tokens_in_a_batch_of_any_size(dev):
+    """single tokens of more (sequence, kv head) pairs than a grid's second dimension holds"""
+    B, H, Hk, D = 16400, 8, 4, 16
+    q, k, v, table, lut, _ = make(dev, torch.bfloat16, B, 1, 70, H, Hk, D, buckets=8, max_distance=48)
+    out, lse = _ops().relpos_attn_fwd(q, k, v, table, lut, align_end=True)
+    for s in (slice(0, 50), slice(8000, 8060), slice(B - 50, B)):
+        o, l = _ops().relpos_attn_fwd(q[s], k[s], v[s], table, lut, align_end=True)
+        assert torch.equal(o, out[s]) and torch.equal(l, lse[s])
