@@ -22,6 +22,14 @@ def _rows_ok(t):
         (t.dim() < 4 or t.shape[0] == 1 or t.stride(0) * es % 16 == 0) and t.data_ptr() % 16 == 0
 
 
+def _rows(t):
+    """t as the kernels take it: a gradient may come with any strides, or contiguous from any element of a larger one (then contiguous() is t itself)"""
+    if _rows_ok(t):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _RelposAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, bucket_map, how):
@@ -34,9 +42,7 @@ class _RelposAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, table, bucket_map, out, lse, key_mask, k_lens, cu_q, cu_k = ctx.saved_tensors
-        if not _rows_ok(dout):
-            dout = dout.contiguous()
-        dq, dk, dv, dtable = ops.relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, need_dtable=ctx.needs_input_grad[3], key_mask=key_mask,
+        dq, dk, dv, dtable = ops.relpos_attn_bwd(q, k, v, table, bucket_map, out, _rows(dout), lse, need_dtable=ctx.needs_input_grad[3], key_mask=key_mask,
                                                  k_lens=k_lens, cu_q=cu_q, cu_k=cu_k, **ctx.how)
         return dq, dk, dv, dtable, None, None
 
@@ -63,12 +69,10 @@ class _RelposSelfAttention(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, table, bucket_map, out, lse, key_mask, cu_q, cu_k = ctx.saved_tensors
         q, k, v = _RelposSelfAttention._blocks(qkv, *ctx.heads)
-        if not _rows_ok(dout):
-            dout = dout.contiguous()
         # packed: the rows outside every sequence are left alone by the kernels, and their gradient is zero
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device) if cu_q is None else torch.zeros(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = _RelposSelfAttention._blocks(dqkv, *ctx.heads)
-        dtable = ops.relpos_attn_bwd(q, k, v, table, bucket_map, out, dout, lse, need_dtable=ctx.needs_input_grad[1], key_mask=key_mask, cu_q=cu_q, cu_k=cu_k,
+        dtable = ops.relpos_attn_bwd(q, k, v, table, bucket_map, out, _rows(dout), lse, need_dtable=ctx.needs_input_grad[1], key_mask=key_mask, cu_q=cu_q, cu_k=cu_k,
                                      dq=dq, dk=dk, dv=dv, **ctx.how)[3]
         return dqkv, dtable, None, None, None, None
 

@@ -202,3 +202,22 @@ def test_bits_of_single_tokens_in_a_batch_of_any_size(dev):
     for s in (slice(0, 50), slice(8000, 8060), slice(B - 50, B)):
         o, l = _ops().relpos_attn_fwd(q[s], k[s], v[s], table, lut, align_end=True)
         assert torch.equal(o, out[s]) and torch.equal(l, lse[s])
+
+
+# ---- gradients that torch hands on
+def test_gradients_that_start_anywhere(dev):
+    """dout as a slice of a larger contiguous gradient: contiguous, and on no 16 bytes"""
+    from spokennlp_amd import relpos as R
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v, table, lut, dout = make(dev, dtype, 2, 70, 70, 4, 2, 64, fused=True)
+        want = passes(q, k, v, table, lut, dout)
+        for pad in (1, 3, 7):
+            leaves = [x.clone().requires_grad_(True) for x in (q, k, v, table)]
+            y = torch.cat([torch.zeros(pad, dtype=dtype, device=dev), R.relpos_attention(*leaves, lut).flatten()])
+            y.backward(torch.cat([torch.ones(pad, dtype=dtype, device=dev), dout.flatten()]))
+            for x, g in zip(leaves, want[2:]):
+                assert torch.equal(x.grad, g)
+            qkv = torch.cat([x.flatten(-2) for x in (q, k, v)], -1).requires_grad_(True)
+            y = torch.cat([torch.zeros(pad, dtype=dtype, device=dev), R.relpos_self_attention(qkv, 4, table, lut, kv_heads=2).flatten()])
+            y.backward(torch.cat([torch.ones(pad, dtype=dtype, device=dev), dout.flatten()]))
+            assert torch.equal(qkv.grad, torch.cat([x.flatten(-2) for x in want[2:5]], -1))
