@@ -420,8 +420,9 @@ int amdseg_heads_bwd_rows(const float* gout, const float* x, int M, int H, float
  * row, and a row that sees only one has the softmax of scale q . k over it; lse is that of these scores, gradients are those of the formula.  An entry of -inf
  * hides its bucket's keys.
  * Padded form (cu_q == cu_k == NULL): B sequences of Lq query and Lk key rows; k_lens (optional, int32 [B]) = keys held of each (a cache).
- * Packed form: sequence b = rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. of k (int32 [B + 1], device); Tq, Tk = rows of the buffers, Lq, Lk = the longest
- * sequence (a launch hint: too small a value costs time, not rows).  Rows outside every sequence: written as zeros (lse -inf) with zero_tail, else left alone.
+ * Packed form: sequence b = rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. of k (int32 [B + 1], device); Tq, Tk = rows of the buffers, Lq, Lk >= 1 =
+ * the longest sequence (a hint: Lk says how much of a key mask is held in LDS; no value changes a result, or what a call launches or needs as ws, which grow
+ * with rows + sequences).  Rows outside every sequence: written as zeros (lse -inf) with zero_tail, else left alone.
  * Values of cu_* / k_lens / map out of range are clamped on the device: wrong rows, never an access outside the buffers.
  * Strides are in elements, {sequence, row, head}, the last dimension contiguous; rows start on 16 bytes (pointers and strides).  heads a multiple of
  * kv_heads (each kv head serves heads / kv_heads query heads), D % 8 == 0, D <= 128, span <= 1024.  dtype: AMDSEG_BF16 or AMDSEG_F32 (products of

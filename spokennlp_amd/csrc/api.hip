@@ -704,11 +704,11 @@ static int relpos_args(const struct amdseg_relpos_cfg* c, RpArgs& a) {
 static size_t relpos_up(size_t n) { return (n + 255) / 256 * 256; }
 static size_t relpos_rows(const RpArgs& a) { return a.cu_q ? (size_t)a.heads * a.Tq : (size_t)a.B * a.heads * a.Lq; }
 static size_t relpos_bwd_ws(const RpArgs& a, int dtype, size_t* sums_at, size_t* part_at, size_t* kv_at, size_t* q_at) {
-    const size_t nd = 2 * ((size_t)a.span + RP_PAD) + 1, bk = 64 * rp_dkv_qt(a, dtype), nrb = (a.Lk + bk - 1) / bk;
+    const size_t nd = 2 * ((size_t)a.span + RP_PAD) + 1, bk = 64 * rp_dkv_qt(a, dtype);
     *sums_at = relpos_up(8 * relpos_rows(a));
     *part_at = *sums_at + relpos_up(4 * nd * a.heads);
     const size_t qs = rp_qsplit(a), parts = qs * rp_dkv_parts(a, rp_dkv_qt(a, dtype), (int)qs), ks = rp_nsplit(a.Lq, a.Lk, a.cu_q != nullptr);
-    *kv_at = *part_at + relpos_up(4 * nd * a.heads * a.B * nrb * qs);
+    *kv_at = *part_at + relpos_up(4 * nd * a.heads * (size_t)rp_partials(a, (int)bk, (int)qs));
     *q_at = *kv_at + (parts > 1 ? relpos_up(8 * parts * a.B * a.Lk * a.kv_heads * a.D) : 0);
     return *q_at + (ks > 1 ? 4 * ks * relpos_rows(a) * (a.D + 1) : 0);
 }

@@ -30,7 +30,9 @@ struct RpArgs {
     const int* map; const void* table; int table_bf16;
     int B, Lq, Lk, heads, kv_heads, D, Tq, Tk, span, buckets, causal, align_end, zero_tail;
     float scale;
-    int nrb;                    // row blocks of a sequence (grid); a workgroup steps by it, so a wrong `longest` hint costs time, never rows
+    int nrb;                    // padded: row blocks of a sequence
+    int slots, slot_group;      // packed: row blocks of the batch (rp_slot), how many of them in a row stream the same K / V
+    int nmain;                  // workgroups of one split (the others zero rows outside every sequence)
     int mask_words;             // 8-byte words of the key mask in LDS
     int nsplit, split_keys;     // forward and dQ: splits over the keys, keys of one (a multiple of 64)
     float* part_o; float* part_ml;           // forward, nsplit > 1: [nsplit][rows][D] unnormalised sums, [nsplit][rows][2] maximum and sum
@@ -38,7 +40,7 @@ struct RpArgs {
     float* part_q;              // backward, nsplit > 1: [nsplit][rows][D] sums of dq, then [nsplit][rows] sums of ds
     int parts, qsplit;          // backward: workgroups that share a kv head's query heads, and its query rows, in the dK / dV kernel
     float* part_kv;             // backward, parts * qsplit > 1: [dk, dv][parts * qsplit][rows of k][kv_heads][D]
-    float* part_d;              // backward: [heads][B * nrb * qsplit][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
+    float* part_d;              // backward: [heads][B * nrb * qsplit, or slots][2 (span + RP_PAD) + 1] sums of ds over equal rel, or NULL
 };
 
 // one sequence: where its rows start and how many there are.  The values of cu_q / cu_k / k_lens come from device memory that the host has not seen:
@@ -84,6 +86,46 @@ __device__ __forceinline__ void rp_place(int id, int nrb, int B, int heads, int 
     if (last_first) rb = nrb - 1 - rb;
     b = pair / kv_heads;
     h = (pair % kv_heads) * G + gi;
+}
+
+// The same for a packed batch, whose lengths the host does not know.  Row blocks of `rows` rows are numbered through (slots), T / rows + B numbers at most: grid
+// and partial sums grow with the tokens, not with sequences times the longest.  Up to 64 sequences: one behind the other by a scan over their lengths, so that the
+// numbers without a block come last (64 x 60 tokens: 9.2 us forward, 14 with a third of the workgroups empty in between).  More: sequence b's start at cu[b] / rows + b
+// -- floor(y / rows) - floor(x / rows) + 1 >= ceil((y - x) / rows), so they fit -- and 64 candidates a step are looked at.  Every wave finds its sequence for
+// itself.  Runs of `slot_group` slots of one kv head (mostly of one sequence) go to one XCD.
+// -> false: no row block of this number (or none at all: slot >= a.slots)
+__device__ __forceinline__ bool rp_slot(const RpArgs& a, const int* cu, int T, int rows, int heads, int id, bool last_first, int& slot, int& rb, int& h, int& b) {
+    const int G = heads / a.kv_heads, sg = a.slot_group, t = id >> 3, rest = t % (sg * G), pair = t / (sg * G) * 8 + (id & 7);
+    slot = pair / a.kv_heads * sg + rest % sg;
+    h = pair % a.kv_heads * G + rest / sg;
+    if (slot >= a.slots) return false;
+    const int lane = threadIdx.x & 63;
+    if (a.B <= 64) {
+        const int from = rp_clamp(cu[min(lane, a.B)], 0, T), to = rp_clamp(cu[min(lane + 1, a.B)], from, T), n = lane < a.B ? (to - from + rows - 1) / rows : 0;
+        int end = n;                                        // blocks of the sequences up to this lane's
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(end, o, 64); end += lane >= o ? x : 0; }
+        const int at = last_first ? __shfl(end, 63, 64) - 1 - slot : slot;
+        const uint64_t vote = __ballot(end - n <= at && at < end);
+        if (vote == 0) return false;
+        b = __builtin_ctzll(vote);
+        rb = __builtin_amdgcn_readlane(at - (end - n), b);
+        return true;
+    }
+    const int at = last_first ? a.slots - 1 - slot : slot;
+    int lo = 0, n = a.B;
+    while (true) {
+        const int step = (n + 63) / 64, x = lo + lane * step;
+        const uint64_t vote = __ballot(lane * step < n && rp_clamp(cu[min(x, a.B)], 0, T) / rows + x <= at);
+        if (vote == 0) return false;                        // in front of the first sequence
+        const int k = __popcll(vote) - 1;
+        lo += k * step;
+        if (step == 1) break;
+        n = min(step, n - k * step);
+    }
+    b = lo;
+    rb = at - (rp_clamp(cu[b], 0, T) / rows + b);
+    return rb >= 0;
 }
 
 // ------------------------------------------------------------------------------------------------ tiles and products

@@ -78,17 +78,18 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
     uint64_t* words = reinterpret_cast<uint64_t*>(smem + NB * 2 * Ti::BYTES);     // after the buffers of K and V chunks: the mask's words, the table
     float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int nmain = a.B * a.heads * a.nrb;
+    const int nmain = a.nmain;
     const int nsplit = MIXED ? a.nsplit : 1, split = nmain ? (int)blockIdx.x / nmain : nsplit;
     if (split >= nsplit) {
         const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq);
         rp_zero_rows((T*)a.dq, a.sdq, a.heads, a.D, lead, end, a.Tq, blockIdx.x - nmain * nsplit, RP_TAIL_WGS, tid);
         return;
     }
-    int rb, h, b;
-    rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
-    const RpSeq sq = rp_seq(a, b);
     constexpr int BQ_ = 64 * QT_;
+    int slot, rb, h, b;
+    if (!a.cu_q) rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
+    else if (!rp_slot(a, a.cu_q, a.Tq, BQ_, a.heads, blockIdx.x, a.causal, slot, rb, h, b)) return;
+    const RpSeq sq = rp_seq(a, b);
     constexpr bool AHEAD = sizeof(T) == 2;
     if (rb * BQ_ >= sq.qn) return;
     RpTable table;
@@ -279,15 +280,13 @@ __global__ __launch_bounds__(256, 2) void rp_dq_kernel(RpArgs a) {
                 if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, blind ? zero : dq[ct][d] * a.scale);
         }
     };
-    for (; rb * BQ_ < sq.qn; rb += a.nrb) {
-        constexpr int FQ = DT <= 4 ? QT_ : 1;               // (D > 64: 16 columns a wave, the second part needs the registers)
-        if constexpr (MIXED && sizeof(T) == 2)
-            if (rp_fine(a, sq, rb * BQ_)) {
-                for (int q0 = rb * BQ_; q0 < min((rb + 1) * BQ_, sq.qn); q0 += 64 * FQ) block(std::integral_constant<int, FQ>(), std::true_type(), q0);
-                continue;
-            }
-        block(std::integral_constant<int, QT_>(), std::false_type(), rb * BQ_);
-    }
+    constexpr int FQ = DT <= 4 ? QT_ : 1;                   // (D > 64: 16 columns a wave, the second part needs the registers)
+    if constexpr (MIXED && sizeof(T) == 2)
+        if (rp_fine(a, sq, rb * BQ_)) {
+            for (int q0 = rb * BQ_; q0 < min((rb + 1) * BQ_, sq.qn); q0 += 64 * FQ) block(std::integral_constant<int, FQ>(), std::true_type(), q0);
+            return;
+        }
+    block(std::integral_constant<int, QT_>(), std::false_type(), rb * BQ_);
 }
 
 // CUT: the query heads of a group, or the query rows, are dealt over several workgroups (an instance of its own, as above)
@@ -301,26 +300,34 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     float* tab = rows + NB * 128;                                // mirrored: entry x = bias of rel = -(x - mid), so that it ascends with the query
     float* bins = tab + ND;                                 // [4 waves][ND], mirrored like the table; only with part_d
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
-    const int parts = CUT ? a.parts : 1, qsplit = CUT ? a.qsplit : 1, nmain = a.B * a.kv_heads * parts * a.nrb, split = nmain ? (int)blockIdx.x / nmain : qsplit;
+    const int parts = CUT ? a.parts : 1, qsplit = CUT ? a.qsplit : 1, nmain = a.nmain, split = nmain ? (int)blockIdx.x / nmain : qsplit;
     if (split >= qsplit) {
         const int lead = rp_clamp(a.cu_k[0], 0, a.Tk), end = rp_clamp(a.cu_k[a.B], lead, a.Tk);
         rp_zero_rows((T*)a.dk, a.sdk, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain * qsplit, RP_TAIL_WGS, tid);
         rp_zero_rows((T*)a.dv, a.sdv, a.kv_heads, a.D, lead, end, a.Tk, blockIdx.x - nmain * qsplit, RP_TAIL_WGS, tid);
         return;
     }
-    int rb, hp, b;
-    rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.kv_heads * parts, a.kv_heads, false, rb, hp, b);
+    constexpr int BK = 64 * QT;
+    int slot = 0, rb, hp, b = 0;
+    bool some = true;                                       // (packed: is there a row block of this number?)
+    if (CUT || !a.cu_k) rp_place(blockIdx.x - split * nmain, a.nrb, a.B, a.kv_heads * parts, a.kv_heads, false, rb, hp, b);
+    else {
+        some = rp_slot(a, a.cu_k, a.Tk, BK, a.kv_heads, blockIdx.x, false, slot, rb, hp, b);
+        if (slot >= a.slots) return;
+    }
     const int hk = hp / parts, G = a.heads / a.kv_heads / parts, h0 = hp * G;       // this workgroup's query heads: h0 .. h0 + G - 1
     const RpSeq sq = rp_seq(a, b);
-    constexpr int BK = 64 * QT;
     const float c2 = a.scale * RP_LOG2E;
     const bool causal = a.causal;
     const int rows_k = a.cu_k ? sq.kn : a.Lk;               // padded: rows past k_lens are gradients of zero, and written
-    float* part = a.part_d ? a.part_d + (((int64_t)h0 * a.B * a.nrb + (int64_t)b * a.nrb + rb) * qsplit + split) * ND : nullptr;     // of the first head
-    const int64_t part_h = (int64_t)a.B * a.nrb * qsplit * ND;
-    if (part && rb * BK >= rows_k)
-        for (int gi = 0; gi < G; ++gi)
-            for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
+    const int64_t part_h = (int64_t)(CUT || !a.cu_k ? a.B * a.nrb * qsplit : a.slots) * ND;        // one head's partials
+    float* part = a.part_d ? a.part_d + h0 * part_h + (int64_t)(CUT || !a.cu_k ? (b * a.nrb + rb) * qsplit + split : slot) * ND : nullptr;     // of the first head
+    if (!some || rb * BK >= rows_k) {
+        if (part)
+            for (int gi = 0; gi < G; ++gi)
+                for (int x = tid; x < ND; x += 256) part[gi * part_h + x] = 0.f;
+        return;
+    }
     float* bw = bins + w * ND;
     RpTable table;
     table.start(a, -1, tid);
@@ -333,261 +340,255 @@ __global__ __launch_bounds__(256, DT * sizeof(T) * QT <= 16 ? 2 : 1) void rp_dkv
     }
     rp_cleared();
     const int64_t all_rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
-    bool again = false;                                     // (a second row block of a sequence longer than the hint adds to the first one's sums)
 
-    for (; rb * BK < rows_k; rb += a.nrb) {
-        const int k0 = rb * BK, kw = k0 + w * 16 * QT;
-        int c_first = 0, n_ch = (sq.qn + 63) / 64, r_first = 0;
-        if (causal) {                                       // query rows before r_first see none of these keys, and nothing of them is used
-            int kf = k0;
-            if (a.key_mask) {
-                const uint8_t* m = a.key_mask + (a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb);
-                uint64_t vis = 0;
-                for (; kf < min(k0 + BK, sq.kn) && !(vis = __ballot(kf + l < sq.kn && m[kf + l] != 0)); kf += 64) {}
-                kf += vis ? __builtin_ctzll(vis) : 0;
-            }
-            r_first = max(0, kf - sq.off);
-            c_first = r_first / 64;
+    const int k0 = rb * BK, kw = k0 + w * 16 * QT;
+    int c_first = 0, n_ch = (sq.qn + 63) / 64, r_first = 0;
+    if (causal) {                                       // query rows before r_first see none of these keys, and nothing of them is used
+        int kf = k0;
+        if (a.key_mask) {
+            const uint8_t* m = a.key_mask + (a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb);
+            uint64_t vis = 0;
+            for (; kf < min(k0 + BK, sq.kn) && !(vis = __ballot(kf + l < sq.kn && m[kf + l] != 0)); kf += 64) {}
+            kf += vis ? __builtin_ctzll(vis) : 0;
         }
-        if (CUT && qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
-        const T *qb, *ob;
-        const float* stat_h;
-        auto fetch = [&](int c, int buf) {
-            const uint64_t ok = rp_low_bits(sq.qn - c * 64) & ~rp_low_bits(r_first - c * 64);
-            rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + buf * 2 * Ti::BYTES, w, l);
-            ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
-            if (w == 0 && ((ok >> l) & 1)) {                // 64 rows' stat: 4 bytes a lane
-                amdseg_glds4(stat_h + c * 64 + l, rows + buf * 128);
-                amdseg_glds4(stat_h + all_rows + c * 64 + l, rows + buf * 128 + 64);
-            }
-        };
-        auto head = [&](int gi) {                           // a head's first chunk, on its way before anything else is waited for
-            const int h = h0 + gi;
-            qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
-            ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
-            stat_h = a.stat + rp_row(a, sq, b, h, 0);
-            if (NB == 2 && c_first < n_ch) fetch(c_first, 0);
-        };
-        if (again) __syncthreads();                         // (nobody is left in the buffers)
-        head(0);
-        bool seen[QT];
-        bool any = false, all = true;
-        typename Ti::frag fk[QT][Ti::KB], fv[QT][Ti::KB];
-#pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            const int key = kw + ct * 16 + i16;
-            const bool in = key < rp_seen(a, sq, sq.qn);
-            const int64_t kt = (int64_t)(sq.k0 + key);
-            seen[ct] = in && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
-#pragma unroll
-            for (int kk = 0; kk < Ti::KB; ++kk) {
-                fk[ct][kk] = Ti::gfrag((const T*)a.k + b * a.sk.sb + kt * a.sk.st + hk * a.sk.sh, kk, g, a.D, in);
-                fv[ct][kk] = Ti::gfrag((const T*)a.v + b * a.sv.sb + kt * a.sv.st + hk * a.sv.sh, kk, g, a.D, in);
-            }
+        r_first = max(0, kf - sq.off);
+        c_first = r_first / 64;
+    }
+    if (CUT && qsplit > 1) { c_first = max(c_first, split * (RP_SPLIT_ROWS / 64)); n_ch = min(n_ch, (split + 1) * (RP_SPLIT_ROWS / 64)); }
+    const T *qb, *ob;
+    const float* stat_h;
+    auto fetch = [&](int c, int buf) {
+        const uint64_t ok = rp_low_bits(sq.qn - c * 64) & ~rp_low_bits(r_first - c * 64);
+        rq.load(qb + (int64_t)c * 64 * a.sq.st, ok, smem + buf * 2 * Ti::BYTES, w, l);
+        ro.load(ob + (int64_t)c * 64 * a.sdo.st, ok, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
+        if (w == 0 && ((ok >> l) & 1)) {                // 64 rows' stat: 4 bytes a lane
+            amdseg_glds4(stat_h + c * 64 + l, rows + buf * 128);
+            amdseg_glds4(stat_h + all_rows + c * 64 + l, rows + buf * 128 + 64);
         }
+    };
+    auto head = [&](int gi) {                           // a head's first chunk, on its way before anything else is waited for
+        const int h = h0 + gi;
+        qb = (const T*)a.q + b * a.sq.sb + (int64_t)sq.q0 * a.sq.st + h * a.sq.sh;
+        ob = (const T*)a.dout + b * a.sdo.sb + (int64_t)sq.q0 * a.sdo.st + h * a.sdo.sh;
+        stat_h = a.stat + rp_row(a, sq, b, h, 0);
+        if (NB == 2 && c_first < n_ch) fetch(c_first, 0);
+    };
+    head(0);
+    bool seen[QT];
+    bool any = false, all = true;
+    typename Ti::frag fk[QT][Ti::KB], fv[QT][Ti::KB];
 #pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            any |= seen[ct];
-            all &= seen[ct];
+    for (int ct = 0; ct < QT; ++ct) {
+        const int key = kw + ct * 16 + i16;
+        const bool in = key < rp_seen(a, sq, sq.qn);
+        const int64_t kt = (int64_t)(sq.k0 + key);
+        seen[ct] = in && (!a.key_mask || a.key_mask[(a.cu_k ? (int64_t)sq.k0 : (int64_t)b * a.mask_sb) + key] != 0);
+#pragma unroll
+        for (int kk = 0; kk < Ti::KB; ++kk) {
+            fk[ct][kk] = Ti::gfrag((const T*)a.k + b * a.sk.sb + kt * a.sk.st + hk * a.sk.sh, kk, g, a.D, in);
+            fv[ct][kk] = Ti::gfrag((const T*)a.v + b * a.sv.sb + kt * a.sv.st + hk * a.sv.sh, kk, g, a.D, in);
         }
-        const bool wave_any = __any(any), wave_all = __all(all);
-        if (!wave_all)                                      // what stands in hidden rows reaches no product
+    }
 #pragma unroll
-            for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-                for (int kk = 0; kk < Ti::KB; ++kk) {
-                    fk[ct][kk] = seen[ct] ? fk[ct][kk] : (typename Ti::frag){};
-                    fv[ct][kk] = seen[ct] ? fv[ct][kk] : (typename Ti::frag){};
-                }
-        if (!__syncthreads_or(any)) { n_ch = 0; asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // (the chunk under way lands before anybody leaves)
-        f32x4 dk[QT][DT], dv[QT][DT];
+    for (int ct = 0; ct < QT; ++ct) {
+        any |= seen[ct];
+        all &= seen[ct];
+    }
+    const bool wave_any = __any(any), wave_all = __all(all);
+    if (!wave_all)                                      // what stands in hidden rows reaches no product
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
-        for (int gi = 0; gi < G; ++gi) {
-            if (gi) { __syncthreads(); head(gi); }          // (nobody is left in the buffers, the table, the bins)
-            table.finish(a, tab, h0 + gi);
-            if (part)
-                for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
-            int buf = 0;
-            f32x4 far_sum = {0.f, 0.f, 0.f, 0.f};           // one side at a time: the chunks come in the order of -rel
-            auto commit = [&](int at) {
-                const float t = wave_sum(far_sum[0] + far_sum[1] + far_sum[2] + far_sum[3]);
-                if (l == 0) bw[at] += t;
-                far_sum = (f32x4){0.f, 0.f, 0.f, 0.f};
-            };
-            int side = 0;                                   // -1: rel >= span summed so far, 1: rel <= -span
-            float diag[4 + QT], past = 0.f;                 // block diagonals 1 - QT .. 4 of the chunk
+            for (int kk = 0; kk < Ti::KB; ++kk) {
+                fk[ct][kk] = seen[ct] ? fk[ct][kk] : (typename Ti::frag){};
+                fv[ct][kk] = seen[ct] ? fv[ct][kk] : (typename Ti::frag){};
+            }
+    if (!__syncthreads_or(any)) { n_ch = 0; asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // (the chunk under way lands before anybody leaves)
+    f32x4 dk[QT][DT], dv[QT][DT];
 #pragma unroll
-            for (int k = 0; k < 4 + QT; ++k) diag[k] = 0.f;
-            auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0, int there) __attribute__((always_inline)) {
-                const char* tO = tQ + Ti::BYTES;
-                const float* rowd = rowl + 64;
-                const float* bt = tab + (rel0 + mid + 4 * g - i16);
-                const float far = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0];
+    for (int ct = 0; ct < QT; ++ct)
 #pragma unroll
-                for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
-                    f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS], dr[Ti::RPS], z[Ti::RPS + QT - 1];
-                    rp_bias(near, bt, kp * Ti::RPS + 1 - QT, far, z);
+        for (int d = 0; d < DT; ++d) { dk[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+    for (int gi = 0; gi < G; ++gi) {
+        if (gi) { __syncthreads(); head(gi); }          // (nobody is left in the buffers, the table, the bins)
+        table.finish(a, tab, h0 + gi);
+        if (part)
+            for (int x = tid; x < 4 * ND; x += 256) bins[x] = 0.f;
+        int buf = 0;
+        f32x4 far_sum = {0.f, 0.f, 0.f, 0.f};           // one side at a time: the chunks come in the order of -rel
+        auto commit = [&](int at) {
+            const float t = wave_sum(far_sum[0] + far_sum[1] + far_sum[2] + far_sum[3]);
+            if (l == 0) bw[at] += t;
+            far_sum = (f32x4){0.f, 0.f, 0.f, 0.f};
+        };
+        int side = 0;                                   // -1: rel >= span summed so far, 1: rel <= -span
+        float diag[4 + QT], past = 0.f;                 // block diagonals 1 - QT .. 4 of the chunk
+#pragma unroll
+        for (int k = 0; k < 4 + QT; ++k) diag[k] = 0.f;
+        auto chunk = [&](const bool near, const bool edge, const char* tQ, const float* rowl, int rel0, int there) __attribute__((always_inline)) {
+            const char* tO = tQ + Ti::BYTES;
+            const float* rowd = rowl + 64;
+            const float* bt = tab + (rel0 + mid + 4 * g - i16);
+            const float far = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0];
+#pragma unroll
+            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+                f32x4 s[QT][Ti::RPS], dp[QT][Ti::RPS], lr[Ti::RPS], dr[Ti::RPS], z[Ti::RPS + QT - 1];
+                rp_bias(near, bt, kp * Ti::RPS + 1 - QT, far, z);
+#pragma unroll
+                for (int j = 0; j < Ti::RPS; ++j) {
+                    const int f = kp * Ti::RPS + j;
+                    lr[j] = *reinterpret_cast<const f32x4*>(rowl + f * 16 + g * 4);
+                    dr[j] = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
+                }
+#pragma unroll
+                for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
                     for (int j = 0; j < Ti::RPS; ++j) {
                         const int f = kp * Ti::RPS + j;
-                        lr[j] = *reinterpret_cast<const f32x4*>(rowl + f * 16 + g * 4);
-                        dr[j] = *reinterpret_cast<const f32x4*>(rowd + f * 16 + g * 4);
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < Ti::KB; ++kk)
-#pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j) {
-                            const int f = kp * Ti::RPS + j;
-                            const typename Ti::frag fq = Ti::rowf(tQ, f * 16 + i16, kk, g), fo = Ti::rowf(tO, f * 16 + i16, kk, g);
-#pragma unroll
-                            for (int ct = 0; ct < QT; ++ct) {
-                                s[ct][j] = Ti::mma(fq, fk[ct][kk], kk == 0 ? rp_start<T>(z[j - ct + QT - 1]) : s[ct][j]);
-                                dp[ct][j] = Ti::mma(fo, fv[ct][kk], kk == 0 ? dr[j] : dp[ct][j]);
-                            }
-                        }
-                    if (sizeof(T) == 4)
-#pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j)
-#pragma unroll
-                            for (int ct = 0; ct < QT; ++ct) s[ct][j] += z[j - ct + QT - 1];
-                    if (edge) {                             // a hidden key's column, rel > 0 with `causal`, a row behind the sequence: p = 0
-#pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int row = (kp * Ti::RPS + j) * 16 + 4 * g + r;
-#pragma unroll
-                                for (int ct = 0; ct < QT; ++ct)
-                                    s[ct][j][r] = seen[ct] && row < there && !(causal && rel0 + row - 16 * ct - i16 < 0) ? s[ct][j][r] : -INFINITY;
-                            }
-                    }
-                    typename Ti::frag fp[QT], fds[QT];
-                    constexpr bool AHEAD = sizeof(T) == 2;  // column fragments one step ahead, as in rp_dq_kernel
-                    typename Ti::frag fo, fq;
-                    if constexpr (AHEAD) { fo = Ti::colf(tO, kp, 0, l); fq = Ti::colf(tQ, kp, 0, l); __builtin_amdgcn_sched_barrier(0); }
-#pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) {
-#pragma unroll
-                        for (int j = 0; j < Ti::RPS; ++j)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, lr[j][r]));
-                                s[ct][j][r] = p;
-                                dp[ct][j][r] *= p;
-                            }
-                        fp[ct] = Ti::pf(s[ct]);
-                        fds[ct] = Ti::pf(dp[ct]);
-                    }
-                    if (part) {
-                        if (near) {
-                            // tiles of one block diagonal first add up element by element
-#pragma unroll
-                            for (int k = 0; k < Ti::RPS + QT - 1; ++k) {
-                                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                                bool have = false;
-#pragma unroll
-                                for (int j = 0; j < Ti::RPS; ++j)
-#pragma unroll
-                                    for (int ct = 0; ct < QT; ++ct)
-                                        if (j - ct + QT - 1 == k) {
-                                            if (have) {
-#pragma unroll
-                                                for (int r = 0; r < 4; ++r) x[r] += dp[ct][j][r];
-                                            } else x = dp[ct][j];
-                                            have = true;
-                                        }
-                                rp_diag_add(x, diag[kp * Ti::RPS + k], diag[kp * Ti::RPS + k + 1]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int ct = 0; ct < QT; ++ct)
-#pragma unroll
-                                for (int j = 0; j < Ti::RPS; ++j) far_sum += dp[ct][j];
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const typename Ti::frag co = AHEAD ? fo : Ti::colf(tO, kp, d, l), cq = AHEAD ? fq : Ti::colf(tQ, kp, d, l);
-                        if (AHEAD && d + 1 < DT) { fo = Ti::colf(tO, kp, d + 1, l); fq = Ti::colf(tQ, kp, d + 1, l); }
+                        const typename Ti::frag fq = Ti::rowf(tQ, f * 16 + i16, kk, g), fo = Ti::rowf(tO, f * 16 + i16, kk, g);
 #pragma unroll
                         for (int ct = 0; ct < QT; ++ct) {
-                            dv[ct][d] = Ti::mma(co, fp[ct], dv[ct][d]);
-                            dk[ct][d] = Ti::mma(cq, fds[ct], dk[ct][d]);
+                            s[ct][j] = Ti::mma(fq, fk[ct][kk], kk == 0 ? rp_start<T>(z[j - ct + QT - 1]) : s[ct][j]);
+                            dp[ct][j] = Ti::mma(fo, fv[ct][kk], kk == 0 ? dr[j] : dp[ct][j]);
                         }
                     }
+                if (sizeof(T) == 4)
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct) s[ct][j] += z[j - ct + QT - 1];
+                if (edge) {                             // a hidden key's column, rel > 0 with `causal`, a row behind the sequence: p = 0
+#pragma unroll
+                    for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int row = (kp * Ti::RPS + j) * 16 + 4 * g + r;
+#pragma unroll
+                            for (int ct = 0; ct < QT; ++ct)
+                                s[ct][j][r] = seen[ct] && row < there && !(causal && rel0 + row - 16 * ct - i16 < 0) ? s[ct][j][r] : -INFINITY;
+                        }
                 }
-            };
-            for (int c = c_first; c < n_ch; ++c, buf ^= NB - 1) {
-                if (NB == 1) { __syncthreads(); fetch(c, 0); }
-                rp_landed();
-                const char* tQ = smem + buf * 2 * Ti::BYTES;
-                const float* rowl = rows + buf * 128;
-                if (NB == 2 && c + 1 < n_ch) fetch(c + 1, buf ^ 1);
-                const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
-                if (!wave_any || (causal && rel0 + 63 < 0)) continue;
-                const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
-                if (part && side < 0 && rel0 > 0) { commit(0); side = 0; }
-                if (part && !near) side = rel0 > 0 ? 1 : -1;
-                chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0) || (c + 1) * 64 > sq.qn, tQ, rowl, rel0, sq.qn - c * 64);
-                if (part && near) {
-                    float* bd = bw + (rel0 - 16 * (QT - 1) + mid + 16 * g - i16);
-                    *bd = rp_join4(diag[0], diag[1], diag[2], diag[3], past, l);
-                    // the upper ones go on into the next chunk, 64 rel further; after the last near chunk they are stored too (nothing beyond rel0 + 63)
+                typename Ti::frag fp[QT], fds[QT];
+                constexpr bool AHEAD = sizeof(T) == 2;  // column fragments one step ahead, as in rp_dq_kernel
+                typename Ti::frag fo, fq;
+                if constexpr (AHEAD) { fo = Ti::colf(tO, kp, 0, l); fq = Ti::colf(tQ, kp, 0, l); __builtin_amdgcn_sched_barrier(0); }
 #pragma unroll
-                    for (int k = 0; k < QT; ++k) diag[k] = diag[4 + k];
+                for (int ct = 0; ct < QT; ++ct) {
 #pragma unroll
-                    for (int k = QT; k < 4 + QT; ++k) diag[k] = 0.f;
-                    if (c + 1 >= n_ch || rel0 + 64 - (16 * QT - 1) >= span) {
-                        const float rest = rp_join4(diag[0], QT > 1 ? diag[1] : 0.f, 0.f, 0.f, past, l);
-                        if (64 - 16 * (QT - 1) + 16 * g - i16 <= 63) bd[64] = rest;
-                        past = 0.f;
+                    for (int j = 0; j < Ti::RPS; ++j)
 #pragma unroll
-                        for (int k = 0; k < QT; ++k) diag[k] = 0.f;
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j][r], c2, lr[j][r]));
+                            s[ct][j][r] = p;
+                            dp[ct][j][r] *= p;
+                        }
+                    fp[ct] = Ti::pf(s[ct]);
+                    fds[ct] = Ti::pf(dp[ct]);
+                }
+                if (part) {
+                    if (near) {
+                        // tiles of one block diagonal first add up element by element
+#pragma unroll
+                        for (int k = 0; k < Ti::RPS + QT - 1; ++k) {
+                            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                            bool have = false;
+#pragma unroll
+                            for (int j = 0; j < Ti::RPS; ++j)
+#pragma unroll
+                                for (int ct = 0; ct < QT; ++ct)
+                                    if (j - ct + QT - 1 == k) {
+                                        if (have) {
+#pragma unroll
+                                            for (int r = 0; r < 4; ++r) x[r] += dp[ct][j][r];
+                                        } else x = dp[ct][j];
+                                        have = true;
+                                    }
+                            rp_diag_add(x, diag[kp * Ti::RPS + k], diag[kp * Ti::RPS + k + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+                            for (int j = 0; j < Ti::RPS; ++j) far_sum += dp[ct][j];
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const typename Ti::frag co = AHEAD ? fo : Ti::colf(tO, kp, d, l), cq = AHEAD ? fq : Ti::colf(tQ, kp, d, l);
+                    if (AHEAD && d + 1 < DT) { fo = Ti::colf(tO, kp, d + 1, l); fq = Ti::colf(tQ, kp, d + 1, l); }
+#pragma unroll
+                    for (int ct = 0; ct < QT; ++ct) {
+                        dv[ct][d] = Ti::mma(co, fp[ct], dv[ct][d]);
+                        dk[ct][d] = Ti::mma(cq, fds[ct], dk[ct][d]);
                     }
                 }
             }
-            if (part) {
-                if (c_first >= n_ch) __syncthreads();       // (the zeroed bins: no chunk's barrier came in between)
-                if (side) commit(side < 0 ? 0 : ND - 1);
-                __syncthreads();
-                for (int x = tid; x < ND; x += 256) {
-                    const float t = (bins[x] + bins[ND + x]) + (bins[2 * ND + x] + bins[3 * ND + x]);
-                    float* o = part + gi * part_h + (ND - 1 - x);
-                    *o = again ? *o + t : t;
+        };
+        for (int c = c_first; c < n_ch; ++c, buf ^= NB - 1) {
+            if (NB == 1) { __syncthreads(); fetch(c, 0); }
+            rp_landed();
+            const char* tQ = smem + buf * 2 * Ti::BYTES;
+            const float* rowl = rows + buf * 128;
+            if (NB == 2 && c + 1 < n_ch) fetch(c + 1, buf ^ 1);
+            const int rel0 = c * 64 + sq.off - kw;      // (query - key) of the tile's first row and the wave's first column
+            if (!wave_any || (causal && rel0 + 63 < 0)) continue;
+            const bool near = rel0 + 63 > -span && rel0 - (16 * QT - 1) < span;
+            if (part && side < 0 && rel0 > 0) { commit(0); side = 0; }
+            if (part && !near) side = rel0 > 0 ? 1 : -1;
+            chunk(near, !wave_all || (causal && rel0 - (16 * QT - 1) < 0) || (c + 1) * 64 > sq.qn, tQ, rowl, rel0, sq.qn - c * 64);
+            if (part && near) {
+                float* bd = bw + (rel0 - 16 * (QT - 1) + mid + 16 * g - i16);
+                *bd = rp_join4(diag[0], diag[1], diag[2], diag[3], past, l);
+                // the upper ones go on into the next chunk, 64 rel further; after the last near chunk they are stored too (nothing beyond rel0 + 63)
+#pragma unroll
+                for (int k = 0; k < QT; ++k) diag[k] = diag[4 + k];
+#pragma unroll
+                for (int k = QT; k < 4 + QT; ++k) diag[k] = 0.f;
+                if (c + 1 >= n_ch || rel0 + 64 - (16 * QT - 1) >= span) {
+                    const float rest = rp_join4(diag[0], QT > 1 ? diag[1] : 0.f, 0.f, 0.f, past, l);
+                    if (64 - 16 * (QT - 1) + 16 * g - i16 <= 63) bd[64] = rest;
+                    past = 0.f;
+#pragma unroll
+                    for (int k = 0; k < QT; ++k) diag[k] = 0.f;
                 }
             }
         }
-        again = true;
-        // a hidden key's column is zero, whatever dout held
-#pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            const int key = kw + ct * 16 + i16;
-            if (key >= rows_k) continue;
-            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            if (CUT) {
-                const int64_t rows_all = (int64_t)a.B * a.Lk, row = (int64_t)b * a.Lk + key;
-                float* kp_ = a.part_kv + ((((hp - hk * parts) * qsplit + split) * rows_all + row) * a.kv_heads + hk) * a.D;
-                float* vp_ = kp_ + parts * qsplit * rows_all * a.kv_heads * a.D;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    if (d * 16 + g * 4 < a.D) {
-                        *reinterpret_cast<f32x4*>(kp_ + d * 16 + g * 4) = seen[ct] ? dk[ct][d] * a.scale : z;
-                        *reinterpret_cast<f32x4*>(vp_ + d * 16 + g * 4) = seen[ct] ? dv[ct][d] : z;
-                    }
-                continue;
+        if (part) {
+            if (c_first >= n_ch) __syncthreads();       // (the zeroed bins: no chunk's barrier came in between)
+            if (side) commit(side < 0 ? 0 : ND - 1);
+            __syncthreads();
+            for (int x = tid; x < ND; x += 256) {
+                const float t = (bins[x] + bins[ND + x]) + (bins[2 * ND + x] + bins[3 * ND + x]);
+                part[gi * part_h + (ND - 1 - x)] = t;
             }
-            T* kp_ = (T*)a.dk + b * a.sdk.sb + (int64_t)(sq.k0 + key) * a.sdk.st + hk * a.sdk.sh;
-            T* vp_ = (T*)a.dv + b * a.sdv.sb + (int64_t)(sq.k0 + key) * a.sdv.st + hk * a.sdv.sh;
+        }
+    }
+    // a hidden key's column is zero, whatever dout held
+#pragma unroll
+    for (int ct = 0; ct < QT; ++ct) {
+        const int key = kw + ct * 16 + i16;
+        if (key >= rows_k) continue;
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        if (CUT) {
+            const int64_t rows_all = (int64_t)a.B * a.Lk, row = (int64_t)b * a.Lk + key;
+            float* kp_ = a.part_kv + ((((hp - hk * parts) * qsplit + split) * rows_all + row) * a.kv_heads + hk) * a.D;
+            float* vp_ = kp_ + parts * qsplit * rows_all * a.kv_heads * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 if (d * 16 + g * 4 < a.D) {
-                    Ti::st4(kp_ + d * 16 + g * 4, seen[ct] ? dk[ct][d] * a.scale : z);
-                    Ti::st4(vp_ + d * 16 + g * 4, seen[ct] ? dv[ct][d] : z);
+                    *reinterpret_cast<f32x4*>(kp_ + d * 16 + g * 4) = seen[ct] ? dk[ct][d] * a.scale : z;
+                    *reinterpret_cast<f32x4*>(vp_ + d * 16 + g * 4) = seen[ct] ? dv[ct][d] : z;
                 }
+            continue;
         }
+        T* kp_ = (T*)a.dk + b * a.sdk.sb + (int64_t)(sq.k0 + key) * a.sdk.st + hk * a.sdk.sh;
+        T* vp_ = (T*)a.dv + b * a.sdv.sb + (int64_t)(sq.k0 + key) * a.sdv.st + hk * a.sdv.sh;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (d * 16 + g * 4 < a.D) {
+                Ti::st4(kp_ + d * 16 + g * 4, seen[ct] ? dk[ct][d] * a.scale : z);
+                Ti::st4(vp_ + d * 16 + g * 4, seen[ct] ? dv[ct][d] : z);
+            }
     }
 }
 
@@ -724,9 +725,9 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     const int tail = a.zero_tail ? RP_TAIL_WGS : 0;
     a.mask_words = rp_mask_bytes(a) / 8;
     const int qt = rp_dq_qt(a, dtype), kt = rp_dkv_qt(a, dtype);
-    a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
-    const int64_t n = (int64_t)a.B * a.nrb * a.heads * a.nsplit + tail;
-    if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
+    rp_blocks(a, a.Lq, a.Tq, 64 * qt, a.heads);
+    const int64_t n = (int64_t)a.nmain * a.nsplit + tail;
+    if (a.nmain < 0 || n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + ND * 4;
     int rc = 0;
     if (n > 0) {
@@ -739,7 +740,6 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
         if (rc) return rc;
     }
     if ((rc = amdseg_launch_status())) return rc;
-    a.nrb = (a.Lk + 64 * kt - 1) / (64 * kt);
     if (a.nsplit > 1 && n > 0) {
         const int64_t vecs = (int64_t)a.B * a.heads * a.Lq * (a.D / 4);
         if ((vecs + 255) / 256 > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
@@ -748,8 +748,9 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
     }
     a.qsplit = rp_qsplit(a);
     a.parts = rp_dkv_parts(a, kt, a.qsplit);
-    const int64_t m = (int64_t)a.B * a.kv_heads * a.parts * a.qsplit * a.nrb + tail;
-    if (m > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
+    rp_blocks(a, a.Lk, a.Tk, 64 * kt, a.kv_heads * a.parts);
+    const int64_t m = (int64_t)a.nmain * a.qsplit + tail;
+    if (a.nmain < 0 || m > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     const int lds2 = rp_nb<T, DT> * (2 * RpTile<T, DT>::BYTES + 512) + ND * 4 * (a.part_d ? 5 : 1);
     if (m == 0) {
     } else if (sizeof(T) == 4 || DT > 4 || kt == 1) {
@@ -765,7 +766,7 @@ static int rp_bwd_launch(RpArgs a, int dtype, void* dtable, float* sums, hipStre
         if ((rc = amdseg_launch_status())) return rc;
     }
     if (!a.part_d) return 0;
-    return amdseg_relpos_sums_impl(a.part_d, sums, (int64_t)a.B * a.nrb * a.qsplit, a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
+    return amdseg_relpos_sums_impl(a.part_d, sums, rp_partials(a, 64 * kt, a.qsplit), a.map, a.span, RP_PAD, a.buckets, a.heads, dtable, a.table_bf16, s);
 }
 template <typename T>
 static int rp_bwd_d(const RpArgs& a, int dtype, void* dtable, float* sums, hipStream_t s) {

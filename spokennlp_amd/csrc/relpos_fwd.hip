@@ -18,8 +18,7 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     float* tab = reinterpret_cast<float*>(words + a.mask_words);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i16 = l & 15;
     int id = blockIdx.x;
-    const int nmain = a.B * a.heads * a.nrb;
-    const int split = nmain ? id / nmain : a.nsplit;
+    const int nmain = a.nmain, split = nmain ? id / nmain : a.nsplit;
     if (split >= a.nsplit) {                                // the buffer rows outside every sequence
         const int lead = rp_clamp(a.cu_q[0], 0, a.Tq), end = rp_clamp(a.cu_q[a.B], lead, a.Tq), which = id - nmain * a.nsplit;
         rp_zero_rows((T*)a.out, a.so, a.heads, a.D, lead, end, a.Tq, which, RP_TAIL_WGS, tid);
@@ -30,10 +29,11 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
         return;
     }
     id -= split * nmain;
-    int rb, h, b;
-    rp_place(id, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
-    const RpSeq sq = rp_seq(a, b);
     constexpr int BQ = 64 * QT;
+    int slot, rb, h, b;
+    if (!a.cu_q) rp_place(id, a.nrb, a.B, a.heads, a.kv_heads, a.causal, rb, h, b);
+    else if (!rp_slot(a, a.cu_q, a.Tq, BQ, a.heads, id, a.causal, slot, rb, h, b)) return;
+    const RpSeq sq = rp_seq(a, b);
     if (rb * BQ >= sq.qn) return;
     RpTable table;
     table.start(a, 1, tid);
@@ -52,156 +52,151 @@ __global__ __launch_bounds__(256, 2) void rp_fwd_kernel(RpArgs a) {
     const float c2 = a.scale * RP_LOG2E;
     const int mid = a.span + RP_PAD, span = a.span;
     const bool causal = a.causal;
-    bool first = true;
 
-    for (; rb * BQ < sq.qn; rb += a.nrb) {
-        const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
-        int c = 0, c_end = keys.upto(rp_seen(a, sq, q0 + BQ));
-        if (a.nsplit > 1) { c = split * (a.split_keys / 64); c_end = min(c_end, c + a.split_keys / 64); }
-        auto fetch = [&](int at, int buf, uint64_t bits) {
-            rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
-            rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
-        };
-        uint64_t bits;
-        c = keys.seek(c, c_end, bits);
-        int buf = 0;
-        if (NB == 2 && c < c_end) fetch(c, 0, bits);        // on its way before anything else is waited for
-        typename Ti::frag fq[QT][Ti::KB];
+    const int q0 = rb * BQ, qw = q0 + w * 16 * QT;
+    int c = 0, c_end = keys.upto(rp_seen(a, sq, q0 + BQ));
+    if (a.nsplit > 1) { c = split * (a.split_keys / 64); c_end = min(c_end, c + a.split_keys / 64); }
+    auto fetch = [&](int at, int buf, uint64_t bits) {
+        rk.load(kb + (int64_t)at * 64 * a.sk.st, bits, smem + buf * 2 * Ti::BYTES, w, l);
+        rv.load(vb + (int64_t)at * 64 * a.sv.st, bits, smem + buf * 2 * Ti::BYTES + Ti::BYTES, w, l);
+    };
+    uint64_t bits;
+    c = keys.seek(c, c_end, bits);
+    int buf = 0;
+    if (NB == 2 && c < c_end) fetch(c, 0, bits);        // on its way before anything else is waited for
+    typename Ti::frag fq[QT][Ti::KB];
 #pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            const int q = qw + ct * 16 + i16;
+    for (int ct = 0; ct < QT; ++ct) {
+        const int q = qw + ct * 16 + i16;
 #pragma unroll
-            for (int kk = 0; kk < Ti::KB; ++kk) fq[ct][kk] = Ti::gfrag(qbase + (int64_t)q * a.sq.st, kk, g, a.D, q < sq.qn);
-        }
-        if (first) table.finish(a, tab, h);
-        first = false;
-        f32x4 o[QT][DT];
-        float m_run[QT], l_part[QT];
+        for (int kk = 0; kk < Ti::KB; ++kk) fq[ct][kk] = Ti::gfrag(qbase + (int64_t)q * a.sq.st, kk, g, a.D, q < sq.qn);
+    }
+    table.finish(a, tab, h);
+    f32x4 o[QT][DT];
+    float m_run[QT], l_part[QT];
 #pragma unroll
-        for (int ct = 0; ct < QT; ++ct) {
-            m_run[ct] = -INFINITY; l_part[ct] = 0.f;
+    for (int ct = 0; ct < QT; ++ct) {
+        m_run[ct] = -INFINITY; l_part[ct] = 0.f;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        }
-        // one chunk: `near` = some |rel| < span (scores start from the table; else from 0, and the constant joins in the exponent), `edge` = some (i, j) hidden
-        auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
-            const char* tV = tK + Ti::BYTES;
-            f32x4 s[QT][4], z[3 + QT];
-            rp_bias(near, tab + (rel0 + mid + 4 * g - i16), 1 - QT, 0.f, z);
+        for (int d = 0; d < DT; ++d) o[ct][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    // one chunk: `near` = some |rel| < span (scores start from the table; else from 0, and the constant joins in the exponent), `edge` = some (i, j) hidden
+    auto chunk = [&](const bool near, const bool edge, const char* tK, int rel0, uint64_t now) __attribute__((always_inline)) {
+        const char* tV = tK + Ti::BYTES;
+        f32x4 s[QT][4], z[3 + QT];
+        rp_bias(near, tab + (rel0 + mid + 4 * g - i16), 1 - QT, 0.f, z);
 #pragma unroll
-            for (int kk = 0; kk < Ti::KB; ++kk)
+        for (int kk = 0; kk < Ti::KB; ++kk)
 #pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g);
+            for (int f = 0; f < 4; ++f) {
+                const typename Ti::frag fk = Ti::rowf(tK, f * 16 + i16, kk, g);
 #pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) {
-                        s[ct][f] = Ti::mma(fk, fq[ct][kk], kk == 0 ? rp_start<T>(z[f - ct + QT - 1]) : s[ct][f]);
-                    }
-                }
-            if (sizeof(T) == 4)
-#pragma unroll
-                for (int f = 0; f < 4; ++f)
-#pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) s[ct][f] += z[f - ct + QT - 1];
-            if (edge) {
-#pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int ct = 0; ct < QT; ++ct)
-                            s[ct][f][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][f][r] : -INFINITY;
+                for (int ct = 0; ct < QT; ++ct) {
+                    s[ct][f] = Ti::mma(fk, fq[ct][kk], kk == 0 ? rp_start<T>(z[f - ct + QT - 1]) : s[ct][f]);
                 }
             }
-            const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
-            typename Ti::frag ahead = Ti::colf(tV, 0, 0, l);        // V fragments are read one step ahead: the first under the exponentials
-            __builtin_amdgcn_sched_barrier(0);
+        if (sizeof(T) == 4)
 #pragma unroll
-            for (int ct = 0; ct < QT; ++ct) {
-                float mx = s[ct][0][0];
+            for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int f = 0; f < 4; ++f)
+                for (int ct = 0; ct < QT; ++ct) s[ct][f] += z[f - ct + QT - 1];
+        if (edge) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[ct][f][r]);
-                mx = fmaf(mx, c2, fc);
-                if (__any(mx > m_run[ct])) {                // wave-uniform: some row's running maximum grows
-                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                    const float m_new = fmaxf(m_run[ct], mx);
-                    const float al = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[ct] - m_new);
-                    m_run[ct] = m_new;
-                    l_part[ct] *= al;
+            for (int f = 0; f < 4; ++f) {
+                const uint32_t nib = (uint32_t)(now >> (f * 16 + 4 * g));
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[ct][d][r] *= al;
-                }
-                const float mu = fc - (m_run[ct] == -INFINITY ? 0.f : m_run[ct]);
-                float sum = 0.f;
-#pragma unroll
-                for (int f = 0; f < 4; ++f)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[ct][f][r], c2, mu));
-                        s[ct][f][r] = e;
-                        sum += e;
-                    }
-                l_part[ct] += sum;
+                    for (int ct = 0; ct < QT; ++ct)
+                        s[ct][f][r] = ((nib >> r) & 1) && !(causal && rel0 + 16 * (f - ct) + 4 * g + r - i16 > 0) ? s[ct][f][r] : -INFINITY;
             }
-#pragma unroll
-            for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
-                typename Ti::frag fp[QT];
-#pragma unroll
-                for (int ct = 0; ct < QT; ++ct) fp[ct] = Ti::pf(&s[ct][kp * Ti::RPS]);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const typename Ti::frag fv = ahead;
-                    if (d + 1 < DT) ahead = Ti::colf(tV, kp, d + 1, l);
-                    else if (kp + 1 < 64 / Ti::KSTEP) ahead = Ti::colf(tV, kp + 1, 0, l);
-#pragma unroll
-                    for (int ct = 0; ct < QT; ++ct) o[ct][d] = Ti::mma(fv, fp[ct], o[ct][d]);
-                }
-            }
-        };
-        while (c < c_end) {
-            if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
-            rp_landed();                                    // this chunk is there (and the table), nobody reads the buffer of the one before it any more
-            const char* tK = smem + buf * 2 * Ti::BYTES;
-            const int rel0 = c * 64 - (qw + sq.off);        // rel of the chunk's first key and the wave's first query
-            const uint64_t now = bits;
-            c = keys.seek(c + 1, c_end, bits);
-            buf ^= NB - 1;
-            if (NB == 2 && c < c_end) fetch(c, buf, bits);
-            if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
-            const bool near = rp_near<T>(rel0, qw, span);
-            chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
         }
+        const float fc = near ? 0.f : tab[rel0 > 0 ? 2 * mid : 0] * c2;
+        typename Ti::frag ahead = Ti::colf(tV, 0, 0, l);        // V fragments are read one step ahead: the first under the exponentials
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ct = 0; ct < QT; ++ct) {
-            const int q = qw + ct * 16 + i16;
-            float ls = l_part[ct];
-            ls += __shfl_xor(ls, 16, 64);
-            ls += __shfl_xor(ls, 32, 64);
-            if (q >= sq.qn) continue;
-            const int64_t row = rp_row(a, sq, b, h, q);
-            if (a.nsplit > 1) {
-                const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
-                float* po = a.part_o + (split * rows + row) * a.D;
+            float mx = s[ct][0][0];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[ct][f][r]);
+            mx = fmaf(mx, c2, fc);
+            if (__any(mx > m_run[ct])) {                // wave-uniform: some row's running maximum grows
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float m_new = fmaxf(m_run[ct], mx);
+                const float al = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[ct] - m_new);
+                m_run[ct] = m_new;
+                l_part[ct] *= al;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
-                    if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(po + d * 16 + g * 4) = o[ct][d];
-                if (g == 0) { a.part_ml[(split * rows + row) * 2] = m_run[ct]; a.part_ml[(split * rows + row) * 2 + 1] = ls; }
-                continue;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[ct][d][r] *= al;
             }
-            const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);    // a row that saw no key: zero; NaN stays
-            T* op = (T*)a.out + b * a.so.sb + (int64_t)(sq.q0 + q) * a.so.st + h * a.so.sh;
+            const float mu = fc - (m_run[ct] == -INFINITY ? 0.f : m_run[ct]);
+            float sum = 0.f;
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[ct][f][r], c2, mu));
+                    s[ct][f][r] = e;
+                    sum += e;
+                }
+            l_part[ct] += sum;
+        }
+#pragma unroll
+        for (int kp = 0; kp < 64 / Ti::KSTEP; ++kp) {
+            typename Ti::frag fp[QT];
+#pragma unroll
+            for (int ct = 0; ct < QT; ++ct) fp[ct] = Ti::pf(&s[ct][kp * Ti::RPS]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const typename Ti::frag fv = ahead;
+                if (d + 1 < DT) ahead = Ti::colf(tV, kp, d + 1, l);
+                else if (kp + 1 < 64 / Ti::KSTEP) ahead = Ti::colf(tV, kp + 1, 0, l);
+#pragma unroll
+                for (int ct = 0; ct < QT; ++ct) o[ct][d] = Ti::mma(fv, fp[ct], o[ct][d]);
+            }
+        }
+    };
+    while (c < c_end) {
+        if (NB == 1) { __syncthreads(); fetch(c, 0, bits); }
+        rp_landed();                                    // this chunk is there (and the table), nobody reads the buffer of the one before it any more
+        const char* tK = smem + buf * 2 * Ti::BYTES;
+        const int rel0 = c * 64 - (qw + sq.off);        // rel of the chunk's first key and the wave's first query
+        const uint64_t now = bits;
+        c = keys.seek(c + 1, c_end, bits);
+        buf ^= NB - 1;
+        if (NB == 2 && c < c_end) fetch(c, buf, bits);
+        if (qw >= sq.qn || (causal && rel0 - (16 * QT - 1) > 0)) continue;
+        const bool near = rp_near<T>(rel0, qw, span);
+        chunk(near, now != ~0ull || (causal && rel0 + 63 > 0), tK, rel0, now);
+    }
+#pragma unroll
+    for (int ct = 0; ct < QT; ++ct) {
+        const int q = qw + ct * 16 + i16;
+        float ls = l_part[ct];
+        ls += __shfl_xor(ls, 16, 64);
+        ls += __shfl_xor(ls, 32, 64);
+        if (q >= sq.qn) continue;
+        const int64_t row = rp_row(a, sq, b, h, q);
+        if (a.nsplit > 1) {
+            const int64_t rows = a.cu_q ? (int64_t)a.heads * a.Tq : (int64_t)a.B * a.heads * a.Lq;
+            float* po = a.part_o + (split * rows + row) * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, o[ct][d] * inv);
-            if (a.lse && g == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m_run[ct] + __builtin_amdgcn_logf(ls)) * RP_LN2;
+                if (d * 16 + g * 4 < a.D) *reinterpret_cast<f32x4*>(po + d * 16 + g * 4) = o[ct][d];
+            if (g == 0) { a.part_ml[(split * rows + row) * 2] = m_run[ct]; a.part_ml[(split * rows + row) * 2 + 1] = ls; }
+            continue;
         }
-        __syncthreads();                                    // (another row block of a packed sequence longer than the hint)
+        const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);    // a row that saw no key: zero; NaN stays
+        T* op = (T*)a.out + b * a.so.sb + (int64_t)(sq.q0 + q) * a.so.st + h * a.so.sh;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (d * 16 + g * 4 < a.D) Ti::st4(op + d * 16 + g * 4, o[ct][d] * inv);
+        if (a.lse && g == 0) a.lse[row] = ls == 0.f ? -INFINITY : (m_run[ct] + __builtin_amdgcn_logf(ls)) * RP_LN2;
     }
 }
 
@@ -437,8 +432,8 @@ static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
     const int lds = 2 * rp_nb<T, DT> * RpTile<T, DT>::BYTES + a.mask_words * 8 + (2 * (a.span + RP_PAD) + 1) * 4;
     const int rc = rp_allow_lds((const void*)rp_fwd_kernel<T, DT, QT>, lds);
     if (rc) return rc;
-    const int64_t n = (int64_t)a.B * a.heads * a.nrb * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
-    if (n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
+    const int64_t n = (int64_t)a.nmain * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
+    if (a.nmain < 0 || n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
     hipLaunchKernelGGL((rp_fwd_kernel<T, DT, QT>), dim3((unsigned)n), dim3(256), lds, s, a);
     const int rc2 = amdseg_launch_status();
     return rc2 ? rc2 : rp_join_launch<T>(a, s);
@@ -457,7 +452,7 @@ int amdseg_relpos_fwd_impl(const RpArgs& a0, int dtype, hipStream_t s) {
     RpArgs a = a0;
     if (rp_few(a)) return dtype == 1 ? rp_few_d<float>(a, s) : rp_few_d<bf16_t>(a, s);
     const int qt = rp_fwd_qt(a, dtype);
-    a.nrb = (a.Lq + 64 * qt - 1) / (64 * qt);
+    rp_blocks(a, a.Lq, a.Tq, 64 * qt, a.heads);
     a.mask_words = rp_mask_bytes(a) / 8;
     if (dtype == 1) return rp_fwd_d<float, 1>(a, s);
     return qt == 1 ? rp_fwd_d<bf16_t, 1>(a, s) : rp_fwd_d<bf16_t, 2>(a, s);

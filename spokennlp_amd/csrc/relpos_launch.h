@@ -24,14 +24,35 @@ static inline int rp_allow_lds(const void* kernel, int bytes) {
 // D > 64 in bf16: two accumulators of 128 columns cost the dK / dV kernel its second wave a SIMD (16 x 512: 113 us against 104 with one tile), and a forward grid of three rounds or more runs better on three waves a SIMD of one tile (4 x 2048:
 // 177 against 165).
 static inline int rp_qt(int64_t wgs_of_two, int most_of_one, int dtype) { return dtype == 1 ? 1 : wgs_of_two <= most_of_one ? 1 : 2; }
-static inline int64_t rp_wgs_of_two(const RpArgs& a) { return (int64_t)((a.Lq + 127) / 128) * a.B * a.heads; }
+// (packed: a sequence's last block is half full on average)
+static inline int64_t rp_blocks_of_two(const RpArgs& a, int L, int T) { return a.cu_q ? (int64_t)(T + 127) / 128 + a.B / 2 : (int64_t)((L + 127) / 128) * a.B; }
+static inline int64_t rp_wgs_of_two(const RpArgs& a) { return rp_blocks_of_two(a, a.Lq, a.Tq) * a.heads; }
 static inline int rp_dq_qt(const RpArgs& a, int dtype) { return rp_qt(rp_wgs_of_two(a), a.D > 64 ? 256 : 384, dtype); }
 static inline int rp_fwd_qt(const RpArgs& a, int dtype) { return a.D > 64 && rp_wgs_of_two(a) >= 768 ? 1 : rp_dq_qt(a, dtype); }
-static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt((int64_t)((a.Lk + 127) / 128) * a.B * a.kv_heads, 256, dtype); }
+static inline int rp_dkv_qt(const RpArgs& a, int dtype) { return a.D > 64 ? 1 : rp_qt(rp_blocks_of_two(a, a.Lk, a.Tk) * a.kv_heads, 256, dtype); }
+// row blocks of a batch (packed: as many as there can be)
+static inline int64_t rp_row_blocks(const RpArgs& a, int L, int T, int rows) { return a.cu_q ? (int64_t)T / rows + a.B : (int64_t)((L + rows - 1) / rows) * a.B; }
+// how the workgroups of one split are numbered (rp_place, rp_slot): row blocks of `rows` rows, `heads` of them over a.kv_heads.  nmain < 0: too many.  Packed: runs of
+// 8 slots of a kv head, shorter ones where that would leave less than 64 runs for the 8 XCDs
+static inline void rp_blocks(RpArgs& a, int L, int T, int rows, int heads) {
+    const int64_t n = rp_row_blocks(a, L, T, rows);
+    int64_t main = n * heads;
+    a.nrb = a.cu_q ? 0 : (L + rows - 1) / rows;
+    a.slots = a.cu_q ? (int)std::min<int64_t>(n, RP_MAX_WGS) : 0;
+    a.slot_group = 1;
+    if (a.cu_q) {
+        a.slot_group = (int)std::max<int64_t>(1, std::min<int64_t>(8, n * a.kv_heads / 64));
+        const int64_t pairs = (n + a.slot_group - 1) / a.slot_group * a.kv_heads;
+        main = a.B ? (pairs + 7) / 8 * 8 * a.slot_group * (heads / a.kv_heads) : 0;
+    }
+    a.nmain = main > RP_MAX_WGS ? -1 : (int)main;
+}
+// partial sums of ds over equal rel, per head
+static inline int64_t rp_partials(const RpArgs& a, int rows, int qsplit) { return a.cu_q && !a.B ? 0 : rp_row_blocks(a, a.Lk, a.Tk, rows) * qsplit; }
 // dK / dV of shared kv heads: a workgroup walks the rows of all G query heads; where that leaves less than two workgroups a CU, `parts` of them take G / parts
 // heads each and rp_join_kv_kernel adds their fp32 sums (3 x 1023 causal, 16 / 4 heads, D = 128: 150 -> 75 us with the join;
-// at RP_PART_STEPS chunks a walk, 4 x 256 rows of 16 / 4 heads, 37 -> 23, below that there is little to share out).  Not for packed sequences: `longest` is
-// a hint there and must not change bits.
+// at RP_PART_STEPS chunks a walk, 4 x 256 rows of 16 / 4 heads, 37 -> 23, below that there is little to share out).  Not for packed sequences, whose
+// lengths the host does not know.
 #define RP_PART_STEPS 16
 static inline int rp_dkv_parts(const RpArgs& a, int kt, int qsplit) {
     const int G = a.heads / a.kv_heads;

@@ -221,3 +221,57 @@ def test_gradients_that_start_anywhere(dev):
             y = torch.cat([torch.zeros(pad, dtype=dtype, device=dev), R.relpos_self_attention(qkv, 4, table, lut, kv_heads=2).flatten()])
             y.backward(torch.cat([torch.ones(pad, dtype=dtype, device=dev), dout.flatten()]))
             assert torch.equal(qkv.grad, torch.cat([x.flatten(-2) for x in want[2:5]], -1))
+
+
+# ---- packed batches without a hint, and with one long sequence among short ones
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_hints_change_nothing_at_all(dev, dtype, causal):
+    """many short sequences and one long one (and empty ones, rows in front and behind): every hint gives the same bits, dtable's too, and the padded call's rows"""
+    print("CASE", dtype, causal, flush=True)
+    g = torch.Generator().manual_seed(7)
+    lens = torch.randint(0, 40, (300,), generator=g).tolist()
+    lens[41], lens[42], lens[299] = 1300, 0, 129
+    cu = [11]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    H, Hk, D, T = 4, 2, 64, cu[-1] + 50
+    cut = torch.tensor(cu, dtype=torch.int32, device=dev)
+    q, k, v, table, lut, dout = (x[0] if x.dim() == 4 else x for x in make(dev, dtype, 1, T, T, H, Hk, D, fused=True, bidirectional=not causal))
+    m = (torch.rand(T, generator=g) < 0.9).to(dev)
+    for mask in (None, m):
+        base = None
+        for hint in (None, 1300, 64, 1):
+            r = passes(q, k, v, table, lut, dout, cu_q=cut, cu_k=cut, max_q=hint, max_k=hint, causal=causal, key_mask=mask)
+            base = base or r
+            assert all(torch.equal(x, y) for x, y in zip(r, base)), hint
+        total = torch.zeros(table.shape, dtype=F64, device=dev)
+        for b, n in enumerate(lens):
+            s = slice(cu[b], cu[b] + n)
+            if n and (b % 20 == 0 or n > 100):
+                one = passes(q[None, s], k[None, s], v[None, s], table, lut, dout[None, s], causal=causal, key_mask=None if mask is None else mask[None, s])
+                for x, y in zip((base[0][s], base[1][:, s], base[2][s]), (one[0][0], one[1][0], one[2][0])):
+                    assert torch.equal(x, y), b
+                assert rel(base[3][s], one[3][0]) < TOL[dtype] and rel(base[4][s], one[4][0]) < TOL[dtype]
+        for x in (base[0], base[2], base[3], base[4]):
+            assert not x[:11].any() and not x[cu[-1]:].any()
+        # dtable of every sequence for itself, in 64 bits
+        for b, n in enumerate(lens):
+            if n:
+                s = slice(cu[b], cu[b] + n)
+                total += passes(q[None, s], k[None, s], v[None, s], table.float(), lut, dout[None, s], causal=causal,
+                                key_mask=None if mask is None else mask[None, s])[5].to(F64)
+        assert rel(base[5], total) < 2 * TOL[dtype]
+
+
+def test_packed_batch_of_many_sequences(dev):
+    """2048 sequences in 131072 tokens without a hint"""
+    B, n, H, D = 2048, 64, 12, 16
+    q, k, v, table, lut, dout = make(dev, torch.bfloat16, B, n, n, H, H, D, fused=True)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev) * n
+    a = passes(q, k, v, table, lut, dout)
+    free = torch.cuda.max_memory_allocated(dev)
+    torch.cuda.reset_peak_memory_stats(dev)
+    b = passes(*(x.flatten(0, 1) for x in (q, k, v)), table, lut, dout.flatten(0, 1), cu_q=cu, cu_k=cu)
+    print("peak", free >> 20, torch.cuda.max_memory_allocated(dev) >> 20, flush=True)
+    assert torch.equal(b[0], a[0].flatten(0, 1)) and all(torch.equal(b[i], a[i].flatten(0, 1)) for i in (2, 3, 4)) and rel(b[5], a[5]) < TOL[torch.bfloat16]
