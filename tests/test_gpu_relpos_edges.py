@@ -275,3 +275,54 @@ def test_packed_batch_of_many_sequences(dev):
     b = passes(*(x.flatten(0, 1) for x in (q, k, v)), table, lut, dout.flatten(0, 1), cu_q=cu, cu_k=cu)
     print("peak", free >> 20, torch.cuda.max_memory_allocated(dev) >> 20, flush=True)
     assert torch.equal(b[0], a[0].flatten(0, 1)) and all(torch.equal(b[i], a[i].flatten(0, 1)) for i in (2, 3, 4)) and rel(b[5], a[5]) < TOL[torch.bfloat16]
+
+
+# ---- two 16-row tiles a wave (bf16), against the 64-bit oracle, dtable included
+TWO = [  # B, Lq, Lk, H, Hk, D
+    (12, 385, 385, 12, 12, 64), (20, 130, 130, 12, 12, 32), (40, 70, 70, 12, 12, 64), (8, 300, 300, 16, 16, 96), (8, 260, 411, 24, 12, 40), (5, 700, 700, 24, 12, 64),
+    (26, 1100, 100, 12, 12, 64)]
+
+
+def thresholds():
+    """grids of up to so many workgroups of two tiles take one: forward and dQ at D <= 64, beyond, dK / dV"""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "spokennlp_amd", "csrc", "relpos_launch.h")).read()
+    wide, narrow = re.search(r"rp_qt\(rp_wgs_of_two\(a\), a\.D > 64 \? (\d+) : (\d+), dtype\)", text).groups()
+    return int(narrow), int(wide), int(re.search(r"rp_qt\(rp_blocks_of_two\(a, a\.Lk, a\.Tk\) \* a\.kv_heads, (\d+), dtype\)", text).group(1))
+
+
+@pytest.mark.parametrize("shape", TWO)
+@pytest.mark.parametrize("how", ["plain", "causal", "ragged", "span 48", "span 200", "packed"])
+def test_two_tiles_a_wave(dev, shape, how):
+    """forward, dQ and (D <= 64) dK / dV with 32 rows a wave: whole and half empty blocks, blocks of few keys, heads dealt over workgroups, rows cut into pieces"""
+    print("CASE", shape, how, flush=True)
+    B, Lq, Lk, H, Hk, D = shape
+    narrow, wide, kv = thresholds()
+    assert -(-Lq // 128) * B * H > (narrow if D <= 64 else wide) and (D > 64 or -(-Lk // 128) * B * Hk > kv), "a shape for one tile"
+    span = int(how[5:]) if how.startswith("span") else 128
+    q, k, v, table, lut, dout = make(dev, torch.bfloat16, *shape, max_distance=span, bidirectional=how != "causal", fused=Lq == Lk)
+    opt = {}
+    if how == "causal":
+        opt = dict(causal=True, align_end=Lq < Lk)
+    elif how == "ragged":
+        opt = dict(k_lens=torch.tensor([max(1, Lk - 31 * b) for b in range(B)], dtype=torch.int32, device=dev),
+                   key_mask=torch.rand(B, Lk, generator=torch.Generator().manual_seed(4)).to(dev) < 0.8)
+    a = check(dev, q, k, v, table, lut, dout, **opt)
+    if how == "packed":
+        cq, ck = (torch.arange(B + 1, dtype=torch.int32, device=dev) * n for n in (Lq, Lk))
+        p = passes(*(x.flatten(0, 1) for x in (q, k, v)), table, lut, dout.flatten(0, 1), cu_q=cq, cu_k=ck)
+        assert torch.equal(p[0], a[0].flatten(0, 1)) and torch.equal(p[1], a[1].transpose(0, 1).flatten(1)) and torch.equal(p[2], a[2].flatten(0, 1))
+        assert rel(p[3], a[3].flatten(0, 1)) < TOL[torch.bfloat16] and rel(p[4], a[4].flatten(0, 1)) < TOL[torch.bfloat16] and rel(p[5], a[5]) < TOL[torch.bfloat16]
+
+
+def test_spans_of_one_and_none_with_two_tiles(dev):
+    """the diagonal sums where the near band is narrower than a tile: span 0 (one bucket: no positions), 1 and 15 with an unordered map"""
+    ops = _ops()
+    q, k, v, _, _, dout = make(dev, torch.bfloat16, 12, 385, 385, 12, 12, 64)
+    table = torch.randn(5, 12, generator=torch.Generator().manual_seed(1)).to(dev)
+    for span in (1, 15):
+        lut = torch.randint(0, 5, (2 * span + 1,), generator=torch.Generator().manual_seed(span)).int().to(dev)
+        check(dev, q, k, v, table, lut, dout, causal=span == 15)
+    check(dev, q, k, v, table, torch.zeros(1, dtype=torch.int32, device=dev) + 2, dout, one_bucket=True)
+    assert ops.relpos_bias_fwd(table, lut, 3, 3).shape == (12, 3, 3)
