@@ -343,10 +343,11 @@ __device__ __forceinline__ float rp_table(const RpArgs& a, int bk, int h) {
 // digits left: q . k vanishes beside 1e9, and exp2(s - lse) in backward is off by the rounding of lse (2^-24 of it; 2^-10 at most here).  Infinities stay.
 #define RP_HUGE 16384.f
 #define RP_DOUBLING 128.f
-__device__ __forceinline__ float rp_entry(const RpArgs& a, int bk, int h) {
-    const float t = rp_table(a, bk, h), x = fabsf(t);
+__device__ __forceinline__ float rp_entry(float t) {
+    const float x = fabsf(t);
     return x > RP_HUGE && x < INFINITY ? copysignf(RP_HUGE + RP_DOUBLING * __builtin_amdgcn_logf(x * (1.f / RP_HUGE)), t) : t;
 }
+__device__ __forceinline__ float rp_entry(const RpArgs& a, int bk, int h) { return rp_entry(rp_table(a, bk, h)); }
 struct RpTable {
     int bk[2], n, mid, sign, tid;
     __device__ __forceinline__ int map(const RpArgs& a, int x) const { return a.map[rp_clamp(sign * (x - mid), -a.span, a.span) + a.span]; }

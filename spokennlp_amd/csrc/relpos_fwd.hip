@@ -271,10 +271,18 @@ __global__ __launch_bounds__(256, DT * sizeof(T) >= 32 ? 1 : 2) void rp_few_kern
             for (int f = 0; f < 4; ++f)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) bk[f][r] = a.map[rp_clamp(rel0 + 16 * f + r, -a.span, a.span) + a.span];
+            bool huge = false;
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[f][r] = rp_entry(a, bk[f][r], h) * inv;
+                for (int r = 0; r < 4; ++r) { z[f][r] = rp_table(a, bk[f][r], h); huge |= fabsf(z[f][r]) > RP_HUGE; }
+            if (__any(huge))
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[f][r] = rp_entry(z[f][r]);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) z[f] *= inv;
         } else
 #pragma unroll
             for (int f = 0; f < 4; ++f) z[f] = (f32x4){0.f, 0.f, 0.f, 0.f};
