@@ -64,7 +64,7 @@ __global__ ATTN_FWD_BOUNDS void attn_fwd_kernel(AttnArgs a) {
     // Q as the B operand of S^T = K Q^T : lane holds Q[q][kk*32 + g*8 .. +8]
     // The softmax scale is folded into the Q fragments: exact for a power of two (head_dim 64: 1/8; scores bit-identical to scaling them
     // afterwards), one more bf16 rounding of q otherwise.  The additive key mask then starts the MFMA accumulators as it comes out of LDS --
-    // no mask / scale multiplies per chunk (8 packed multiplies of this VALU-bound loop)
+    // no mask / scale multiplies per chunk (16 multiplies of this VALU-bound loop)
     bf16x8 fq[2];
     {
         const bf16_t* qp = a.qkv + (tok0 + q) * a.H3 + h * HD;
@@ -194,7 +194,7 @@ __global__ ATTN_FWD_BOUNDS void attn_fwd_kernel(AttnArgs a) {
                 for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
         }
         const float m_use = (BAND && m_run == -INFINITY) ? 0.f : m_run;   // a row whose visited keys were all masked so far
-        // p = 2^(s * scale * log2e - m): packed fp32 fma (two scores per instruction), native 2^x, packed partial sums
+        // p = 2^(s * scale * log2e - m): one fma, native 2^x, partial sums two by two (plain instructions: the build rules out the packed fp32 ones)
         {
             const f32x2 sc2v = {sc2, sc2}, negm = {-m_use, -m_use};
             f32x2 ps2 = {0.f, 0.f};
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_bwd_dq_kernel(AttnArgs a) {
             for (int f2 = 0; f2 < 2; ++f2) {
                 const float4 m4 = mbc[hf * 2 + f2];
                 const f32x2 n2 = {nlse_s, nlse_s};
-                const f32x2 lo2 = (f32x2){m4.x, m4.y} + n2, hi2 = (f32x2){m4.z, m4.w} + n2;                  // packed add
+                const f32x2 lo2 = (f32x2){m4.x, m4.y} + n2, hi2 = (f32x2){m4.z, m4.w} + n2;
                 sacc4[hf * 2 + f2] = (f32x4){lo2.x, lo2.y, hi2.x, hi2.y};
                 pacc4[hf * 2 + f2] = (f32x4){0.f, 0.f, 0.f, 0.f};
             }
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_bwd_dkv_kernel(AttnArgs a) {
             for (int f2 = 0; f2 < 2; ++f2) {
                 const float4 l4 = lsc[hf * 2 + f2];
                 const f32x2 m2 = {mbs, mbs};
-                const f32x2 lo2 = m2 - (f32x2){l4.x, l4.y}, hi2 = m2 - (f32x2){l4.z, l4.w};                  // packed add
+                const f32x2 lo2 = m2 - (f32x2){l4.x, l4.y}, hi2 = m2 - (f32x2){l4.z, l4.w};
                 sacc4[hf * 2 + f2] = (f32x4){lo2.x, lo2.y, hi2.x, hi2.y};
                 pacc4[hf * 2 + f2] = (f32x4){0.f, 0.f, 0.f, 0.f};
             }

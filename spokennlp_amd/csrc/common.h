@@ -129,7 +129,8 @@ __device__ __forceinline__ float gelu_grad_fast(float x) {
     const float er = erf_as_from_e(fabsf(x) * 0.70710678118654752f, e);
     return 0.5f * (1.0f + copysignf(er, x)) + x * 0.39894228040143268f * e;
 }
-// Two elements at a time on the packed-fp32 VALU ops (v_pk_mul/add/fma_f32): the GELU epilogues are VALU-bound -- at K = 768 the
+// Two elements at a time, in plain instructions (the build rules out v_pk_mul / add / fma_f32, for which this form was made and measured; the step
+// of bert-base took 12.70 ms with either): the GELU epilogues are VALU-bound -- at K = 768 the
 // ~25 VALU slots per element of the scalar form cost MORE SIMD time than the 1536 MFMA flops of the element (ablation: 25.6 us
 // of the 114 us FFN-up GEMM, 16.5 us of its GELU' backward).  Same formula and constants as gelu_fast / gelu_grad_fast:
 //   gelu(x)  = h + |h| (1 - q),  gelu'(x) = 1/2 + s (1 - q) + x e / sqrt(2 pi),   h = x/2, s = copysign(1/2, x),
@@ -212,7 +213,7 @@ __device__ __forceinline__ void gelu_both2(f32x2 x, f32x2& h, f32x2& d) {
 #endif
 }
 // ... with the derivative already in the units of its one-byte code (gemm_epi.h: q = round(gelu' * 200 + 27)): the scale rides the polynomial's
-// constants and the offset the final sum, one packed fma in place of two scalar multiply-adds per pair (the epilogue that calls this is VALU time)
+// constants and the offset the final sum, one fma in place of two multiply-adds an element (the epilogue that calls this is VALU time)
 __device__ __forceinline__ void gelu_both2q(f32x2 x, f32x2& h, f32x2& dq, float scale, float off) {
 #ifndef AMDSEG_GELU_ERF_EPILOGUE
     f32x2 r, x2c;
@@ -264,7 +265,7 @@ __device__ __forceinline__ void gelu_tanh_both(float x, float& h, float& d) {
 // act: 0 = exact (erf) GELU, 1 = gelu_new; wave-uniform
 __device__ __forceinline__ float gelu_act(float x, int act) { return act ? gelu_tanh_fast(x) : gelu_fast(x); }
 __device__ __forceinline__ float gelu_grad_act(float x, int act) { return act ? gelu_tanh_grad_fast(x) : gelu_grad_fast(x); }
-// four values of one accumulator fragment at a time (the erf form runs on the packed ops)
+// four values of one accumulator fragment at a time (the erf form two by two)
 __device__ __forceinline__ void gelu_act4(float* v, int act) {
     if (act) {
 #pragma unroll

@@ -5,7 +5,8 @@
 // query rows of every head of its group (dk, dv, the sums for dtable).  Seven products instead of the five of the formulas; results do not depend on
 // any order of arrival.
 // Bound by vector issue beside the products (0.55 .. 0.6 and 0.36 of the cycles; two waves a SIMD, which overlap them only in part), no LDS conflicts.  12 heads,
-// D = 64, bf16: 32 x 512 dQ 74 us, dK / dV 105 us (table sums 5 + 5); 4 x 4096 409 .. 426 and 545 us, 750 TFLOP/s of the executed products together.
+// D = 64, bf16, no mask: 32 x 512 dQ 73 us, dK / dV 99 us (88 without the table's gradient; table sums 5 + 5); 4 x 4096 407 and 527 us, 770 TFLOP/s of the
+// executed products together.  256 x 64 53 and 66, fp32 4 x 1024 at D = 128 370 and 489.
 //
 // delta.  sum_j ds_ij = 0, so a bucket that holds most of a row's probability has for its gradient what is left of a cancellation; delta taken from the
 // bf16 `out` is off by up to 2^-8 of it, the same way for every element of the row (1 % of dtable measured, 40 queries against 3 .. 1500 keys).  What the
@@ -21,7 +22,7 @@
 // by r lanes inside its 16 (a DPP operand modifier of the add itself) puts equal rel into equal lanes: the 16 x 16 tiles of one block diagonal add
 // up in one register per lane, the lanes that fall off the end belong to the next block diagonal's register.  7 adds per 4 elements, no LDS; the registers
 // live on from chunk to chunk until no later tile reaches their rel, and each sum is STORED once into the wave's own LDS bins (with ds_add_f32 instead,
-// four a chunk, the kernel took 141 us instead of 105 at 32 x 512: LDS float atomics).  Chunks beyond the span add into one register per side instead (one add per element).
+// four a chunk, the kernel took 141 us against 107 at 32 x 512: LDS float atomics).  Chunks beyond the span add into one register per side instead (one add per element).
 #include "relpos.h"
 #include "relpos_launch.h"
 

@@ -4,8 +4,8 @@
 // One workgroup = 4 waves x QT * 16 query rows of one (sequence, head); the keys stream through LDS in chunks of 64 with an online softmax.  S^T = K Q^T
 // keeps a query in a lane (its maximum and sum are lane scalars, the probabilities are the second operand of O^T += V^T P^T as they stand).
 // Bound by vector issue around the exponential, not by the products: a score costs its fma, its quarter-rate exponential, its share of maximum, sum and
-// conversion against 4 D / 256 matrix cycles.  12 heads, D = 64, bf16: 32 x 512 54 us (300 TFLOP/s, a third of it prologues and stores of 1536 workgroups),
-// 4 x 4096 322 us (640 TFLOP/s), 1 x 16384 1.0 ms (820 TFLOP/s).
+// conversion against 4 D / 256 matrix cycles.  12 heads, D = 64, bf16, no mask, both products of every pair
+// counted: 32 x 512 55 us (470 TFLOP/s, a third of it prologues and stores of 1536 workgroups), 4 x 4096 323 us (640), 1 x 16384 1.0 ms (820).
 #include "relpos.h"
 #include "relpos_launch.h"
 
