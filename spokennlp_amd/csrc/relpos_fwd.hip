@@ -442,6 +442,7 @@ static int rp_fwd_launch(const RpArgs& a, hipStream_t s) {
     if (rc) return rc;
     const int64_t n = (int64_t)a.nmain * a.nsplit + (a.zero_tail ? RP_TAIL_WGS : 0);
     if (a.nmain < 0 || n > RP_MAX_WGS) return AMDSEG_ERR_SHAPE;
+    if (n == 0) return 0;                                   // (no sequence, and the rows outside stay as they are)
     hipLaunchKernelGGL((rp_fwd_kernel<T, DT, QT>), dim3((unsigned)n), dim3(256), lds, s, a);
     const int rc2 = amdseg_launch_status();
     return rc2 ? rc2 : rp_join_launch<T>(a, s);

@@ -277,6 +277,24 @@ def test_packed_batch_of_many_sequences(dev):
     assert torch.equal(b[0], a[0].flatten(0, 1)) and all(torch.equal(b[i], a[i].flatten(0, 1)) for i in (2, 3, 4)) and rel(b[5], a[5]) < TOL[torch.bfloat16]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_sequence_into_given_outputs(dev, dtype):
+    """offsets of no sequence, outputs given: nothing to launch, everything stays; and sequences of queries without keys, of keys without queries"""
+    ops = _ops()
+    q, k, v, table, lut, dout = (x[0] if x.dim() == 4 else x for x in make(dev, dtype, 1, 90, 90, 4, 2, 64))
+    cu = torch.zeros(1, dtype=torch.int32, device=dev)
+    mine = torch.full_like(q, 7.0)
+    assert ops.relpos_attn_fwd(q, k, v, table, lut, cu_q=cu, cu_k=cu, out=mine)[0] is mine and bool((mine == 7).all())
+    none, all_ = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 0, 0], [0, 50, 90]))
+    for many in (False, True):                              # (two sequences, and more than 64)
+        if many:
+            none, all_ = none[:1].expand(101).contiguous(), torch.cat([all_[:1].expand(50), all_[1:2].expand(30), all_[2:].expand(21)]).contiguous()
+        a = passes(q[:0], k, v, table, lut, dout[:0], cu_q=none, cu_k=all_)
+        assert a[0].shape[0] == 0 and not a[3].any() and not a[4].any() and not a[5].any() and bool(torch.isfinite(a[5]).all())
+        a = passes(q, k[:0], v[:0], table, lut, dout, cu_q=all_, cu_k=none)
+        assert not a[0].any() and bool((a[1] == -math.inf).all()) and not a[2].any() and not a[5].any()
+
+
 # ---- two 16-row tiles a wave (bf16), against the 64-bit oracle, dtable included
 TWO = [  # B, Lq, Lk, H, Hk, D
     (12, 385, 385, 12, 12, 64), (20, 130, 130, 12, 12, 32), (40, 70, 70, 12, 12, 64), (8, 300, 300, 16, 16, 96), (8, 260, 411, 24, 12, 40), (5, 700, 700, 24, 12, 64),
