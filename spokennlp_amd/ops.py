@@ -695,7 +695,9 @@ def relpos_attn_fwd(q, k, v, table, bucket_map, scale=None, key_mask=None, k_len
     Padded: q [B, Lq, heads, D], k / v [B, Lk, kv_heads, D] (any strides with a contiguous last dimension and rows on 16 bytes: column blocks of a fused
     projection, a cache), k_lens int32 [B] = keys held, key_mask bool / uint8 [B, Lk].  Packed: q [tokens, heads, D], cu_q / cu_k int32 [B + 1],
     max_q / max_k = longest sequence (hints that change no result; max_k saves time with a key mask), key_mask [tokens].  bf16 or fp32; table [buckets, heads] of either; scale: D ** -0.5.
-    Query i stands at position i, or (align_end) so that the last query stands at the last key.  A row that sees no key: zero, lse -inf.
+    Query i stands at position i, or (align_end) so that the last query stands at the last key.  A row that sees no key: zero, lse -inf, no gradient.
+    K / V rows that no query sees (masked, behind the keys held, with causal behind the last query) and q / dout of rows that see no key may hold anything;
+    finite table entries may have any size (include/amdseg.h says how large ones count).
     Returns (out, lse); lse fp32 [B, heads, Lq] / [heads, tokens], None unless need_lse.  `out`: rows outside every packed sequence are left as they were
     (a fresh tensor has zeros there)."""
     def more(c, _):

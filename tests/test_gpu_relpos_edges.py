@@ -295,6 +295,29 @@ def test_no_sequence_into_given_outputs(dev, dtype):
         assert not a[0].any() and bool((a[1] == -math.inf).all()) and not a[2].any() and not a[5].any()
 
 
+@pytest.mark.parametrize("seed", range(3))
+def test_bad_offsets_of_many_sequences_stay_inside(dev, seed):
+    """100 sequences whose offsets run backwards, past the buffers and below zero: clamped on the device, some rows are wrong, none outside is touched"""
+    ops = _ops()
+    T = 700
+    q, k, v, table, lut, dout = (x[0] if x.dim() == 4 else x for x in make(dev, torch.bfloat16, 1, T, T, 4, 2, 64, seed=seed))
+    g = torch.Generator().manual_seed(seed)
+    cu = torch.randint(-300, T + 900, (101,), generator=g).int()
+    cu[7], cu[50] = -(1 << 31), (1 << 31) - 1
+    if seed:
+        cu = cu.sort().values if seed == 1 else cu.sort(descending=True).values
+    cu = cu.to(dev)
+    guard = [torch.full((3 * T,) + x.shape[1:], 7.0, dtype=x.dtype, device=dev) for x in (q, q, k, v)]
+    for causal in (False, True):
+        _, lse = ops.relpos_attn_fwd(q, k, v, table, lut, cu_q=cu, cu_k=cu, out=guard[0][T:2 * T], causal=causal)
+        lse = torch.nan_to_num(lse, neginf=0.0)
+        dt = ops.relpos_attn_bwd(q, k, v, table, lut, torch.zeros_like(q), dout, lse, cu_q=cu, cu_k=cu, dq=guard[1][T:2 * T], dk=guard[2][T:2 * T], dv=guard[3][T:2 * T],
+                                 causal=causal)[3]
+        assert dt.shape == table.shape
+        for x in guard:
+            assert bool((x[:T] == 7).all()) and bool((x[2 * T:] == 7).all())
+
+
 # ---- two 16-row tiles a wave (bf16), against the 64-bit oracle, dtable included
 TWO = [  # B, Lq, Lk, H, Hk, D
     (12, 385, 385, 12, 12, 64), (20, 130, 130, 12, 12, 32), (40, 70, 70, 12, 12, 64), (8, 300, 300, 16, 16, 96), (8, 260, 411, 24, 12, 40), (5, 700, 700, 24, 12, 64),
